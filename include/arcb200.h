@@ -468,6 +468,53 @@ int arcb_op_decode_attention_static(const void* d_q16, const void* d_k, const vo
                                     const uint8_t* d_item_skip, int32_t n_items, int32_t n_heads,
                                     int32_t t_max, int32_t n_splits, int32_t act_format, void* stream);
 
+/* Attention of query items that share cached rows: samples of one prompt, requests behind one preamble, draft tokens of a
+ * sequence.  Item i of group g attends rows [0, d_group_len[g]) of cache row d_group_seq[g], which all items of the group
+ * share and which are read once for them, and rows [d_item_begin[i], d_item_end[i]) of cache row d_item_seq[i], its own:
+ *   out[i][h] = softmax(scale * q[i][h] K^T) V   over both, K and V of head h / (n_heads / n_kv).
+ * An item that sees no row, or is skipped, gets zeros.  No counterpart in the reference, whose samples of a prompt each keep
+ * and read a copy of it (src/inference.py:794-827).
+ *   formats: queries and outputs in act_format, cache in kv_format; the two are equal, or half over a bfloat16 cache.
+ *   Scores, maxima and sums are 32 bits; heads of 64 or 128.
+ *   Arrays start on 16 bytes.  max_* are upper bounds the work is laid out for (0: n_items, t_max, t_max); more items in a
+ *   group than max_group is an error, longer rows only cost time.
+ *   d_status (optional): set to ARCB_DEV_BAD_INDEX's value, 4, where a group or an item names rows outside the cache, or the
+ *   groups do not cover the items one after the other; such rows count as not there. */
+typedef struct arcb_prefix_attention_args {
+  const void* d_q;               /* item i, head h: dim values at d_q + i * q_pitch + h * dim         */
+  const void* d_k;               /* [n_seqs][n_kv][t_max][dim]                                        */
+  const void* d_v;
+  void* d_out;                   /* [n_items][n_heads][dim]                                           */
+  const int32_t* d_group_first;  /* [n_groups + 1] items of group g: [first[g], first[g + 1]); 0 ... n_items */
+  const int32_t* d_group_seq;    /* [n_groups]                                                        */
+  const int32_t* d_group_len;    /* [n_groups]                                                        */
+  const int32_t* d_item_seq;     /* [n_items], NULL: the item's number                                */
+  const int32_t* d_item_begin;   /* [n_items], NULL: 0                                                */
+  const int32_t* d_item_end;     /* [n_items], NULL: no item has rows of its own                      */
+  const uint8_t* d_item_skip;    /* optional [n_items]                                                */
+  int32_t* d_status;             /* optional                                                          */
+  void* d_scratch;               /* >= arcb_prefix_attention_scratch_bytes(args)                      */
+  int64_t scratch_bytes;
+  int64_t q_pitch;               /* elements, 0: n_heads * dim                                        */
+  int32_t n_groups, n_items, n_heads, n_kv, dim, n_seqs, t_max;
+  int32_t max_group, max_prefix, max_own;
+  float scale;
+  int32_t act_format, kv_format; /* ARCB_ACT_*                                                        */
+  int32_t reserved;
+} arcb_prefix_attention_args;
+
+/* Reads the sizes and formats, and whether d_item_end is set; < 0: the error. */
+int64_t arcb_prefix_attention_scratch_bytes(const arcb_prefix_attention_args* args);
+int arcb_op_prefix_attention(const arcb_prefix_attention_args* args, void* stream);
+
+/* Copies rows between the sequences of a cache [n_planes][n_seqs][n_heads][t_max] of row_bytes bytes: h_copies[i] = (src, dst,
+ * begin, end) takes rows [begin, end) of every plane and head of sequence src to the same rows of sequence dst.  All rows are
+ * read before any is written, so that sequences may change places (forks, reordered beams, compactions in one call); a
+ * sequence is written by at most one copy.  h_copies is host memory and free to change when the call returns.  Nothing but the
+ * named rows is written.  No counterpart in the reference. */
+int arcb_op_cache_copy(void* d_cache, int32_t n_planes, int32_t n_seqs, int32_t n_heads, int32_t t_max, int32_t row_bytes,
+                       const int32_t* h_copies /* [n_copies][4] */, int32_t n_copies, void* stream);
+
 /* ln_f -> lm_head -> argmax (src/inference.py:418/424/459 + 574/611): logits fp32
  * [rows][14] and the index of the first maximum. d_row_index (optional) gathers rows of x. */
 int arcb_op_head(const float* d_x, const int32_t* d_row_index, const float* d_lnf_w,

@@ -46,7 +46,7 @@ EXPORTS = [
     "arcb_session_poll", "arcb_engine_saturation_count", "arcb_session_attention_probe", "arcb_launch_count", "arcb_op_rmsnorm", "arcb_op_gemm",
     "arcb_op_gemm_residual", "arcb_gemm_splitk_scratch_bytes", "arcb_op_gemm_residual_splitk",
     "arcb_attn_scratch_bytes", "arcb_op_decode_attention", "arcb_op_decode_attention_static",
-    "arcb_op_head", "arcb_build_prompts", "arcb_canonicalize_candidates", "arcb_pack_prompts", "arcb_mask_stats",
+    "arcb_op_head", "arcb_prefix_attention_scratch_bytes", "arcb_op_prefix_attention", "arcb_op_cache_copy", "arcb_build_prompts", "arcb_canonicalize_candidates", "arcb_pack_prompts", "arcb_mask_stats",
 ]
 STATIC_ATTN_MAX_RECORDS = 16384
 
@@ -152,6 +152,18 @@ class CandidateArgs(C.Structure):
     ]
 
 
+class PrefixAttentionArgs(C.Structure):
+    _fields_ = [
+        ("d_q", C.c_void_p), ("d_k", C.c_void_p), ("d_v", C.c_void_p), ("d_out", C.c_void_p),
+        ("d_group_first", C.c_void_p), ("d_group_seq", C.c_void_p), ("d_group_len", C.c_void_p),
+        ("d_item_seq", C.c_void_p), ("d_item_begin", C.c_void_p), ("d_item_end", C.c_void_p), ("d_item_skip", C.c_void_p),
+        ("d_status", C.c_void_p), ("d_scratch", C.c_void_p), ("scratch_bytes", C.c_int64), ("q_pitch", C.c_int64),
+        ("n_groups", C.c_int32), ("n_items", C.c_int32), ("n_heads", C.c_int32), ("n_kv", C.c_int32), ("dim", C.c_int32),
+        ("n_seqs", C.c_int32), ("t_max", C.c_int32), ("max_group", C.c_int32), ("max_prefix", C.c_int32), ("max_own", C.c_int32),
+        ("scale", C.c_float), ("act_format", C.c_int32), ("kv_format", C.c_int32), ("reserved", C.c_int32),
+    ]
+
+
 _lib = None
 
 
@@ -210,6 +222,10 @@ def load() -> C.CDLL:
     lib.arcb_attn_scratch_bytes.argtypes = [i32, i32, i32]
     lib.arcb_op_decode_attention.argtypes = [vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, vp, i32, vp]
     lib.arcb_op_decode_attention_static.argtypes = [vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, vp]
+    lib.arcb_prefix_attention_scratch_bytes.restype = i64
+    lib.arcb_prefix_attention_scratch_bytes.argtypes = [C.POINTER(PrefixAttentionArgs)]
+    lib.arcb_op_prefix_attention.argtypes = [C.POINTER(PrefixAttentionArgs), vp]
+    lib.arcb_op_cache_copy.argtypes = [vp, i32, i32, i32, i32, i32, vp, i32, vp]
     lib.arcb_op_head.argtypes = [vp, vp, vp, vp, vp, vp, i32, i32, f32, vp]
     _lib = lib
     return lib

@@ -1,0 +1,358 @@
+// Attention of queries that share cached rows (samples of one prompt, requests behind one preamble, draft tokens of a
+// sequence): o = softmax(scale q K^T) V over the rows of the item's group and the rows of its own.
+//
+// A softmax over a set of rows can be put together from parts: with m = max, l = sum exp(s - m), a = sum exp(s - m) v of every
+// part, the whole is sum_i a_i exp(m_i - m) / sum_i l_i exp(m_i - m), m = max m_i.  So the shared rows are gone through once for
+// all queries of a group that use a key head (items x rep rows), the own rows once an item, and a last kernel joins the parts.
+#include <cmath>
+
+#include "../../include/arcb200.h"
+#include "attn_prefix.cuh"
+#include "gemm.cuh"
+#include "launch.cuh"
+
+int arcb_fail(int code, const char* msg);
+int arcb_fail_cuda(cudaError_t e, const char* where);
+
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+// A CTA's part of the work: query rows (row r is item item0 + (r0 + r) / rep, head kvh * rep + (r0 + r) % rep), cached rows
+// [begin, end) of a sequence, and which part of the results it is.
+struct ApWork {
+  int item0, r0, rows, kvh, seq, begin, end, part;
+};
+
+// Numbers: tiles of one (group, head, range) follow each other, so that they find its rows in L2.
+__device__ __forceinline__ ApWork ap_work(const AttnPrefixArgs& a, long long w, int tile1, int tile2) {
+  ApWork k;
+  const long long n1 = (long long)a.n_groups * a.n_kv * a.plan.tiles1 * a.plan.splits1;
+  int len, at0, split, splits;
+  if (w < n1) {
+    const int t = (int)(w % a.plan.tiles1); w /= a.plan.tiles1;
+    splits = a.plan.splits1;
+    split = (int)(w % splits); w /= splits;
+    k.kvh = (int)(w % a.n_kv);
+    const int g = (int)(w / a.n_kv);
+    int first, last;
+    if (a.uniform > 0) {
+      first = g * a.uniform;
+      last = first + a.uniform;
+      k.seq = first;
+      len = a.group_len[first];
+    } else {
+      first = a.group_first[g];
+      last = a.group_first[g + 1];
+      k.seq = a.group_seq[g];
+      len = a.group_len[g];
+    }
+    const bool bad = first < 0 || last < first || last > a.n_items || last - first > a.max_group || len < 0 || len > a.t_max ||
+                     (len > 0 && (k.seq < 0 || k.seq >= a.n_seqs)) || (g == 0 && first != 0) || (g == a.n_groups - 1 && last != a.n_items);
+    if (bad) {
+      if (threadIdx.x == 0) arcb_set_error(a.status, ARCB_DEV_BAD_INDEX);
+      first = min(max(first, 0), a.n_items);
+      last = min(max(last, first), min(a.n_items, first + a.max_group));
+      len = 0;
+    }
+    k.item0 = first;
+    k.r0 = t * tile1;
+    k.rows = min(tile1, (last - first) * a.rep - k.r0);
+    at0 = 0;
+    k.part = split;
+  } else {
+    w -= n1;
+    splits = a.plan.splits2;
+    split = (int)(w % splits); w /= splits;
+    const int t = (int)(w % a.plan.tiles2); w /= a.plan.tiles2;
+    k.kvh = (int)(w % a.n_kv);
+    k.item0 = (int)(w / a.n_kv);
+    k.r0 = t * tile2;
+    k.rows = min(tile2, a.rep - k.r0);
+    k.seq = a.item_seq ? a.item_seq[k.item0] : k.item0;
+    at0 = a.item_begin ? a.item_begin[k.item0] : 0;
+    len = a.item_end[k.item0] - at0;
+    if (len > 0 && (at0 < 0 || at0 + len > a.t_max || k.seq < 0 || k.seq >= a.n_seqs)) {
+      if (threadIdx.x == 0) arcb_set_error(a.status, ARCB_DEV_BAD_INDEX);
+      len = 0;
+    }
+    if (len < 0 || (a.item_skip && a.item_skip[k.item0])) len = 0;
+    k.part = a.plan.splits1 + split;
+  }
+  int chunk = (len + splits - 1) / splits;
+  chunk = (chunk + 63) & ~63;
+  k.begin = at0 + min(split * chunk, len);
+  k.end = at0 + min((split + 1) * chunk, len);
+  return k;
+}
+
+__device__ __forceinline__ float* ap_record(const AttnPrefixArgs& a, long long ih, int part) {
+  return a.scratch + ((size_t)ih * a.plan.parts + part) * (a.dim + AP_PAD);
+}
+
+// Outputs saturate in half, as all of the library's do; NaN stays NaN.
+__device__ __forceinline__ void ap_store4(void* out, size_t at, float4 v, int fmt) {
+  if (fmt != 1 || !(isnan(v.x) || isnan(v.y) || isnan(v.z) || isnan(v.w))) {
+    st_act4(out, at, v, fmt);
+    return;
+  }
+  const float f[4] = {v.x, v.y, v.z, v.w};
+  for (int i = 0; i < 4; ++i) reinterpret_cast<__half*>(out)[at + i] = isnan(f[i]) ? __float2half_rn(f[i]) : __float2half_rn(fminf(fmaxf(f[i], -65504.f), 65504.f));
+}
+
+// ---- multiply-adds in 32 bits, for any format ----
+// Four warps of four query rows; 32 cached rows at a time in shared memory.  Scores: a lane has a cached row; sums: a lane has
+// every 32nd value column.
+constexpr int AS_ROWS = 16, AS_KEYS = 32;
+
+template <int D>
+__global__ void __launch_bounds__(128)
+attn_prefix_simple_kernel(AttnPrefixArgs a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  __shared__ __align__(16) float s_q[AS_ROWS][D];
+  __shared__ __align__(16) float s_k[AS_KEYS][D + 4];
+  __shared__ __align__(16) float s_v[AS_KEYS][D];
+  const int lane = threadIdx.x & 31, wj = threadIdx.x >> 5;
+  const ApWork w = ap_work(a, blockIdx.x, AS_ROWS, AS_ROWS);
+  if (w.rows <= 0) return;
+  for (int i = threadIdx.x; i < AS_ROWS * D / 4; i += 128) {
+    const int r = i / (D / 4), c = i % (D / 4) * 4;
+    float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (r < w.rows) {
+      const int R = w.r0 + r;
+      q = ld_act4(a.q, (size_t)(w.item0 + R / a.rep) * a.q_pitch + (size_t)(w.kvh * a.rep + R % a.rep) * D + c, a.act_fmt);
+    }
+    *reinterpret_cast<float4*>(&s_q[r][c]) = q;
+  }
+  const size_t row0 = ((size_t)w.seq * a.n_kv + w.kvh) * (size_t)a.t_max;
+  const float sc = a.scale * LOG2E;
+  float m[4], l[4], acc[4][D / 32];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) acc[r][i] = 0.f;
+  }
+  for (int t = w.begin; t < w.end; t += AS_KEYS) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < AS_KEYS * D / 4; i += 128) {
+      const int r = i / (D / 4), c = i % (D / 4) * 4;
+      float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
+      if (t + r < w.end) {
+        k = ld_act4(a.k, (row0 + t + r) * D + c, a.kv_fmt);
+        v = ld_act4(a.v, (row0 + t + r) * D + c, a.kv_fmt);
+      }
+      *reinterpret_cast<float4*>(&s_k[r][c]) = k;
+      *reinterpret_cast<float4*>(&s_v[r][c]) = v;
+    }
+    __syncthreads();
+    if (wj * 4 >= w.rows) continue;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int c = 0; c < D; c += 4) {
+      const float4 k = *reinterpret_cast<const float4*>(&s_k[lane][c]);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float4 q = *reinterpret_cast<const float4*>(&s_q[wj * 4 + r][c]);
+        s[r] = fmaf(q.x, k.x, s[r]);
+        s[r] = fmaf(q.y, k.y, s[r]);
+        s[r] = fmaf(q.z, k.z, s[r]);
+        s[r] = fmaf(q.w, k.w, s[r]);
+      }
+    }
+    float p[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      s[r] = t + lane < w.end ? s[r] * sc : -INFINITY;
+      float mx = s[r];
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      mx = fmaxf(mx, m[r]);
+      const float safe = mx == -INFINITY ? 0.f : mx;
+      const float alpha = exp2f(m[r] - safe);
+      m[r] = mx;
+      p[r] = exp2f(s[r] - safe);
+      l[r] = l[r] * alpha + p[r];
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) acc[r][i] *= alpha;
+    }
+    const int n = min(AS_KEYS, w.end - t);
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) {
+      float v[D / 32];
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) v[i] = s_v[j][lane + 32 * i];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float pr = __shfl_sync(0xffffffffu, p[r], j);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) acc[r][i] = fmaf(pr, v[i], acc[r][i]);
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int R = w.r0 + wj * 4 + r;
+    if (wj * 4 + r >= w.rows) break;
+    const int item = w.item0 + R / a.rep;
+    const long long ih = (long long)item * a.n_heads + w.kvh * a.rep + R % a.rep;
+    const float sum = warp_sum(l[r]);
+    if (a.plan.parts == 1) {
+      const bool none = sum == 0.f || (a.item_skip && a.item_skip[item]);
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        const float o = none ? 0.f : acc[r][i] / sum;
+        const size_t at = (size_t)ih * D + lane + 32 * i;
+        if (a.act_fmt == 1 && isnan(o)) reinterpret_cast<__half*>(a.out)[at] = __float2half_rn(o);
+        else st_act(a.out, at, o, a.act_fmt);
+      }
+    } else {
+      float* rec = ap_record(a, ih, w.part);
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) rec[lane + 32 * i] = acc[r][i];
+      if (lane == 0) {
+        rec[D] = m[r];
+        rec[D + 1] = sum;
+      }
+    }
+  }
+}
+
+// One warp per (item, head): joins the parts in order.  Lane s keeps the factors of parts s and s + 32.
+__global__ void __launch_bounds__(128)
+attn_prefix_join_kernel(AttnPrefixArgs a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const long long ih = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (ih >= (long long)a.n_items * a.n_heads) return;
+  const int n = a.plan.parts, rec = a.dim + AP_PAD;
+  const bool skip = a.item_skip && a.item_skip[ih / a.n_heads];
+  const float* r0 = a.scratch + (size_t)ih * n * rec;
+  float m_s[2], l_s[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int s = lane + 32 * i;
+    const float2 ml = s < n ? *reinterpret_cast<const float2*>(r0 + (size_t)s * rec + a.dim) : make_float2(-INFINITY, 0.f);
+    m_s[i] = ml.x;
+    l_s[i] = ml.y;
+  }
+  float m = fmaxf(m_s[0], m_s[1]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const float safe = m == -INFINITY ? 0.f : m;
+  const float f0 = exp2f(m_s[0] - safe), f1 = exp2f(m_s[1] - safe);
+  const float l = warp_sum(l_s[0] * f0 + l_s[1] * f1);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int c = lane * 4;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int s = 0; s < n; ++s) {
+    const float f = __shfl_sync(0xffffffffu, s < 32 ? f0 : f1, s & 31);
+    if (c < a.dim && f != 0.f) {        // an empty part's sums count for nothing, whatever they are
+      const float4 v = *reinterpret_cast<const float4*>(r0 + (size_t)s * rec + c);
+      o.x += v.x * f; o.y += v.y * f; o.z += v.z * f; o.w += v.w * f;
+    }
+  }
+  if (c < a.dim) {
+    if (skip) o = make_float4(0.f, 0.f, 0.f, 0.f);
+    else o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    ap_store4(a.out, (size_t)ih * a.dim + c, o, a.act_fmt);
+  }
+}
+
+void fill_plan(AttnPrefixArgs& a) {
+  a.rep = a.n_heads / a.n_kv;
+  a.plan = prefix_plan(a.n_groups, a.max_group, a.max_prefix, a.n_items, a.item_end ? a.max_own : 0, a.n_kv, a.rep, AS_ROWS, AS_ROWS, arcb_num_sms());
+}
+
+}  // namespace
+
+bool arcb_attn_prefix_supported(int n_heads, int n_kv, int dim, int act_fmt, int kv_fmt) {
+  return n_kv > 0 && n_heads > 0 && n_heads % n_kv == 0 && (dim == 64 || dim == 128) &&
+         (act_fmt == kv_fmt || (act_fmt == 1 && kv_fmt == 0));
+}
+
+long long arcb_attn_prefix_scratch(const AttnPrefixArgs& args) {
+  AttnPrefixArgs a = args;
+  fill_plan(a);
+  const int n = a.plan.parts;
+  return n > 1 ? (long long)a.n_items * a.n_heads * n * (a.dim + AP_PAD) * 4 : 0;
+}
+
+int arcb_launch_attn_prefix(AttnPrefixArgs a, cudaStream_t stream) {
+  if (a.n_items <= 0) return 0;
+  fill_plan(a);
+  const PrefixPlan& p = a.plan;
+  if (p.parts < 1 || (p.parts > 1 && !a.scratch)) return -1;
+  const long long blocks = (long long)a.n_groups * a.n_kv * p.tiles1 * p.splits1 + (long long)a.n_items * a.n_kv * p.tiles2 * p.splits2;
+  const long long joins = ((long long)a.n_items * a.n_heads + 3) / 4;
+  if (blocks > 0x7fffffffLL || joins > 0x7fffffffLL) return -1;
+  cudaError_t e = a.dim == 64 ? arcb_launch(attn_prefix_simple_kernel<64>, dim3((unsigned)blocks), dim3(128), 0, stream, a)
+                              : arcb_launch(attn_prefix_simple_kernel<128>, dim3((unsigned)blocks), dim3(128), 0, stream, a);
+  arcb_count_launch(1);
+  if (e == cudaSuccess && p.parts > 1) {
+    e = arcb_launch(attn_prefix_join_kernel, dim3((unsigned)joins), dim3(128), 0, stream, a);
+    arcb_count_launch(1);
+  }
+  return (int)e;
+}
+
+static int to_fmt(int act_format) { return act_format == ARCB_ACT_F16 ? 1 : act_format == ARCB_ACT_BF16 ? 0 : 2; }
+
+// Checks and converts; the message says what is wrong.
+static int prefix_args(const arcb_prefix_attention_args* p, AttnPrefixArgs& a, bool sizes_only) {
+  if (!p) return arcb_fail(ARCB_E_ARG, "null argument");
+  if (p->n_items <= 0 || p->n_heads <= 0 || p->n_kv <= 0 || p->n_seqs <= 0 || p->t_max <= 0 || p->n_groups < 0)
+    return arcb_fail(ARCB_E_ARG, "bad prefix attention sizes");
+  if (p->n_heads % p->n_kv) return arcb_fail(ARCB_E_ARG, "n_kv must divide n_heads");
+  if (p->act_format < ARCB_ACT_F16 || p->act_format > ARCB_ACT_F32 || p->kv_format < ARCB_ACT_F16 || p->kv_format > ARCB_ACT_F32)
+    return arcb_fail(ARCB_E_ARG, "unknown act_format or kv_format");
+  a.act_fmt = to_fmt(p->act_format);
+  a.kv_fmt = to_fmt(p->kv_format);
+  if (!arcb_attn_prefix_supported(p->n_heads, p->n_kv, p->dim, a.act_fmt, a.kv_fmt))
+    return arcb_fail(ARCB_E_UNSUPPORTED, "prefix attention: heads of 64 or 128, queries in the cache's format or half over a bfloat16 cache");
+  if (!(std::fabs(p->scale) <= 3.0e38f)) return arcb_fail(ARCB_E_ARG, "scale must be finite");
+  a.n_groups = p->n_groups; a.n_items = p->n_items; a.n_heads = p->n_heads; a.n_kv = p->n_kv; a.dim = p->dim; a.n_seqs = p->n_seqs; a.t_max = p->t_max;
+  auto bound = [](int v, int most) { return v <= 0 || v > most ? most : v; };
+  a.max_group = bound(p->max_group, p->n_items);
+  a.max_prefix = bound(p->max_prefix, p->t_max);
+  a.max_own = bound(p->max_own, p->t_max);
+  a.item_end = p->d_item_end;
+  if (!p->n_groups && !p->d_item_end) return arcb_fail(ARCB_E_ARG, "prefix attention needs groups, rows of the items' own, or both");
+  if (sizes_only) return ARCB_OK;
+  if (!p->d_q || !p->d_k || !p->d_v || !p->d_out) return arcb_fail(ARCB_E_ARG, "null attention argument");
+  if (p->n_groups && (!p->d_group_first || !p->d_group_seq || !p->d_group_len)) return arcb_fail(ARCB_E_ARG, "null group arrays");
+  const long long pitch = p->q_pitch ? p->q_pitch : (long long)p->n_heads * p->dim;
+  const int es = a.act_fmt == 2 ? 4 : 2;
+  if (pitch < 0 || (pitch * es) % 16) return arcb_fail(ARCB_E_ARG, "q_pitch must be a multiple of 16 bytes");
+  if ((reinterpret_cast<uintptr_t>(p->d_q) | reinterpret_cast<uintptr_t>(p->d_k) | reinterpret_cast<uintptr_t>(p->d_v) |
+       reinterpret_cast<uintptr_t>(p->d_out) | reinterpret_cast<uintptr_t>(p->d_scratch)) % 16)
+    return arcb_fail(ARCB_E_ARG, "attention arrays must be aligned to 16 bytes");
+  a.q = p->d_q; a.q_pitch = pitch; a.k = p->d_k; a.v = p->d_v; a.out = p->d_out;
+  a.group_first = p->d_group_first; a.group_seq = p->d_group_seq; a.group_len = p->d_group_len;
+  a.item_seq = p->d_item_seq; a.item_begin = p->d_item_begin; a.item_skip = p->d_item_skip;
+  a.scale = p->scale; a.scratch = reinterpret_cast<float*>(p->d_scratch); a.status = p->d_status;
+  return ARCB_OK;
+}
+
+extern "C" int64_t arcb_prefix_attention_scratch_bytes(const arcb_prefix_attention_args* p) {
+  AttnPrefixArgs a{};
+  const int r = prefix_args(p, a, true);
+  return r ? r : arcb_attn_prefix_scratch(a);
+}
+
+extern "C" int arcb_op_prefix_attention(const arcb_prefix_attention_args* p, void* stream) {
+  AttnPrefixArgs a{};
+  const int r = prefix_args(p, a, false);
+  if (r) return r;
+  const long long need = arcb_attn_prefix_scratch(a);
+  if (need > 0 && (!p->d_scratch || p->scratch_bytes < need))
+    return arcb_fail(ARCB_E_ARG, "scratch is smaller than arcb_prefix_attention_scratch_bytes");
+  const int e = arcb_launch_attn_prefix(a, (cudaStream_t)stream);
+  if (e > 0) return arcb_fail_cuda((cudaError_t)e, "prefix attention");
+  if (e < 0) return arcb_fail(ARCB_E_ARG, "prefix attention: too much work for one call");
+  return ARCB_OK;
+}
