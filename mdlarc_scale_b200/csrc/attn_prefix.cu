@@ -7,7 +7,7 @@
 #include <cmath>
 
 #include "../../include/arcb200.h"
-#include "attn_prefix.cuh"
+#include "attn_prefix_impl.cuh"
 #include "gemm.cuh"
 #include "launch.cuh"
 
@@ -16,91 +16,7 @@ int arcb_fail_cuda(cudaError_t e, const char* where);
 
 namespace {
 
-constexpr float LOG2E = 1.4426950408889634f;
-
-// A CTA's part of the work: query rows (row r is item item0 + (r0 + r) / rep, head kvh * rep + (r0 + r) % rep), cached rows
-// [begin, end) of a sequence, and which part of the results it is.
-struct ApWork {
-  int item0, r0, rows, kvh, seq, begin, end, part;
-};
-
-// Numbers: tiles of one (group, head, range) follow each other, so that they find its rows in L2.
-__device__ __forceinline__ ApWork ap_work(const AttnPrefixArgs& a, long long w, int tile1, int tile2) {
-  ApWork k;
-  const long long n1 = (long long)a.n_groups * a.n_kv * a.plan.tiles1 * a.plan.splits1;
-  int len, at0, split, splits;
-  if (w < n1) {
-    const int t = (int)(w % a.plan.tiles1); w /= a.plan.tiles1;
-    splits = a.plan.splits1;
-    split = (int)(w % splits); w /= splits;
-    k.kvh = (int)(w % a.n_kv);
-    const int g = (int)(w / a.n_kv);
-    int first, last;
-    if (a.uniform > 0) {
-      first = g * a.uniform;
-      last = first + a.uniform;
-      k.seq = first;
-      len = a.group_len[first];
-    } else {
-      first = a.group_first[g];
-      last = a.group_first[g + 1];
-      k.seq = a.group_seq[g];
-      len = a.group_len[g];
-    }
-    const bool bad = first < 0 || last < first || last > a.n_items || last - first > a.max_group || len < 0 || len > a.t_max ||
-                     (len > 0 && (k.seq < 0 || k.seq >= a.n_seqs)) || (g == 0 && first != 0) || (g == a.n_groups - 1 && last != a.n_items);
-    if (bad) {
-      if (threadIdx.x == 0) arcb_set_error(a.status, ARCB_DEV_BAD_INDEX);
-      first = min(max(first, 0), a.n_items);
-      last = min(max(last, first), min(a.n_items, first + a.max_group));
-      len = 0;
-    }
-    k.item0 = first;
-    k.r0 = t * tile1;
-    k.rows = min(tile1, (last - first) * a.rep - k.r0);
-    at0 = 0;
-    k.part = split;
-  } else {
-    w -= n1;
-    splits = a.plan.splits2;
-    split = (int)(w % splits); w /= splits;
-    const int t = (int)(w % a.plan.tiles2); w /= a.plan.tiles2;
-    k.kvh = (int)(w % a.n_kv);
-    k.item0 = (int)(w / a.n_kv);
-    k.r0 = t * tile2;
-    k.rows = min(tile2, a.rep - k.r0);
-    k.seq = a.item_seq ? a.item_seq[k.item0] : k.item0;
-    at0 = a.item_begin ? a.item_begin[k.item0] : 0;
-    len = a.item_end[k.item0] - at0;
-    if (len > 0 && (at0 < 0 || at0 + len > a.t_max || k.seq < 0 || k.seq >= a.n_seqs)) {
-      if (threadIdx.x == 0) arcb_set_error(a.status, ARCB_DEV_BAD_INDEX);
-      len = 0;
-    }
-    if (len < 0 || (a.item_skip && a.item_skip[k.item0])) len = 0;
-    k.part = a.plan.splits1 + split;
-  }
-  int chunk = (len + splits - 1) / splits;
-  chunk = (chunk + 63) & ~63;
-  k.begin = at0 + min(split * chunk, len);
-  k.end = at0 + min((split + 1) * chunk, len);
-  return k;
-}
-
-__device__ __forceinline__ float* ap_record(const AttnPrefixArgs& a, long long ih, int part) {
-  return a.scratch + ((size_t)ih * a.plan.parts + part) * (a.dim + AP_PAD);
-}
-
-// Outputs saturate in half, as all of the library's do; NaN stays NaN.
-__device__ __forceinline__ void ap_store4(void* out, size_t at, float4 v, int fmt) {
-  if (fmt != 1 || !(isnan(v.x) || isnan(v.y) || isnan(v.z) || isnan(v.w))) {
-    st_act4(out, at, v, fmt);
-    return;
-  }
-  const float f[4] = {v.x, v.y, v.z, v.w};
-  for (int i = 0; i < 4; ++i) reinterpret_cast<__half*>(out)[at + i] = isnan(f[i]) ? __float2half_rn(f[i]) : __float2half_rn(fminf(fmaxf(f[i], -65504.f), 65504.f));
-}
-
-// ---- multiply-adds in 32 bits, for any format ----
+// ---- 32-bit formats: multiply-adds ----
 // Four warps of four query rows; 32 cached rows at a time in shared memory.  Scores: a lane has a cached row; sums: a lane has
 // every 32nd value column.
 constexpr int AS_ROWS = 16, AS_KEYS = 32;
@@ -114,7 +30,7 @@ attn_prefix_simple_kernel(AttnPrefixArgs a) {
   __shared__ __align__(16) float s_k[AS_KEYS][D + 4];
   __shared__ __align__(16) float s_v[AS_KEYS][D];
   const int lane = threadIdx.x & 31, wj = threadIdx.x >> 5;
-  const ApWork w = ap_work(a, blockIdx.x, AS_ROWS, AS_ROWS);
+  const ApWork w = ap_work(a, blockIdx.x);
   if (w.rows <= 0) return;
   for (int i = threadIdx.x; i < AS_ROWS * D / 4; i += 128) {
     const int r = i / (D / 4), c = i % (D / 4) * 4;
@@ -126,7 +42,7 @@ attn_prefix_simple_kernel(AttnPrefixArgs a) {
     *reinterpret_cast<float4*>(&s_q[r][c]) = q;
   }
   const size_t row0 = ((size_t)w.seq * a.n_kv + w.kvh) * (size_t)a.t_max;
-  const float sc = a.scale * LOG2E;
+  const float sc = a.scale * AP_LOG2E;
   float m[4], l[4], acc[4][D / 32];
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
@@ -265,7 +181,7 @@ attn_prefix_join_kernel(AttnPrefixArgs a) {
 
 void fill_plan(AttnPrefixArgs& a) {
   a.rep = a.n_heads / a.n_kv;
-  a.plan = prefix_plan(a.n_groups, a.max_group, a.max_prefix, a.n_items, a.item_end ? a.max_own : 0, a.n_kv, a.rep, AS_ROWS, AS_ROWS, arcb_num_sms());
+  a.plan = prefix_plan(a.n_groups, a.max_group, a.max_prefix, a.n_items, a.item_end ? a.max_own : 0, a.n_kv, a.rep, a.kv_fmt == 2 ? AS_ROWS : 64, arcb_num_sms());
 }
 
 }  // namespace
@@ -290,7 +206,8 @@ int arcb_launch_attn_prefix(AttnPrefixArgs a, cudaStream_t stream) {
   const long long blocks = (long long)a.n_groups * a.n_kv * p.tiles1 * p.splits1 + (long long)a.n_items * a.n_kv * p.tiles2 * p.splits2;
   const long long joins = ((long long)a.n_items * a.n_heads + 3) / 4;
   if (blocks > 0x7fffffffLL || joins > 0x7fffffffLL) return -1;
-  cudaError_t e = a.dim == 64 ? arcb_launch(attn_prefix_simple_kernel<64>, dim3((unsigned)blocks), dim3(128), 0, stream, a)
+  cudaError_t e = a.kv_fmt != 2 ? arcb_attn_prefix_mma(a, (unsigned)blocks, stream)
+                : a.dim == 64 ? arcb_launch(attn_prefix_simple_kernel<64>, dim3((unsigned)blocks), dim3(128), 0, stream, a)
                               : arcb_launch(attn_prefix_simple_kernel<128>, dim3((unsigned)blocks), dim3(128), 0, stream, a);
   arcb_count_launch(1);
   if (e == cudaSuccess && p.parts > 1) {

@@ -33,6 +33,9 @@ struct AttnPrefixArgs {
 
 constexpr int AP_PAD = 4;     // of a partial result: the sums of a row's values, its maximum (log2 units), its sum, two spare
 
+// 16-bit formats (attn_prefix_mma.cu); `a` as the launcher has filled it
+cudaError_t arcb_attn_prefix_mma(const AttnPrefixArgs& a, unsigned blocks, cudaStream_t stream);
+
 bool arcb_attn_prefix_supported(int n_heads, int n_kv, int dim, int act_fmt, int kv_fmt);
 // bytes of a.scratch for these sizes
 long long arcb_attn_prefix_scratch(const AttnPrefixArgs& a);

@@ -1,0 +1,92 @@
+// What the kernels of attention over shared cached rows have in common: how a CTA finds its part of the work, where partial
+// results go, how outputs are rounded.
+#pragma once
+#include "attn_prefix.cuh"
+
+namespace {
+
+constexpr float AP_LOG2E = 1.4426950408889634f;
+
+// A CTA's part of the work: query rows (row r is item item0 + (r0 + r) / rep, head kvh * rep + (r0 + r) % rep), cached rows
+// [begin, end) of a sequence, and which part of the results it is.
+struct ApWork {
+  int item0, r0, rows, kvh, seq, begin, end, part;
+};
+
+// Numbers: tiles of one (group, head, range) follow each other, so that they find its rows in L2.
+__device__ __forceinline__ ApWork ap_work(const AttnPrefixArgs& a, long long w) {
+  ApWork k;
+  const long long n1 = (long long)a.n_groups * a.n_kv * a.plan.tiles1 * a.plan.splits1;
+  int len, at0, split, splits;
+  if (w < n1) {
+    const int t = (int)(w % a.plan.tiles1); w /= a.plan.tiles1;
+    splits = a.plan.splits1;
+    split = (int)(w % splits); w /= splits;
+    k.kvh = (int)(w % a.n_kv);
+    const int g = (int)(w / a.n_kv);
+    int first, last;
+    if (a.uniform > 0) {
+      first = g * a.uniform;
+      last = first + a.uniform;
+      k.seq = first;
+      len = a.group_len[first];
+    } else {
+      first = a.group_first[g];
+      last = a.group_first[g + 1];
+      k.seq = a.group_seq[g];
+      len = a.group_len[g];
+    }
+    const bool bad = first < 0 || last < first || last > a.n_items || last - first > a.max_group || len < 0 || len > a.t_max ||
+                     (len > 0 && (k.seq < 0 || k.seq >= a.n_seqs)) || (g == 0 && first != 0) || (g == a.n_groups - 1 && last != a.n_items);
+    if (bad) {
+      if (threadIdx.x == 0) arcb_set_error(a.status, ARCB_DEV_BAD_INDEX);
+      first = min(max(first, 0), a.n_items);
+      last = min(max(last, first), min(a.n_items, first + a.max_group));
+      len = 0;
+    }
+    k.item0 = first;
+    k.r0 = t * a.plan.tile1;
+    k.rows = min(a.plan.tile1, (last - first) * a.rep - k.r0);
+    at0 = 0;
+    k.part = split;
+  } else {
+    w -= n1;
+    splits = a.plan.splits2;
+    split = (int)(w % splits); w /= splits;
+    const int t = (int)(w % a.plan.tiles2); w /= a.plan.tiles2;
+    k.kvh = (int)(w % a.n_kv);
+    k.item0 = (int)(w / a.n_kv);
+    k.r0 = t * a.plan.tile2;
+    k.rows = min(a.plan.tile2, a.rep - k.r0);
+    k.seq = a.item_seq ? a.item_seq[k.item0] : k.item0;
+    at0 = a.item_begin ? a.item_begin[k.item0] : 0;
+    len = a.item_end[k.item0] - at0;
+    if (len > 0 && (at0 < 0 || at0 + len > a.t_max || k.seq < 0 || k.seq >= a.n_seqs)) {
+      if (threadIdx.x == 0) arcb_set_error(a.status, ARCB_DEV_BAD_INDEX);
+      len = 0;
+    }
+    if (len < 0 || (a.item_skip && a.item_skip[k.item0])) len = 0;
+    k.part = a.plan.splits1 + split;
+  }
+  int chunk = (len + splits - 1) / splits;
+  chunk = (chunk + 63) & ~63;
+  k.begin = at0 + min(split * chunk, len);
+  k.end = at0 + min((split + 1) * chunk, len);
+  return k;
+}
+
+__device__ __forceinline__ float* ap_record(const AttnPrefixArgs& a, long long ih, int part) {
+  return a.scratch + ((size_t)ih * a.plan.parts + part) * (a.dim + AP_PAD);
+}
+
+// Outputs saturate in half, as all of the library's do; NaN stays NaN.
+__device__ __forceinline__ void ap_store4(void* out, size_t at, float4 v, int fmt) {
+  if (fmt != 1 || !(isnan(v.x) || isnan(v.y) || isnan(v.z) || isnan(v.w))) {
+    st_act4(out, at, v, fmt);
+    return;
+  }
+  const float f[4] = {v.x, v.y, v.z, v.w};
+  for (int i = 0; i < 4; ++i) reinterpret_cast<__half*>(out)[at + i] = isnan(f[i]) ? __float2half_rn(f[i]) : __float2half_rn(fminf(fmaxf(f[i], -65504.f), 65504.f));
+}
+
+}  // namespace
