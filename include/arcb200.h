@@ -503,7 +503,7 @@ typedef struct arcb_prefix_attention_args {
   int32_t reserved;
 } arcb_prefix_attention_args;
 
-/* Reads the sizes and formats, and whether d_item_end is set; < 0: the error. */
+/* Reads the sizes, formats and scale, and whether d_item_end is set; < 0: the error. */
 int64_t arcb_prefix_attention_scratch_bytes(const arcb_prefix_attention_args* args);
 int arcb_op_prefix_attention(const arcb_prefix_attention_args* args, void* stream);
 

@@ -30,7 +30,7 @@ attn_prefix_simple_kernel(AttnPrefixArgs a) {
   __shared__ __align__(16) float s_k[AS_KEYS][D + 4];
   __shared__ __align__(16) float s_v[AS_KEYS][D];
   const int lane = threadIdx.x & 31, wj = threadIdx.x >> 5;
-  const ApWork w = ap_work(a, blockIdx.x);
+  const ApWork w = ap_work(a, a.first_block + blockIdx.x);
   if (w.rows <= 0) return;
   for (int i = threadIdx.x; i < AS_ROWS * D / 4; i += 128) {
     const int r = i / (D / 4), c = i % (D / 4) * 4;
@@ -181,7 +181,10 @@ attn_prefix_join_kernel(AttnPrefixArgs a) {
 
 void fill_plan(AttnPrefixArgs& a) {
   a.rep = a.n_heads / a.n_kv;
-  a.plan = prefix_plan(a.n_groups, a.max_group, a.max_prefix, a.n_items, a.item_end ? a.max_own : 0, a.n_kv, a.rep, a.kv_fmt == 2 ? AS_ROWS : 64, arcb_num_sms());
+  const bool tc = a.kv_fmt != 2 && (a.act_fmt == a.kv_fmt || a.dim == 64) && a.scale != 0.f &&
+                  (long long)a.n_seqs * a.n_kv * a.t_max < (1ll << 31) - 256;
+  a.plan = prefix_plan(a.n_groups, a.max_group, a.max_prefix, a.n_items, a.item_end ? a.max_own : 0, a.n_kv, a.rep, a.kv_fmt == 2 ? AS_ROWS : 64,
+                       tc, arcb_num_sms());
 }
 
 }  // namespace
@@ -203,13 +206,25 @@ int arcb_launch_attn_prefix(AttnPrefixArgs a, cudaStream_t stream) {
   fill_plan(a);
   const PrefixPlan& p = a.plan;
   if (p.parts < 1 || (p.parts > 1 && !a.scratch)) return -1;
-  const long long blocks = (long long)a.n_groups * a.n_kv * p.tiles1 * p.splits1 + (long long)a.n_items * a.n_kv * p.tiles2 * p.splits2;
+  const long long shared = (long long)a.n_groups * a.n_kv * p.tiles1 * p.splits1, own = (long long)a.n_items * a.n_kv * p.tiles2 * p.splits2;
   const long long joins = ((long long)a.n_items * a.n_heads + 3) / 4;
-  if (blocks > 0x7fffffffLL || joins > 0x7fffffffLL) return -1;
-  cudaError_t e = a.kv_fmt != 2 ? arcb_attn_prefix_mma(a, (unsigned)blocks, stream)
-                : a.dim == 64 ? arcb_launch(attn_prefix_simple_kernel<64>, dim3((unsigned)blocks), dim3(128), 0, stream, a)
-                              : arcb_launch(attn_prefix_simple_kernel<128>, dim3((unsigned)blocks), dim3(128), 0, stream, a);
-  arcb_count_launch(1);
+  if (shared + own > 0x7fffffffLL || joins > 0x7fffffffLL) return -1;
+  long long blocks = shared + own;
+  a.first_block = 0;
+  if (p.tc) {
+    const int r = arcb_attn_prefix_tc(a, (unsigned)shared, stream);
+    arcb_count_launch(1);
+    if (r) return r;
+    a.first_block = shared;
+    blocks = own;
+  }
+  cudaError_t e = cudaSuccess;
+  if (blocks > 0) {
+    e = a.kv_fmt != 2 ? arcb_attn_prefix_mma(a, (unsigned)blocks, stream)
+      : a.dim == 64 ? arcb_launch(attn_prefix_simple_kernel<64>, dim3((unsigned)blocks), dim3(128), 0, stream, a)
+                    : arcb_launch(attn_prefix_simple_kernel<128>, dim3((unsigned)blocks), dim3(128), 0, stream, a);
+    arcb_count_launch(1);
+  }
   if (e == cudaSuccess && p.parts > 1) {
     e = arcb_launch(attn_prefix_join_kernel, dim3((unsigned)joins), dim3(128), 0, stream, a);
     arcb_count_launch(1);
@@ -231,13 +246,13 @@ static int prefix_args(const arcb_prefix_attention_args* p, AttnPrefixArgs& a, b
   a.kv_fmt = to_fmt(p->kv_format);
   if (!arcb_attn_prefix_supported(p->n_heads, p->n_kv, p->dim, a.act_fmt, a.kv_fmt))
     return arcb_fail(ARCB_E_UNSUPPORTED, "prefix attention: heads of 64 or 128, queries in the cache's format or half over a bfloat16 cache");
-  if (!(std::fabs(p->scale) <= 3.0e38f)) return arcb_fail(ARCB_E_ARG, "scale must be finite");
+  if (!std::isfinite(p->scale)) return arcb_fail(ARCB_E_ARG, "scale must be finite");
   a.n_groups = p->n_groups; a.n_items = p->n_items; a.n_heads = p->n_heads; a.n_kv = p->n_kv; a.dim = p->dim; a.n_seqs = p->n_seqs; a.t_max = p->t_max;
   auto bound = [](int v, int most) { return v <= 0 || v > most ? most : v; };
   a.max_group = bound(p->max_group, p->n_items);
   a.max_prefix = bound(p->max_prefix, p->t_max);
   a.max_own = bound(p->max_own, p->t_max);
-  a.item_end = p->d_item_end;
+  a.item_end = p->d_item_end; a.scale = p->scale;
   if (!p->n_groups && !p->d_item_end) return arcb_fail(ARCB_E_ARG, "prefix attention needs groups, rows of the items' own, or both");
   if (sizes_only) return ARCB_OK;
   if (!p->d_q || !p->d_k || !p->d_v || !p->d_out) return arcb_fail(ARCB_E_ARG, "null attention argument");
@@ -251,7 +266,7 @@ static int prefix_args(const arcb_prefix_attention_args* p, AttnPrefixArgs& a, b
   a.q = p->d_q; a.q_pitch = pitch; a.k = p->d_k; a.v = p->d_v; a.out = p->d_out;
   a.group_first = p->d_group_first; a.group_seq = p->d_group_seq; a.group_len = p->d_group_len;
   a.item_seq = p->d_item_seq; a.item_begin = p->d_item_begin; a.item_skip = p->d_item_skip;
-  a.scale = p->scale; a.scratch = reinterpret_cast<float*>(p->d_scratch); a.status = p->d_status;
+  a.scratch = reinterpret_cast<float*>(p->d_scratch); a.status = p->d_status;
   return ARCB_OK;
 }
 
@@ -269,6 +284,7 @@ extern "C" int arcb_op_prefix_attention(const arcb_prefix_attention_args* p, voi
   if (need > 0 && (!p->d_scratch || p->scratch_bytes < need))
     return arcb_fail(ARCB_E_ARG, "scratch is smaller than arcb_prefix_attention_scratch_bytes");
   const int e = arcb_launch_attn_prefix(a, (cudaStream_t)stream);
+  if (e >= 1000) return arcb_fail(ARCB_E_UNSUPPORTED, "prefix attention: no tensor map for these arrays");
   if (e > 0) return arcb_fail_cuda((cudaError_t)e, "prefix attention");
   if (e < 0) return arcb_fail(ARCB_E_ARG, "prefix attention: too much work for one call");
   return ARCB_OK;

@@ -29,12 +29,16 @@ struct AttnPrefixArgs {
   // filled by the launcher
   int rep;
   PrefixPlan plan;
+  long long first_block;      // of the launch, in the numbering of the whole work
 };
 
 constexpr int AP_PAD = 4;     // of a partial result: the sums of a row's values, its maximum (log2 units), its sum, two spare
 
 // 16-bit formats (attn_prefix_mma.cu); `a` as the launcher has filled it
 cudaError_t arcb_attn_prefix_mma(const AttnPrefixArgs& a, unsigned blocks, cudaStream_t stream);
+
+// shared rows for many queries (attn_prefix_tc.cu): the blocks of the shared part
+int arcb_attn_prefix_tc(const AttnPrefixArgs& a, unsigned blocks, cudaStream_t stream);
 
 bool arcb_attn_prefix_supported(int n_heads, int n_kv, int dim, int act_fmt, int kv_fmt);
 // bytes of a.scratch for these sizes

@@ -17,7 +17,7 @@ struct ApWork {
 __device__ __forceinline__ ApWork ap_work(const AttnPrefixArgs& a, long long w) {
   ApWork k;
   const long long n1 = (long long)a.n_groups * a.n_kv * a.plan.tiles1 * a.plan.splits1;
-  int len, at0, split, splits;
+  int len, at0, split, splits, grain = 63;
   if (w < n1) {
     const int t = (int)(w % a.plan.tiles1); w /= a.plan.tiles1;
     splits = a.plan.splits1;
@@ -48,6 +48,7 @@ __device__ __forceinline__ ApWork ap_work(const AttnPrefixArgs& a, long long w) 
     k.r0 = t * a.plan.tile1;
     k.rows = min(a.plan.tile1, (last - first) * a.rep - k.r0);
     at0 = 0;
+    grain = a.plan.tc ? 127 : 63;
     k.part = split;
   } else {
     w -= n1;
@@ -66,10 +67,10 @@ __device__ __forceinline__ ApWork ap_work(const AttnPrefixArgs& a, long long w) 
       len = 0;
     }
     if (len < 0 || (a.item_skip && a.item_skip[k.item0])) len = 0;
-    k.part = a.plan.splits1 + split;
+    k.part = a.plan.parts1 + split;
   }
   int chunk = (len + splits - 1) / splits;
-  chunk = (chunk + 63) & ~63;
+  chunk = (chunk + grain) & ~grain;
   k.begin = at0 + min(split * chunk, len);
   k.end = at0 + min((split + 1) * chunk, len);
   return k;

@@ -282,7 +282,7 @@ attn_prefix_mma_kernel(AttnPrefixArgs a) {
   pdl_launch_dependents();
   pdl_wait();
   extern __shared__ __align__(128) uint8_t am_smem[];
-  const ApWork w = ap_work(a, blockIdx.x);
+  const ApWork w = ap_work(a, a.first_block + blockIdx.x);
   if (w.rows <= 0) return;
   if (w.rows <= 16) am_body<D, HALF, QS, 4>(a, w, am_smem);
   else if (w.rows <= 32) am_body<D, HALF, QS, 2>(a, w, am_smem);

@@ -1,0 +1,426 @@
+// Attention over shared cached rows for many query rows of a group: tcgen05 products with their sums in tensor memory.
+//
+// A CTA has up to 256 query rows of one (group, key head) as two tiles of 128, A and B, and goes through a range of cached rows
+// 128 at a time.  With up to 128 rows B has the same queries as A and takes every other key tile, so that there are always two
+// chains (scores, softmax, weights, values) of which one is in the tensor core while the other is at its exponentials; A's and
+// B's sums are then two parts of the result.
+//   warp 0        TMA: key and value tiles as 128 x 64 boxes with the 128-byte swizzle, rings shared by A and B
+//   warps 1, 2    products of A and of B: S = Q K^T (128 TMEM columns), O += P V with P read from TMEM
+//   warp 3        sets the value rows behind the end of the last tile to zero: a weight of 0 does not hide a NaN
+//   warps 4-19    two threads a query row, 64 keys of every tile each: maxima (exchanged), exponentials, row sums, P over the
+//                 thread's own score columns
+// Maxima, sums and results are fp32.  The reference maximum of a row is raised only when it grows by 2^8.  Half queries over a
+// bfloat16 cache are two bfloat16 pieces (exact), and their weights too (2^-16 of a weight off).  In equal formats a weight is one
+// 16-bit value: its error, half a step, adds to an output that is rounded by as much itself (sqrt 2 of that error alone), and a
+// second piece costs half as many products again where products are what bounds the kernel.
+#include <type_traits>
+
+#include "attn_prefix_impl.cuh"
+#include "flash_common.cuh"
+#include "gemm.cuh"
+#include "launch.cuh"
+
+using namespace sm100;
+
+namespace {
+
+constexpr int AT_ROWS = 128, AT_KEYS = 128, AT_THREADS = 640;
+constexpr float AT_RESCALE = 8.f;          // log2 units
+constexpr int AT_BOX = 128 * 64 * 2;
+
+template <int D, bool QS>
+struct AtCfg {
+  static constexpr int BOXES = D / 64;
+  static constexpr int Q_PIECE = BOXES * AT_BOX;                 // a tile of queries
+  static constexpr int Q_BYTES = Q_PIECE * (QS ? 2 : 1);
+  static constexpr int KV_BYTES = BOXES * AT_BOX;
+  static constexpr int FIT = (208 * 1024 - 2 * Q_BYTES) / (2 * KV_BYTES);
+  static constexpr int STAGES = FIT > 4 ? 4 : FIT;
+  static_assert(STAGES >= 2, "two tiles of keys and values");
+  static constexpr int TILES = 2 * Q_BYTES + 2 * STAGES * KV_BYTES;
+  static constexpr int BARS = 256;
+  static constexpr int XCHG = 2 * 2 * 2 * AT_ROWS * 4;
+  static constexpr int SMEM = TILES + BARS + XCHG + 1024;
+  static_assert(SMEM <= 227 * 1024, "shared memory of one CTA");
+};
+
+// HALF: the cache's format.  QS: half queries over a bfloat16 cache.
+// WP: 16-bit pieces of a weight.
+template <int D, bool HALF, bool QS, int WP>
+__global__ void __launch_bounds__(AT_THREADS, 1)
+attn_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, AttnPrefixArgs a, uint32_t idesc_qk,
+                      uint32_t idesc_pv) {
+  using C = AtCfg<D, QS>;
+  pdl_launch_dependents();
+  pdl_wait();
+  const ApWork w = ap_work(a, a.first_block + blockIdx.x);
+  if (w.rows <= 0) return;
+  extern __shared__ __align__(1024) uint8_t at_smem[];
+  const uint32_t raw = smem_u32(at_smem);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* base_ptr = at_smem + (base - raw);
+  const uint32_t q_smem = base, k_smem = base + 2 * C::Q_BYTES, v_smem = k_smem + C::STAGES * C::KV_BYTES, bar0 = base + C::TILES;
+  const uint32_t b_kfull = bar0, b_kempty = b_kfull + 8 * C::STAGES, b_vfull = b_kempty + 8 * C::STAGES, b_vempty = b_vfull + 8 * C::STAGES,
+                 b_clean = b_vempty + 8 * C::STAGES, b_s = b_clean + 8, b_p = b_s + 16, b_o = b_p + 16, b_x = b_o + 16;
+  static_assert(32 * C::STAGES + 8 + 48 + 64 <= C::BARS - 8, "barriers");
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(base_ptr + C::TILES + C::BARS - 8);
+  float (*s_xchg)[2][2][AT_ROWS] = reinterpret_cast<float (*)[2][2][AT_ROWS]>(base_ptr + C::TILES + C::BARS);   // [parity][tile][half][row]
+
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const bool wide = w.rows > AT_ROWS;
+  const int n_tiles = (w.end - w.begin + AT_KEYS - 1) / AT_KEYS;
+  const auto tiles_of = [&](int x) { return wide ? n_tiles : (n_tiles + 1 - x) / 2; };          // key tiles of A and B
+  const int left = w.end - w.begin - (n_tiles - 1) * AT_KEYS;                                   // rows of the last one
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(b_kfull + 8 * s, 1);
+      mbar_init(b_vfull + 8 * s, 1);
+      mbar_init(b_kempty + 8 * s, wide ? 2 : 1);
+      mbar_init(b_vempty + 8 * s, wide ? 2 : 1);
+    }
+    mbar_init(b_clean, 1);
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(b_s + 8 * x, 1);
+      mbar_init(b_p + 8 * x, 256);
+      mbar_init(b_o + 8 * x, 1);
+    }
+    for (int i = 0; i < 8; ++i) mbar_init(b_x + 8 * i, 64);
+    mbar_fence_init();
+    tma_prefetch_desc(&tmap_k);
+    tma_prefetch_desc(&tmap_v);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
+    tmem_relinquish();
+  }
+  // queries, 16 bytes a thread: rows of 128 bytes, eight pieces exclusive-or swizzled by the row
+  {
+    const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;        // a negative scale turns the queries, so that maxima are maxima
+    const int rows = wide ? 2 * AT_ROWS : AT_ROWS;
+    for (int i = threadIdx.x; i < rows * (D / 8); i += AT_THREADS) {
+      const int r = i / (D / 8), c = i % (D / 8);
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (r < w.rows) {
+        const int R = w.r0 + r;
+        v = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.q) + (size_t)(w.item0 + R / a.rep) * a.q_pitch +
+                                            (size_t)(w.kvh * a.rep + R % a.rep) * D + c * 8);
+        v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
+      }
+      const int t = r & (AT_ROWS - 1);
+      uint8_t* dst = base_ptr + (r / AT_ROWS) * C::Q_BYTES + (c >> 3) * AT_BOX + t * 128 + (((c & 7) ^ (t & 7)) << 4);
+      if constexpr (QS) {
+        uint32_t in[4] = {v.x, v.y, v.z, v.w}, hi[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = unpack2_act(in[e], 1);
+          hi[e] = pack2_bf16(f.x, f.y);
+          const float2 h = unpack2_bf16(hi[e]);
+          lo[e] = pack2_bf16(f.x - h.x, f.y - h.y);
+        }
+        *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(dst + C::Q_PIECE) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      } else {
+        *reinterpret_cast<uint4*>(dst) = v;
+      }
+    }
+    fence_proxy_async_smem();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  // S_A [0, 128), S_B [128, 256), O_A [256, 256 + D), O_B
+
+  if (warp < 4) {
+    reg_dealloc_32();
+    if (warp == 0) {
+      const int row = (w.seq * a.n_kv + w.kvh) * a.t_max + w.begin;
+      bool ok = true;
+      auto wait = [&](uint32_t bar, uint32_t parity) {
+        if (ok && !__all_sync(0xffffffffu, mbar_wait_bounded(bar, parity))) {
+          if (lane == 0) arcb_set_error(a.status, ARCB_DEV_WAIT_TIMEOUT_MMA);
+          ok = false;
+        }
+      };
+      int j = 0;
+      for (; j < n_tiles; ++j) {
+        const int s = j % C::STAGES;
+        const uint32_t parity = ((j / C::STAGES) & 1) ^ 1;
+        wait(b_kempty + 8 * s, parity);
+        if (!ok) break;
+        if (lane == 0) {
+          mbar_expect_tx(b_kfull + 8 * s, C::KV_BYTES);
+#pragma unroll
+          for (int c = 0; c < C::BOXES; ++c) tma_load_2d(k_smem + s * C::KV_BYTES + c * AT_BOX, &tmap_k, c * 64, row + j * AT_KEYS, b_kfull + 8 * s);
+        }
+        wait(b_vempty + 8 * s, parity);
+        if (!ok) break;
+        if (lane == 0) {
+          mbar_expect_tx(b_vfull + 8 * s, C::KV_BYTES);
+#pragma unroll
+          for (int c = 0; c < C::BOXES; ++c) tma_load_2d(v_smem + s * C::KV_BYTES + c * AT_BOX, &tmap_v, c * 64, row + j * AT_KEYS, b_vfull + 8 * s);
+        }
+      }
+      if (!ok)        // gave up at tile j: the copies under way end before the CTA does
+        for (int i = j > C::STAGES ? j - C::STAGES : 0; i <= j; ++i) {
+          mbar_wait_bounded(b_kfull + 8 * (i % C::STAGES), (i / C::STAGES) & 1);
+          if (i < j) mbar_wait_bounded(b_vfull + 8 * (i % C::STAGES), (i / C::STAGES) & 1);
+        }
+    } else if (warp < 3) {
+      const int x = warp - 1, n_x = tiles_of(x);
+      const uint32_t el = elect_one();
+      bool ok = true;
+      auto wait = [&](uint32_t bar, uint32_t parity, int code) {
+        if (ok && !__all_sync(0xffffffffu, mbar_wait_bounded(bar, parity))) {
+          if (lane == 0) arcb_set_error(a.status, code);
+          ok = false;
+        }
+      };
+      const uint32_t t_s = tmem_base + x * 128, t_o = tmem_base + 256 + x * D, q_tile = q_smem + (wide ? x * C::Q_BYTES : 0);
+      auto tile = [&](int i) { return wide ? i : 2 * i + x; };
+      for (int i = 0; ok && i <= n_x; ++i) {
+        if (i > 0) {
+          const int j = tile(i - 1), s = j % C::STAGES;
+          wait(b_p + 8 * x, (i - 1) & 1, ARCB_DEV_WAIT_TIMEOUT_ACC);
+          wait(b_vfull + 8 * s, (j / C::STAGES) & 1, ARCB_DEV_WAIT_TIMEOUT_TMA);
+          if (j == n_tiles - 1 && left < AT_KEYS) wait(b_clean, 0, ARCB_DEV_WAIT_TIMEOUT_TMA);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t dv = umma_desc_mn_sw128(v_smem + s * C::KV_BYTES, AT_BOX);
+#pragma unroll
+          for (int piece = 0; piece < WP; ++piece)
+#pragma unroll
+            for (int ks = 0; ks < AT_KEYS / 16; ++ks)
+              umma_f16_ts_if(el, t_o, t_s + (ks >> 2) * 64 + piece * 32 + (ks & 3) * 8, dv + (uint64_t)(ks * (2048 >> 4)), idesc_pv, (i > 1 || piece || ks) ? 1u : 0u);
+          umma_commit_if(el, b_vempty + 8 * s);
+        }
+        if (i == n_x) break;
+        const int j = tile(i), s = j % C::STAGES;
+        wait(b_kfull + 8 * s, (j / C::STAGES) & 1, ARCB_DEV_WAIT_TIMEOUT_TMA);
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int piece = 0; piece < (QS ? 2 : 1); ++piece)
+#pragma unroll
+          for (int c = 0; c < C::BOXES; ++c) {
+            const uint64_t dq = umma_desc_k_sw128(q_tile + piece * C::Q_PIECE + c * AT_BOX);
+            const uint64_t dk = umma_desc_k_sw128(k_smem + s * C::KV_BYTES + c * AT_BOX);
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) umma_f16_if(el, t_s, dq + 2 * ks, dk + 2 * ks, idesc_qk, (piece | c | ks) ? 1u : 0u);
+          }
+        umma_commit_if(el, b_s + 8 * x);
+        umma_commit_if(el, b_kempty + 8 * s);
+      }
+      if (ok && n_x > 0) umma_commit_if(el, b_o + 8 * x);
+    } else if (n_tiles > 0 && left < AT_KEYS) {
+      const int s = (n_tiles - 1) % C::STAGES;
+      if (__all_sync(0xffffffffu, mbar_wait_bounded(b_vfull + 8 * s, ((n_tiles - 1) / C::STAGES) & 1))) {
+        uint8_t* v = base_ptr + 2 * C::Q_BYTES + (C::STAGES + s) * C::KV_BYTES;
+#pragma unroll
+        for (int c = 0; c < C::BOXES; ++c)
+          for (int i = left * 8 + lane; i < AT_KEYS * 8; i += 32) *reinterpret_cast<uint4*>(v + c * AT_BOX + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(b_clean);
+      } else if (lane == 0) {
+        arcb_set_error(a.status, ARCB_DEV_WAIT_TIMEOUT_TMA);
+      }
+    }
+  } else {
+    reg_alloc_112();
+    const int x = (warp - 4) >> 3, half = ((warp >> 2) - 1) & 1, quarter = warp & 3;
+    const int r = quarter * 32 + lane, n_x = tiles_of(x);
+    const uint32_t t_lane = tmem_base + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t t_s = t_lane + x * 128 + half * 64, t_o = t_lane + 256 + x * D + half * (D / 2);
+    const uint32_t xbar = b_x + 8 * (x * 4 + quarter);
+    const float sc = fabsf(a.scale) * AP_LOG2E;
+    const int first_row = (wide ? x * AT_ROWS : 0) + quarter * 32;         // of the warp, among the CTA's
+    const bool idle = first_row >= w.rows;
+    bool ok = true;
+    uint32_t xphase = 0;
+    // hands `mine` to the row's other thread; consecutive exchanges use the buffer's two parts in turn
+    auto swap = [&](float mine, float& theirs) -> bool {
+      s_xchg[xphase][x][half][r] = mine;
+      tc_fence_before();
+      mbar_arrive(xbar);
+      const bool good = mbar_wait_bounded(xbar, xphase);
+      tc_fence_after();
+      theirs = s_xchg[xphase][x][half ^ 1][r];
+      xphase ^= 1u;
+      return good;
+    };
+    float m_ref = -INFINITY, l = 0.f;
+    for (int i = 0; i < n_x; ++i) {
+      if (!__all_sync(0xffffffffu, mbar_wait_bounded(b_s + 8 * x, i & 1))) {
+        if (lane == 0) arcb_set_error(a.status, ARCB_DEV_WAIT_TIMEOUT_ACC);
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      if (idle) {           // rows that do not exist: whatever their columns hold stays with them
+        tc_fence_before();
+        mbar_arrive(b_p + 8 * x);
+        continue;
+      }
+      const int j = wide ? i : 2 * i + x;
+      const int seen = (j == n_tiles - 1 ? left : AT_KEYS) - half * 64;    // of the thread's 64 keys
+      auto load_scores = [&](int c, uint32_t (&sv)[32]) {
+        tmem_ld_32x32(t_s + c * 32, sv);
+        tmem_wait_ld_dep(sv);
+        if (seen < 64)
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (c * 32 + e >= seen) sv[e] = 0xff800000u;
+      };
+      // the scores are read twice (maximum, then exponentials): tensor memory is quicker to read again than 64 registers are
+      // to hold
+      float mine = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t sv[32];
+        load_scores(c, sv);
+        float mx = fmaxf(__uint_as_float(sv[0]), __uint_as_float(sv[1]));
+#pragma unroll
+        for (int e = 2; e < 32; e += 2) mx = max3_f32(mx, __uint_as_float(sv[e]), __uint_as_float(sv[e + 1]));
+        mine = fmaxf(mine, mx);
+      }
+      mine *= sc;
+      float other;
+      const bool good = swap(mine, other);
+      if (!good) arcb_set_error(a.status, ARCB_DEV_WAIT_TIMEOUT_ACC);
+      ok = __all_sync(0xffffffffu, good);
+      if (!ok) break;
+      const float mx = fmaxf(mine, other);
+      float alpha = 1.f;
+      if (mx > m_ref + AT_RESCALE) {     // also the first tile (m_ref = -inf)
+        alpha = m_ref == -INFINITY ? 0.f : ex2_fast(m_ref - mx);
+        m_ref = mx;
+      }
+      l *= alpha;
+      const float m_safe = m_ref == -INFINITY ? 0.f : m_ref;
+      const uint64_t sc2 = pack_f32x2(sc, sc), nm2 = pack_f32x2(-m_safe, -m_safe);
+      if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+        // these scores were asked for behind the last product of values: its sums are complete
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) {
+          uint32_t o[32];
+          tmem_ld_32x32(t_o + c * 32, o);
+          tmem_wait_ld_dep(o);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+          tmem_st_32x32(t_o + c * 32, o);
+        }
+      }
+      float ls0 = 0.f, ls1 = 0.f;
+      uint32_t lo[WP > 1 ? 16 : 1];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t sv[32];
+        load_scores(c, sv);
+        if constexpr (WP > 1) {
+          if (c == 1) tmem_st_32x16(t_s + 32, lo);        // the first half's second pieces, over scores read by now
+        }
+        uint32_t hi[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float t0, t1;
+          shift2_f32(sv[2 * e], sv[2 * e + 1], sc2, nm2, t0, t1);
+          t0 = ex2_fast(t0);
+          t1 = ex2_fast(t1);
+          ls0 += t0;
+          ls1 += t1;
+          hi[e] = pack2_prob(t0, t1, HALF ? 1 : 0);
+          if constexpr (WP > 1) {
+            const float2 f = unpack2_act(hi[e], HALF ? 1 : 0);
+            lo[e] = pack2_prob(t0 - f.x, t1 - f.y, HALF ? 1 : 0);
+          }
+        }
+        tmem_st_32x16(t_s + c * 16, hi);
+        if constexpr (WP > 1) {
+          if (c == 1) tmem_st_32x16(t_s + 48, lo);
+        }
+      }
+      l += ls0 + ls1;
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(b_p + 8 * x);
+    }
+    // results: a quad of lanes writes 64 consecutive bytes of each of its four rows
+    if (!idle) {
+      float l_other = 0.f;
+      if (ok && n_x > 0) {
+        bool good = swap(l, l_other);
+        good = mbar_wait_bounded(b_o + 8 * x, 0) && good;
+        if (!good) arcb_set_error(a.status, ARCB_DEV_WAIT_TIMEOUT_ACC);
+        ok = __all_sync(0xffffffffu, good);
+      }
+      const bool any = ok && n_x > 0;
+      const float l_row = half ? l_other + l : l + l_other;
+      const int piece = lane & 3, quad_row = first_row + lane - piece;
+      auto record = [&](int row, int part) {
+        const int R = w.r0 + row;
+        return ap_record(a, (long long)(w.item0 + R / a.rep) * a.n_heads + w.kvh * a.rep + R % a.rep, part);
+      };
+      const int part = 2 * w.part + (wide ? 0 : x);
+      if (any) tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) {
+        uint32_t o[32];
+        if (any) {
+          tmem_ld_32x32(t_o + c * 32, o);
+          tmem_wait_ld_dep(o);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0u;
+        }
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          uint4 v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = make_uint4(o[g * 16 + e * 4], o[g * 16 + e * 4 + 1], o[g * 16 + e * 4 + 2], o[g * 16 + e * 4 + 3]);
+          quad_transpose(v, lane);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (quad_row + e < w.rows)
+              *reinterpret_cast<uint4*>(record(quad_row + e, part) + half * (D / 2) + c * 32 + g * 16 + piece * 4) = v[e];
+        }
+      }
+      const int row = first_row + lane;
+      if (half == 0 && row < w.rows) {
+        *reinterpret_cast<float2*>(record(row, part) + D) = any ? make_float2(m_ref, l_row) : make_float2(-INFINITY, 0.f);
+        if (wide) *reinterpret_cast<float2*>(record(row, part + 1) + D) = make_float2(-INFINITY, 0.f);     // one part where B has rows of its own
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+template <int D, bool HALF, bool QS, int WP>
+int at_launch(const AttnPrefixArgs& a, unsigned blocks, cudaStream_t stream) {
+  using C = AtCfg<D, QS>;
+  static std::atomic<unsigned long long> done{0};
+  cudaError_t e = arcb_opt_in_smem(attn_prefix_tc_kernel<D, HALF, QS, WP>, C::SMEM, done);
+  if (e != cudaSuccess) return (int)e;
+  CUtensorMap tk, tv;
+  const uint64_t rows = (uint64_t)a.n_seqs * a.n_kv * a.t_max;
+  int r = arcb_make_tmap_2d_16b(&tk, a.k, rows, D, AT_KEYS, 64, HALF);
+  if (!r) r = arcb_make_tmap_2d_16b(&tv, a.v, rows, D, AT_KEYS, 64, HALF);
+  if (r) return 1000 + r;
+  const int fmt = HALF ? 0 : 1;
+  const uint32_t idesc_qk = umma_idesc_f16(AT_ROWS, AT_KEYS, fmt, fmt, 0, 0);
+  const uint32_t idesc_pv = umma_idesc_f16(AT_ROWS, D, fmt, fmt, 0, 1);      // values are MN-major
+  return (int)arcb_launch(attn_prefix_tc_kernel<D, HALF, QS, WP>, dim3(blocks), dim3(AT_THREADS), C::SMEM, stream, tk, tv, a, idesc_qk, idesc_pv);
+}
+
+}  // namespace
+
+int arcb_attn_prefix_tc(const AttnPrefixArgs& a, unsigned blocks, cudaStream_t stream) {
+  if (a.kv_fmt == 1) return a.dim == 64 ? at_launch<64, true, false, 1>(a, blocks, stream) : at_launch<128, true, false, 1>(a, blocks, stream);
+  if (a.act_fmt == 1) return a.dim == 64 ? at_launch<64, false, true, 2>(a, blocks, stream) : -1;
+  return a.dim == 64 ? at_launch<64, false, false, 1>(a, blocks, stream) : at_launch<128, false, false, 1>(a, blocks, stream);
+}
