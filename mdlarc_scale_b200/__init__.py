@@ -33,7 +33,8 @@ def __getattr__(name):  # torch-dependent parts are imported lazily
         return generation.generate
     if name in ("prefix_attention", "copy_cache_rows"):
         from . import prefix
-        return getattr(prefix, name)
+        globals().update(prefix_attention=prefix.prefix_attention, copy_cache_rows=prefix.copy_cache_rows)   # this function costs 2 us a call
+        return globals()[name]
     if name in ("Engine", "engine_for"):
         from . import engine
         return getattr(engine, name)

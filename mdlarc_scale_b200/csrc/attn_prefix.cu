@@ -30,7 +30,7 @@ attn_prefix_simple_kernel(AttnPrefixArgs a) {
   __shared__ __align__(16) float s_k[AS_KEYS][D + 4];
   __shared__ __align__(16) float s_v[AS_KEYS][D];
   const int lane = threadIdx.x & 31, wj = threadIdx.x >> 5;
-  const ApWork w = ap_work(a, a.first_block + blockIdx.x);
+  const ApWork w = ap_work(a, a.first_block + blockIdx.x, threadIdx.x == 0);
   if (w.rows <= 0) return;
   for (int i = threadIdx.x; i < AS_ROWS * D / 4; i += 128) {
     const int r = i / (D / 4), c = i % (D / 4) * 4;
@@ -136,55 +136,71 @@ attn_prefix_simple_kernel(AttnPrefixArgs a) {
   }
 }
 
-// One warp per (item, head): joins the parts in order.  Lane s keeps the factors of parts s and s + 32.
+// Joins the parts of an (item, head), W warps of a CTA for each; warp j adds parts j, j + W, ... in order, the warps' sums are
+// added in order.  With few results of many parts one warp alone would wait for memory a dozen times.
+template <int W>
 __global__ void __launch_bounds__(128)
 attn_prefix_join_kernel(AttnPrefixArgs a) {
   pdl_launch_dependents();
   pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const long long ih = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (ih >= (long long)a.n_items * a.n_heads) return;
-  const int n = a.plan.parts, rec = a.dim + AP_PAD;
-  const bool skip = a.item_skip && a.item_skip[ih / a.n_heads];
+  __shared__ float4 s_sum[W > 1 ? W : 1][32];
+  __shared__ float s_l[W > 1 ? W : 1];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, mine = warp % W;
+  const long long ih = (long long)blockIdx.x * (4 / W) + warp / W;
+  const bool out_of_range = ih >= (long long)a.n_items * a.n_heads;
+  if (W == 1 && out_of_range) return;
+  const int n = a.plan.parts, rec = a.dim + AP_PAD, c = lane * 4;
   const float* r0 = a.scratch + (size_t)ih * n * rec;
-  float m_s[2], l_s[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int s = lane + 32 * i;
-    const float2 ml = s < n ? *reinterpret_cast<const float2*>(r0 + (size_t)s * rec + a.dim) : make_float2(-INFINITY, 0.f);
-    m_s[i] = ml.x;
-    l_s[i] = ml.y;
-  }
-  float m = fmaxf(m_s[0], m_s[1]);
+  float m = -INFINITY;
+  for (int s = lane; s < n; s += 32) m = fmaxf(m, r0[(size_t)s * rec + a.dim]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   const float safe = m == -INFINITY ? 0.f : m;
-  const float f0 = exp2f(m_s[0] - safe), f1 = exp2f(m_s[1] - safe);
-  const float l = warp_sum(l_s[0] * f0 + l_s[1] * f1);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  const int c = lane * 4;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int s = 0; s < n; ++s) {
-    const float f = __shfl_sync(0xffffffffu, s < 32 ? f0 : f1, s & 31);
-    if (c < a.dim && f != 0.f) {        // an empty part's sums count for nothing, whatever they are
-      const float4 v = *reinterpret_cast<const float4*>(r0 + (size_t)s * rec + c);
-      o.x += v.x * f; o.y += v.y * f; o.z += v.z * f; o.w += v.w * f;
+  float l = 0.f;
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int base = 0; base < n; base += 32 * W) {
+    const int s = base + mine + lane * W;
+    float f = 0.f;
+    if (s < n) {
+      const float2 ml = *reinterpret_cast<const float2*>(r0 + (size_t)s * rec + a.dim);
+      f = exp2f(ml.x - safe);
+      l += ml.y * f;
+    }
+    const int here = min(32, (n - base - mine + W - 1) / W);
+#pragma unroll 8
+    for (int i = 0; i < here; ++i) {
+      const float fi = __shfl_sync(0xffffffffu, f, i);
+      if (c < a.dim && fi != 0.f) {        // an empty part's sums count for nothing, whatever they are
+        const float4 v = *reinterpret_cast<const float4*>(r0 + (size_t)(base + mine + i * W) * rec + c);
+        sum.x += v.x * fi; sum.y += v.y * fi; sum.z += v.z * fi; sum.w += v.w * fi;
+      }
     }
   }
-  if (c < a.dim) {
-    if (skip) o = make_float4(0.f, 0.f, 0.f, 0.f);
-    else o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-    ap_store4(a.out, (size_t)ih * a.dim + c, o, a.act_fmt);
+  l = warp_sum(l);
+  if (W > 1) {
+    s_sum[mine][lane] = sum;
+    if (lane == 0) s_l[mine] = l;
+    __syncthreads();
+    if (mine != 0) return;
+#pragma unroll
+    for (int j = 1; j < W; ++j) {
+      const float4 v = s_sum[j][lane];
+      sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+      l += s_l[j];
+    }
   }
+  if (c >= a.dim) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  sum = a.item_skip && a.item_skip[ih / a.n_heads] ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+  ap_store4(a.out, (size_t)ih * a.dim + c, sum, a.act_fmt);
 }
 
 void fill_plan(AttnPrefixArgs& a) {
   a.rep = a.n_heads / a.n_kv;
   const bool tc = a.kv_fmt != 2 && (a.act_fmt == a.kv_fmt || a.dim == 64) && a.scale != 0.f &&
                   (long long)a.n_seqs * a.n_kv * a.t_max < (1ll << 31) - 256;
-  a.plan = prefix_plan(a.n_groups, a.max_group, a.max_prefix, a.n_items, a.item_end ? a.max_own : 0, a.n_kv, a.rep, a.kv_fmt == 2 ? AS_ROWS : 64,
-                       tc, arcb_num_sms());
+  a.plan = prefix_plan(a.n_groups, a.max_group, a.max_prefix, a.n_items, a.item_end ? a.max_own : 0, a.n_kv, a.rep,
+                       a.kv_fmt == 2, tc, arcb_num_sms());
 }
 
 }  // namespace
@@ -209,24 +225,31 @@ int arcb_launch_attn_prefix(AttnPrefixArgs a, cudaStream_t stream) {
   const long long shared = (long long)a.n_groups * a.n_kv * p.tiles1 * p.splits1, own = (long long)a.n_items * a.n_kv * p.tiles2 * p.splits2;
   const long long joins = ((long long)a.n_items * a.n_heads + 3) / 4;
   if (shared + own > 0x7fffffffLL || joins > 0x7fffffffLL) return -1;
-  long long blocks = shared + own;
   a.first_block = 0;
-  if (p.tc) {
-    const int r = arcb_attn_prefix_tc(a, (unsigned)shared, stream);
-    arcb_count_launch(1);
-    if (r) return r;
-    a.first_block = shared;
-    blocks = own;
-  }
   cudaError_t e = cudaSuccess;
-  if (blocks > 0) {
-    e = a.kv_fmt != 2 ? arcb_attn_prefix_mma(a, (unsigned)blocks, stream)
-      : a.dim == 64 ? arcb_launch(attn_prefix_simple_kernel<64>, dim3((unsigned)blocks), dim3(128), 0, stream, a)
-                    : arcb_launch(attn_prefix_simple_kernel<128>, dim3((unsigned)blocks), dim3(128), 0, stream, a);
+  if (p.shared == AP_SHARED_PLAIN) {
+    e = a.dim == 64 ? arcb_launch(attn_prefix_simple_kernel<64>, dim3((unsigned)(shared + own)), dim3(128), 0, stream, a)
+                    : arcb_launch(attn_prefix_simple_kernel<128>, dim3((unsigned)(shared + own)), dim3(128), 0, stream, a);
     arcb_count_launch(1);
+  } else {
+    long long units = shared + own;
+    if (p.shared != AP_SHARED_ROWS && shared > 0) {
+      const int r = p.shared == AP_SHARED_TC ? arcb_attn_prefix_tc(a, (unsigned)shared, stream) : (int)arcb_attn_prefix_mma(a, (unsigned)shared, stream);
+      arcb_count_launch(1);
+      if (r) return r;
+      a.first_block = shared;
+      units = own;
+    }
+    if (units > 0) {
+      e = arcb_attn_prefix_rows(a, units, stream);
+      arcb_count_launch(1);
+    }
   }
   if (e == cudaSuccess && p.parts > 1) {
-    e = arcb_launch(attn_prefix_join_kernel, dim3((unsigned)joins), dim3(128), 0, stream, a);
+    // four warps a result where a warp each would leave SMs without work
+    const bool few = p.parts >= 8 && joins < 4LL * arcb_num_sms();
+    e = few ? arcb_launch(attn_prefix_join_kernel<4>, dim3((unsigned)((long long)a.n_items * a.n_heads)), dim3(128), 0, stream, a)
+            : arcb_launch(attn_prefix_join_kernel<1>, dim3((unsigned)joins), dim3(128), 0, stream, a);
     arcb_count_launch(1);
   }
   return (int)e;

@@ -14,10 +14,10 @@ struct ApWork {
 };
 
 // Numbers: tiles of one (group, head, range) follow each other, so that they find its rows in L2.
-__device__ __forceinline__ ApWork ap_work(const AttnPrefixArgs& a, long long w) {
+__device__ __forceinline__ ApWork ap_work(const AttnPrefixArgs& a, long long w, bool report) {
   ApWork k;
   const long long n1 = (long long)a.n_groups * a.n_kv * a.plan.tiles1 * a.plan.splits1;
-  int len, at0, split, splits, grain = 63;
+  int len, at0, split, splits, grain = 15;
   if (w < n1) {
     const int t = (int)(w % a.plan.tiles1); w /= a.plan.tiles1;
     splits = a.plan.splits1;
@@ -39,7 +39,7 @@ __device__ __forceinline__ ApWork ap_work(const AttnPrefixArgs& a, long long w) 
     const bool bad = first < 0 || last < first || last > a.n_items || last - first > a.max_group || len < 0 || len > a.t_max ||
                      (len > 0 && (k.seq < 0 || k.seq >= a.n_seqs)) || (g == 0 && first != 0) || (g == a.n_groups - 1 && last != a.n_items);
     if (bad) {
-      if (threadIdx.x == 0) arcb_set_error(a.status, ARCB_DEV_BAD_INDEX);
+      if (report) arcb_set_error(a.status, ARCB_DEV_BAD_INDEX);
       first = min(max(first, 0), a.n_items);
       last = min(max(last, first), min(a.n_items, first + a.max_group));
       len = 0;
@@ -48,7 +48,7 @@ __device__ __forceinline__ ApWork ap_work(const AttnPrefixArgs& a, long long w) 
     k.r0 = t * a.plan.tile1;
     k.rows = min(a.plan.tile1, (last - first) * a.rep - k.r0);
     at0 = 0;
-    grain = a.plan.tc ? 127 : 63;
+    grain = a.plan.shared == AP_SHARED_TC ? 127 : a.plan.shared == AP_SHARED_TILES ? 63 : 15;
     k.part = split;
   } else {
     w -= n1;
@@ -63,7 +63,7 @@ __device__ __forceinline__ ApWork ap_work(const AttnPrefixArgs& a, long long w) 
     at0 = a.item_begin ? a.item_begin[k.item0] : 0;
     len = a.item_end[k.item0] - at0;
     if (len > 0 && (at0 < 0 || at0 + len > a.t_max || k.seq < 0 || k.seq >= a.n_seqs)) {
-      if (threadIdx.x == 0) arcb_set_error(a.status, ARCB_DEV_BAD_INDEX);
+      if (report) arcb_set_error(a.status, ARCB_DEV_BAD_INDEX);
       len = 0;
     }
     if (len < 0 || (a.item_skip && a.item_skip[k.item0])) len = 0;
@@ -88,6 +88,15 @@ __device__ __forceinline__ void ap_store4(void* out, size_t at, float4 v, int fm
   }
   const float f[4] = {v.x, v.y, v.z, v.w};
   for (int i = 0; i < 4; ++i) reinterpret_cast<__half*>(out)[at + i] = isnan(f[i]) ? __float2half_rn(f[i]) : __float2half_rn(fminf(fmaxf(f[i], -65504.f), 65504.f));
+}
+
+__device__ __forceinline__ void ap_store2(void* out, size_t at, float x, float y, int fmt) {
+  uint32_t v = pack2_act(x, y, fmt);
+  if (fmt == 1) {
+    if (isnan(x)) v = (v & 0xffff0000u) | 0x7fffu;
+    if (isnan(y)) v = (v & 0xffffu) | 0x7fff0000u;
+  }
+  *reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(out) + at) = v;
 }
 
 }  // namespace

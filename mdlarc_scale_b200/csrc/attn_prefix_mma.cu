@@ -3,8 +3,8 @@
 // Four warps share tiles of 64 keys and values, copied asynchronously into a ring in shared memory (16-byte pieces, exclusive-or
 // swizzled by the row, so that the eight rows of a matrix load fall into different banks).  S = Q K^T and O += P V are
 // m16n8k16 products with fp32 sums; queries, sums and weights stay in registers (the sums of two neighbouring score tiles are
-// the weights' operand as they lie).  With 16, 32 or 64 query rows the warps divide the tile's keys among 4, 2 or 1 groups and
-// the rows among 1, 2 or 4; groups are merged once at the end.  What bounds it is reading the cache: 16 query rows cost
+// the weights' operand as they lie).  With up to 32 query rows the warps divide the tile's keys between two groups and the rows
+// between two, with up to 64 the rows among four; groups are merged once at the end.  What bounds it is reading the cache: 16 query rows cost
 // 16 keys x 128 dims x 2 products of 128 cycles beside 8 KB that an SM receives in 190.
 //
 // Rounding: weights enter the product as two 16-bit pieces (p = hi + lo, 2^-16 of p off with bfloat16), since one piece alone
@@ -12,7 +12,7 @@
 // Maxima, sums and all partial results are fp32; a range's reference maximum is raised only when it grows by 2^8.
 #include <type_traits>
 
-#include "attn_prefix_impl.cuh"
+#include "attn_prefix_frag.cuh"
 #include "flash_common.cuh"
 #include "launch.cuh"
 
@@ -20,38 +20,6 @@ namespace {
 
 constexpr int AM_KEYS = 64;
 constexpr float AM_RESCALE = 8.f;      // log2 units
-
-template <bool HALF>
-__device__ __forceinline__ void am_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (HALF)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void am_ld4(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
-}
-__device__ __forceinline__ void am_ld4t(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
-}
-// two values as pairs of 16-bit pieces
-template <bool HALF>
-__device__ __forceinline__ void am_split(float x, float y, uint32_t& hi, uint32_t& lo) {
-  if constexpr (HALF) {
-    const __half2 h = __floats2half2_rn(x, y);
-    const float2 f = __half22float2(h);
-    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
-    hi = *reinterpret_cast<const uint32_t*>(&h);
-    lo = *reinterpret_cast<const uint32_t*>(&l);
-  } else {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-    hi = *reinterpret_cast<const uint32_t*>(&h);
-    const float2 f = unpack2_bf16(hi);
-    lo = pack2_bf16(x - f.x, y - f.y);
-  }
-}
 
 template <int D>
 struct AmCfg {
@@ -282,10 +250,9 @@ attn_prefix_mma_kernel(AttnPrefixArgs a) {
   pdl_launch_dependents();
   pdl_wait();
   extern __shared__ __align__(128) uint8_t am_smem[];
-  const ApWork w = ap_work(a, a.first_block + blockIdx.x);
+  const ApWork w = ap_work(a, a.first_block + blockIdx.x, threadIdx.x == 0);
   if (w.rows <= 0) return;
-  if (w.rows <= 16) am_body<D, HALF, QS, 4>(a, w, am_smem);
-  else if (w.rows <= 32) am_body<D, HALF, QS, 2>(a, w, am_smem);
+  if (w.rows <= 32) am_body<D, HALF, QS, 2>(a, w, am_smem);
   else am_body<D, HALF, QS, 1>(a, w, am_smem);
 }
 

@@ -53,7 +53,7 @@ attn_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
   using C = AtCfg<D, QS>;
   pdl_launch_dependents();
   pdl_wait();
-  const ApWork w = ap_work(a, a.first_block + blockIdx.x);
+  const ApWork w = ap_work(a, a.first_block + blockIdx.x, threadIdx.x == 0);
   if (w.rows <= 0) return;
   extern __shared__ __align__(1024) uint8_t at_smem[];
   const uint32_t raw = smem_u32(at_smem);
