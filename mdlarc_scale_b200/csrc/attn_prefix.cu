@@ -197,10 +197,9 @@ attn_prefix_join_kernel(AttnPrefixArgs a) {
 
 void fill_plan(AttnPrefixArgs& a) {
   a.rep = a.n_heads / a.n_kv;
-  const bool tc = a.kv_fmt != 2 && (a.act_fmt == a.kv_fmt || a.dim == 64) && a.scale != 0.f &&
-                  (long long)a.n_seqs * a.n_kv * a.t_max < (1ll << 31) - 256;
+  const bool tc = a.kv_fmt != 2 && (a.act_fmt == a.kv_fmt || a.dim == 64) && a.scale != 0.f;
   a.plan = prefix_plan(a.n_groups, a.max_group, a.max_prefix, a.n_items, a.item_end ? a.max_own : 0, a.n_kv, a.rep,
-                       a.kv_fmt == 2, tc, arcb_num_sms());
+                       a.act_fmt != a.kv_fmt && a.dim == 128 ? 16 : 24, a.kv_fmt == 2, tc, arcb_num_sms());
 }
 
 }  // namespace
@@ -233,16 +232,17 @@ int arcb_launch_attn_prefix(AttnPrefixArgs a, cudaStream_t stream) {
     arcb_count_launch(1);
   } else {
     long long units = shared + own;
-    if (p.shared != AP_SHARED_ROWS && shared > 0) {
-      const int r = p.shared == AP_SHARED_TC ? arcb_attn_prefix_tc(a, (unsigned)shared, stream) : (int)arcb_attn_prefix_mma(a, (unsigned)shared, stream);
+    if (p.shared == AP_SHARED_TC && shared > 0) {
+      const int r = arcb_attn_prefix_tc(a, (unsigned)shared, stream);
       arcb_count_launch(1);
       if (r) return r;
       a.first_block = shared;
       units = own;
     }
     if (units > 0) {
-      e = arcb_attn_prefix_rows(a, units, stream);
+      const int r = arcb_attn_prefix_rows(a, units, stream);
       arcb_count_launch(1);
+      if (r) return r;
     }
   }
   if (e == cudaSuccess && p.parts > 1) {
@@ -277,6 +277,7 @@ static int prefix_args(const arcb_prefix_attention_args* p, AttnPrefixArgs& a, b
   a.max_own = bound(p->max_own, p->t_max);
   a.item_end = p->d_item_end; a.scale = p->scale;
   if (!p->n_groups && !p->d_item_end) return arcb_fail(ARCB_E_ARG, "prefix attention needs groups, rows of the items' own, or both");
+  if (a.kv_fmt != 2 && (long long)p->n_seqs * p->n_kv * p->t_max >= (1ll << 31) - 256) return arcb_fail(ARCB_E_UNSUPPORTED, "prefix attention: caches of 2^31 rows");
   if (sizes_only) return ARCB_OK;
   if (!p->d_q || !p->d_k || !p->d_v || !p->d_out) return arcb_fail(ARCB_E_ARG, "null attention argument");
   if (p->n_groups && (!p->d_group_first || !p->d_group_seq || !p->d_group_len)) return arcb_fail(ARCB_E_ARG, "null group arrays");

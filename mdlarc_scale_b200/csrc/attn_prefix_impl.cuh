@@ -14,9 +14,10 @@ struct ApWork {
 };
 
 // Numbers: tiles of one (group, head, range) follow each other, so that they find its rows in L2.
-__device__ __forceinline__ ApWork ap_work(const AttnPrefixArgs& a, long long w, bool report) {
+__device__ __forceinline__ ApWork ap_work(const AttnPrefixArgs& a, long long block, bool report) {
   ApWork k;
-  const long long n1 = (long long)a.n_groups * a.n_kv * a.plan.tiles1 * a.plan.splits1;
+  unsigned w = (unsigned)block;       // fewer than 2^31 (the launcher's check)
+  const unsigned n1 = (unsigned)(a.n_groups * a.n_kv * a.plan.tiles1 * a.plan.splits1);
   int len, at0, split, splits, grain = 15;
   if (w < n1) {
     const int t = (int)(w % a.plan.tiles1); w /= a.plan.tiles1;
@@ -48,7 +49,7 @@ __device__ __forceinline__ ApWork ap_work(const AttnPrefixArgs& a, long long w, 
     k.r0 = t * a.plan.tile1;
     k.rows = min(a.plan.tile1, (last - first) * a.rep - k.r0);
     at0 = 0;
-    grain = a.plan.shared == AP_SHARED_TC ? 127 : a.plan.shared == AP_SHARED_TILES ? 63 : 15;
+    grain = a.plan.shared == AP_SHARED_TC ? 127 : 15;
     k.part = split;
   } else {
     w -= n1;
@@ -90,13 +91,9 @@ __device__ __forceinline__ void ap_store4(void* out, size_t at, float4 v, int fm
   for (int i = 0; i < 4; ++i) reinterpret_cast<__half*>(out)[at + i] = isnan(f[i]) ? __float2half_rn(f[i]) : __float2half_rn(fminf(fmaxf(f[i], -65504.f), 65504.f));
 }
 
-__device__ __forceinline__ void ap_store2(void* out, size_t at, float x, float y, int fmt) {
-  uint32_t v = pack2_act(x, y, fmt);
-  if (fmt == 1) {
-    if (isnan(x)) v = (v & 0xffff0000u) | 0x7fffu;
-    if (isnan(y)) v = (v & 0xffffu) | 0x7fff0000u;
-  }
-  *reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(out) + at) = v;
+__device__ __forceinline__ void ap_store1(void* out, size_t at, float v, int fmt) {
+  if (fmt == 1 && isnan(v)) reinterpret_cast<__half*>(out)[at] = __float2half_rn(v);
+  else st_act(out, at, v, fmt);
 }
 
 }  // namespace

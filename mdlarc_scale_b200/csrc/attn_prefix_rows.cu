@@ -1,56 +1,108 @@
-// Attention over shared cached rows in 16-bit formats for up to 16 query rows at a time: the rows of an item's own, and shared
-// rows that few queries see.
+// Attention over shared cached rows in 16-bit formats for few query rows at a time: the rows of an item's own, and shared
+// rows that up to 24 query rows see.
 //
-// A unit of work is a range of one sequence's cached rows and up to 16 query rows.  A warp takes units by itself: keys and values
-// are copied asynchronously into a ring of its own (16-byte pieces, exclusive-or swizzled by the row), and the ring runs on
-// into the next unit (its queries with its first tile) while this one is finished, so that a unit's start costs no wait and
-// short ranges stream as long ones do.  There is no barrier between warps: every unit writes a part of the result.  S = Q K^T and
-// O += P V are m16n8k16 products with fp32 sums; queries, sums and weights stay in registers.  What bounds it is reading the cache.
+// A unit of work is a range of one sequence's cached rows and up to 24 query rows.  A warp takes units by itself: keys and values
+// travel by TMA into a ring of its own (boxes of 64 columns, 128-byte swizzle), and the ring runs on into the next unit (its
+// queries with its first tile) while this one is finished, so that a unit's start costs no wait and short ranges stream as
+// long ones do.  There is no barrier between warps: every unit writes a part of the result.
 // Descriptions of units are worked out for 32 units of a warp at once, one a lane.
 //
-// Rounding as in attn_prefix_mma.cu: weights are two 16-bit pieces, half queries over a bfloat16 cache too.
-#include "attn_prefix_frag.cuh"
+// The products are transposed, so that the eight columns of m16n8k16 are queries: S^T = K Q^T (16 keys a product) and O^T += V^T P^T
+// (16 value columns a product); weights change from the first one's result to the second one's operand by 8 x 8 transpositions
+// in the warp.  These products are slow here, 14 cycles each, and with 16 queries a product most of them would be padding.  What
+// bounds it is reading the cache.
+//
+// Rounding: a weight enters the product as two 16-bit pieces (p = hi + lo), since one piece alone would be as far off as the
+// output's own rounding; half queries over a bfloat16 cache are two bfloat16 pieces, which is exact.  With up to four query rows the
+// weights' pieces are columns of their own and cost nothing; with more than 16 in equal formats weights are one piece (sqrt 2 of the
+// output's own rounding error in all), where a second one would bind the kernel to its products.  Maxima, sums and all partial
+// results are fp32; a range's reference maximum is raised only when it grows by 2^8.
+#include "attn_prefix_impl.cuh"
 #include "flash_common.cuh"
 #include "gemm.cuh"
 #include "launch.cuh"
+
+using namespace sm100;
 
 namespace {
 
 constexpr float AR_RESCALE = 8.f;      // log2 units
 constexpr int AR_WARPS = 4;
 
-template <int D>
+template <bool HALF>
+__device__ __forceinline__ void ar_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (HALF)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ar_ld4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ar_ld4t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ uint32_t ar_transpose(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+// two values as pairs of 16-bit pieces
+template <bool HALF>
+__device__ __forceinline__ void ar_split(float x, float y, uint32_t& hi, uint32_t& lo) {
+  if constexpr (HALF) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+  } else {
+    hi = pack2_bf16(x, y);
+    const float2 f = unpack2_bf16(hi);
+    lo = pack2_bf16(x - f.x, y - f.y);
+  }
+}
+
+// MOST: the most query rows of a unit of the launch, in eights.
+template <int D, int MOST>
 struct ArCfg {
+  static constexpr int CTAS = MOST == 1 ? 3 : 2;           // of an SM
   static constexpr int KEYS = D == 64 ? 32 : 16;           // of a tile
-  static constexpr int STAGES = 3;
+  static constexpr int STAGES = MOST == 1 ? 2 : 3;
+  static constexpr int BOX = KEYS * 128;
   static constexpr int PLANE = KEYS * D * 2;
   static constexpr int STAGE = 2 * PLANE;
-  static constexpr int Q_BYTES = 16 * D * 2;
-  static constexpr int WARP = STAGES * STAGE + Q_BYTES;
-  static constexpr int SMEM = AR_WARPS * WARP;
-  static_assert(2 * (SMEM + 1024) <= 228 * 1024, "two CTAs an SM");
+  static constexpr int Q_ROWS = MOST == 1 ? 8 : 16;        // that travel with a unit's first tile; more are read when it starts
+  static constexpr int Q_BYTES = Q_ROWS * D * 2;
+  static constexpr int WARP = STAGES * STAGE + Q_BYTES;    // a multiple of 1 KB: the swizzle goes by the address
+  static_assert(WARP % 1024 == 0 && STAGE % 1024 == 0, "swizzled boxes");
+  static constexpr int SMEM = AR_WARPS * (WARP + 8 * STAGES);      // no room to align: without static shared memory it starts aligned
+  static_assert(CTAS * (SMEM + 1024) <= 228 * 1024, "CTAs of an SM");
 };
 
-template <int D, bool HALF, bool QS>
-__global__ void __launch_bounds__(AR_WARPS * 32, 2)
-attn_prefix_rows_kernel(AttnPrefixArgs a, long long n_units) {
-  using C = ArCfg<D>;
-  constexpr int NT = C::KEYS / 8, DK = D / 16, CH = D / 8;
-  pdl_launch_dependents();
-  pdl_wait();
-  extern __shared__ __align__(128) uint8_t ar_smem[];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(ar_smem)) + warp * C::WARP, q_slot = ring + C::STAGES * C::STAGE;
-  const long long n_warps = (long long)gridDim.x * AR_WARPS, mine = (long long)warp * gridDim.x + blockIdx.x;
-  if (mine >= n_units) return;
-  const int n = (int)((n_units - mine + n_warps - 1) / n_warps);          // units of this warp
-
+// What a warp keeps from unit to unit.
+template <int D, int MOST>
+struct ArWarp {
+  using C = ArCfg<D, MOST>;
+  const AttnPrefixArgs& a;
+  const CUtensorMap* maps[2];
+  long long first, stride, n_units;        // this warp's units
+  int n, lane;
+  uint32_t ring, q_slot, bars;
   ApWork batch;
-  int batch_of = -1;
-  auto unit = [&](int i) {
+  int batch_of;
+  ApWork ahead;                            // the unit that tiles are asked for of, its number, its tiles that have not been, and
+  int ahead_i, ahead_left, ahead_row;      // the next one's first row in the cache
+  int flight, put, get;                    // tiles asked for and not used up
+  uint32_t phase;                          // of the slot that is used next
+  bool ok;
+
+  __device__ __forceinline__ ApWork unit(int i) {
     if (i >> 5 != batch_of) {
       batch_of = i >> 5;
-      const long long u = mine + (long long)((batch_of << 5) + lane) * n_warps;
+      const long long u = first + (long long)((batch_of << 5) + lane) * stride;
       if (u < n_units) batch = ap_work(a, a.first_block + u, true);
     }
     ApWork w;
@@ -65,221 +117,372 @@ attn_prefix_rows_kernel(AttnPrefixArgs a, long long n_units) {
     w.part = __shfl_sync(0xffffffffu, batch.part, from);
     if (w.rows <= 0) w.end = w.begin;
     return w;
-  };
-  const int col = lane % CH, row = lane / CH;      // a lane copies piece `col` of rows row, row + 32 / CH, ...
-  // tile t of unit w into slot `put`, with the queries when it is the first
-  auto issue = [&](const ApWork& w, int t, int put) {
-    const uint32_t st = ring + put * C::STAGE;
-    const size_t row0 = (((size_t)w.seq * a.n_kv + w.kvh) * (size_t)a.t_max + w.begin) * CH + col;
-    const int left = w.end - w.begin - t * C::KEYS;
-#pragma unroll
-    for (int plane = 0; plane < 2; ++plane) {
-      const char* src = reinterpret_cast<const char*>(plane ? a.v : a.k) + row0 * 16;
-#pragma unroll
-      for (int i = 0; i < C::KEYS * CH / 32; ++i) {
-        const int r = row + i * (32 / CH);
-        const bool ok = r < left;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(st + plane * C::PLANE + r * (CH * 16) + ((col ^ (r & 7)) << 4)),
-                     "l"(src + (size_t)(ok ? t * C::KEYS + r : 0) * (CH * 16)), "r"(ok ? 16 : 0) : "memory");
-      }
+  }
+  static __device__ __forceinline__ int tiles_of(const ApWork& w) { return (w.end - w.begin + C::KEYS - 1) / C::KEYS; }
+  // query row r of a unit
+  __device__ __forceinline__ const char* query(const ApWork& w, int r) const {
+    const int R = w.r0 + r;
+    return reinterpret_cast<const char*>(a.q) + ((size_t)(w.item0 + R / a.rep) * a.q_pitch + (size_t)(w.kvh * a.rep + R % a.rep) * D) * 2;
+  }
+  __device__ __forceinline__ void look_at(const ApWork& w) {
+    ahead = w;
+    ahead_left = tiles_of(w);
+    ahead_row = (w.seq * a.n_kv + w.kvh) * a.t_max + w.begin;
+  }
+  // the next tile into slot `put`, with the unit's queries when it is the first
+  __device__ __forceinline__ void issue() {
+    const uint32_t bar = bars + 8 * put, st = ring + put * C::STAGE;
+    const bool first_tile = ahead_left == tiles_of(ahead);
+    uint32_t bytes = C::STAGE;
+    if (first_tile && ahead.rows <= C::Q_ROWS) {
+      bytes += ahead.rows * D * 2;
+      if (lane < ahead.rows)
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(q_slot + lane * D * 2),
+                     "l"(query(ahead, lane)), "r"(D * 2), "r"(bar) : "memory");
     }
-    if (t == 0) {
-      const char* q = reinterpret_cast<const char*>(a.q) + col * 16;
+    if (lane == 0) {
+      mbar_expect_tx(bar, bytes);
 #pragma unroll
-      for (int i = 0; i < 16 * CH / 32; ++i) {
-        const int r = row + i * (32 / CH), R = w.r0 + r;
-        const bool ok = r < w.rows;
-        const size_t at = ok ? ((size_t)(w.item0 + R / a.rep) * a.q_pitch + (size_t)(w.kvh * a.rep + R % a.rep) * D) * 2 : 0;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(q_slot + r * (CH * 16) + ((col ^ (r & 7)) << 4)), "l"(q + at), "r"(ok ? 16 : 0) : "memory");
-      }
+      for (int plane = 0; plane < 2; ++plane)
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) tma_load_2d(st + plane * C::PLANE + c * C::BOX, maps[plane], c * 64, ahead_row, bar);
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-  auto tiles_of = [&](const ApWork& w) { return (w.end - w.begin + C::KEYS - 1) / C::KEYS; };
+    ahead_row += C::KEYS;
+    --ahead_left;
+    put = put + 1 == C::STAGES ? 0 : put + 1;
+    ++flight;
+  }
+  // Asks for tiles while there is room, up to the end of the unit behind unit i; into that (cross) only when the queries of
+  // unit i have left their slot.
+  __device__ __forceinline__ void ask(int i, bool cross) {
+    while (flight < C::STAGES) {
+      if (ahead_left == 0) {
+        if (!cross || ahead_i != i || i + 1 == n) break;
+        look_at(unit(++ahead_i));
+        if (ahead_left == 0) break;
+      }
+      issue();
+    }
+  }
+};
 
+// One unit for 8 QT query rows.  PAIR: up to four rows; columns 4 to 7 of the products are second pieces of weights.
+template <int D, int MOST, bool HALF, bool QS, int QT, bool PAIR>
+__device__ __forceinline__ void ar_unit(ArWarp<D, MOST>& s, const ApWork& w, int i) {
+  using C = ArCfg<D, MOST>;
+  constexpr int DK = D / 16, MT = C::KEYS / 16;
+  constexpr bool P2 = !PAIR && (QS || QT <= 2);          // second pieces of weights as products of their own
+  const AttnPrefixArgs& a = s.a;
+  const int lane = s.lane;
   const float sc = fabsf(a.scale) * AP_LOG2E;
   const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;        // a negative scale turns the queries, so that maxima are maxima
-  const bool whole = a.plan.parts == 1;
-
-  ApWork cur = unit(0), ahead = cur;       // the unit at work, and the one that tiles are asked for of
-  int ahead_i = 0, ahead_t = 0;            // its number, and its next tile
-  int flight = 0, put = 0, get = 0;        // tiles asked for and not used up
-  for (int i = 0; i < n; ++i) {
-    const int tiles = tiles_of(cur);
-    // asks for tiles while there is room, up to the end of the next unit; into that (cross) only when this one's queries have
-    // left their slot
-    auto ask = [&](bool cross) {
-      while (flight < C::STAGES) {
-        if (ahead_t == tiles_of(ahead)) {
-          if (!cross || ahead_i != i || i + 1 == n) break;
-          ahead = unit(++ahead_i);
-          ahead_t = 0;
-          if (tiles_of(ahead) == 0) break;
-        }
-        issue(ahead, ahead_t++, put);
-        put = put + 1 == C::STAGES ? 0 : put + 1;
-        ++flight;
-      }
-    };
-    uint32_t q[DK][4], ql[QS ? DK : 1][4];
-    float acc[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  const int tiles = s.tiles_of(w);
+  // A lane has queries (lane % 4) * 2 and the next one of every eight (PAIR: of the first four), and keys or value columns lane / 4
+  // and that plus 8 of every 16.
+  uint32_t q[QT][DK][2], q2[QS ? QT : 1][QS ? DK : 1][2];
+  float acc[QT][DK][4], m[QT][2], off[QT][2], l[QT][2];          // off: what is taken off a score, -m or 0
 #pragma unroll
-    for (int e = 0; e < D / 8; ++e) acc[e][0] = acc[e][1] = acc[e][2] = acc[e][3] = 0.f;
-    for (int t = 0; t < tiles; ++t) {
-      __syncwarp();                        // everybody is done with the tile before, whose slot is asked for now
-      ask(t > 0);
-      if (flight == 1) asm volatile("cp.async.wait_group 0;" ::: "memory");
-      else if (flight == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
-      else asm volatile("cp.async.wait_group 2;" ::: "memory");
-      static_assert(C::STAGES == 3, "waits for one to three tiles under way");
+  for (int b = 0; b < QT; ++b) {
+    m[b][0] = m[b][1] = -INFINITY;
+    off[b][0] = off[b][1] = l[b][0] = l[b][1] = 0.f;
+#pragma unroll
+    for (int e = 0; e < DK; ++e) acc[b][e][0] = acc[b][e][1] = acc[b][e][2] = acc[b][e][3] = 0.f;
+  }
+  auto keep_query = [&](int b, int ks, int y, uint32_t raw) {
+    if constexpr (QS) {
+      const float2 f = unpack2_act(raw ^ flip, 1);
+      ar_split<false>(f.x, f.y, q[b][ks][y], q2[b][ks][y]);
+    } else {
+      q[b][ks][y] = raw ^ flip;
+    }
+  };
+  // Pieces of matrix loads: row (lane % 16) and row (lane % 8) + 8 (lane / 16) of 16; 16-byte piece 2 ks + h lies at (2 ks + h) ^ row % 8,
+  // which is one exclusive-or of the address with 32 ks.
+  const uint32_t k_at = (lane & 15) * 128 + (((lane >> 4) ^ (lane & 7)) << 4);
+  const uint32_t v_at = ((lane & 7) + ((lane >> 4) << 3)) * 128 + ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
+  for (int t = 0; t < tiles; ++t) {
+    __syncwarp();                          // everybody is done with the tile before, whose slot is asked for now
+    s.ask(i, t > 0);
+    if (!__all_sync(0xffffffffu, mbar_wait_bounded(s.bars + 8 * s.get, s.phase))) {
+      arcb_set_error(a.status, ARCB_DEV_WAIT_TIMEOUT_TMA);
+      s.ok = false;
+      return;
+    }
+    if (t == 0) {
+#pragma unroll
+      for (int b = 0; b < QT; ++b) {
+        if constexpr (8 * QT <= C::Q_ROWS) {
+          const int r = min(b * 8 + (lane & (PAIR ? 3 : 7)), w.rows - 1);      // rows that do not exist are as the last one
+#pragma unroll
+          for (int ks = 0; ks < DK; ks += 2) {
+            uint32_t in[4];
+            ar_ld4(s.q_slot + r * (D * 2) + ((2 * ks + (lane >> 3)) << 4), in);
+            keep_query(b, ks, 0, in[0]);
+            keep_query(b, ks, 1, in[1]);
+            keep_query(b, ks + 1, 0, in[2]);
+            keep_query(b, ks + 1, 1, in[3]);
+          }
+        } else {
+          const char* src = s.query(w, min(b * 8 + (lane >> 2), w.rows - 1)) + (lane & 3) * 4;
+#pragma unroll
+          for (int ks = 0; ks < DK; ++ks)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) keep_query(b, ks, y, *reinterpret_cast<const uint32_t*>(src + ks * 32 + y * 16));
+        }
+      }
       __syncwarp();
-      if (t == 0) {
+      s.ask(i, true);
+    }
+    const uint32_t kst = s.ring + s.get * C::STAGE + k_at, vst = s.ring + s.get * C::STAGE + C::PLANE + v_at;
+    s.get = s.get + 1 == C::STAGES ? 0 : s.get + 1;
+    s.phase ^= s.get == 0;
+    --s.flight;
+    const int left = w.end - w.begin - t * C::KEYS;        // keys of the tile
+    const bool some = left < C::KEYS;
+    float p[QT][MT][4];
 #pragma unroll
-        for (int ks = 0; ks < DK; ++ks) {
-          const int r = lane & 15;
-          uint32_t in[4];
-          am_ld4(q_slot + r * (CH * 16) + (((2 * ks + (lane >> 4)) ^ (r & 7)) << 4), in);
+    for (int b = 0; b < QT; ++b)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if constexpr (QS) {
-              const float2 f = unpack2_act(in[e] ^ flip, 1);
-              am_split<false>(f.x, f.y, q[ks][e], ql[ks][e]);
-            } else {
-              q[ks][e] = in[e] ^ flip;
-            }
-          }
+      for (int mt = 0; mt < MT; ++mt) p[b][mt][0] = p[b][mt][1] = p[b][mt][2] = p[b][mt][3] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < DK; ++ks) {
+      const uint32_t at = (kst ^ ((ks & 3) << 5)) + (ks >> 2) * C::BOX;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        uint32_t k[4];
+        ar_ld4(at + mt * (16 * 128), k);
+#pragma unroll
+        for (int b = 0; b < QT; ++b) {
+          ar_mma<HALF>(p[b][mt], k, q[b][ks][0], q[b][ks][1]);
+          if constexpr (QS) ar_mma<HALF>(p[b][mt], k, q2[b][ks][0], q2[b][ks][1]);
         }
-        __syncwarp();
-        ask(true);
       }
-      const uint32_t kst = ring + get * C::STAGE, vst = kst + C::PLANE;
-      get = get + 1 == C::STAGES ? 0 : get + 1;
-      --flight;
-      const int left = cur.end - cur.begin - t * C::KEYS;        // keys of the tile
-      float s[NT][4];
+    }
+    if (some)
 #pragma unroll
-      for (int e = 0; e < NT; ++e) s[e][0] = s[e][1] = s[e][2] = s[e][3] = 0.f;
+      for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-      for (int ks = 0; ks < DK; ++ks)
+        for (int j = 0; j < 4; ++j)
+          if (mt * 16 + (lane >> 2) + (j >> 1) * 8 >= left)
 #pragma unroll
-        for (int e = 0; e < NT; e += 2) {
-          const int r = e * 8 + (lane & 7) + ((lane >> 4) << 3);
-          uint32_t b[4];
-          am_ld4(kst + r * (CH * 16) + (((2 * ks + ((lane >> 3) & 1)) ^ (r & 7)) << 4), b);
-          am_mma<HALF>(s[e], q[ks], b[0], b[1]);
-          am_mma<HALF>(s[e + 1], q[ks], b[2], b[3]);
-          if constexpr (QS) {
-            am_mma<HALF>(s[e], ql[ks], b[0], b[1]);
-            am_mma<HALF>(s[e + 1], ql[ks], b[2], b[3]);
-          }
-        }
-      const bool some = left < C::KEYS;
-      if (some)
+            for (int b = 0; b < QT; ++b) p[b][mt][j] = -INFINITY;
+    // the lanes' own maxima tell whether any reference has to be raised; only then are they exchanged
+    float top[QT][2];
+    bool raise = t == 0;
 #pragma unroll
-        for (int e = 0; e < NT; ++e)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (e * 8 + (lane & 3) * 2 + (j & 1) >= left) s[e][j] = -INFINITY;
-      float alpha[2] = {1.f, 1.f};
-      bool raise = false;
+    for (int b = 0; b < QT; ++b)
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        float mx = fmaxf(s[0][2 * x], s[0][2 * x + 1]);
+        float mx = fmaxf(p[b][0][x], p[b][0][2 + x]);
 #pragma unroll
-        for (int e = 1; e < NT; ++e) mx = max3_f32(mx, s[e][2 * x], s[e][2 * x + 1]);
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        mx = mx == -INFINITY ? -INFINITY : mx * sc;
-        if (mx > m[x] + AR_RESCALE || (m[x] == -INFINITY && mx > -INFINITY)) {
-          alpha[x] = m[x] == -INFINITY ? 0.f : ex2_fast(m[x] - mx);
-          raise = true;
-          m[x] = mx;
+        for (int mt = 1; mt < MT; ++mt) mx = max3_f32(mx, p[b][mt][x], p[b][mt][2 + x]);
+        top[b][x] = mx;
+        raise |= mx * sc > m[b][x] + AR_RESCALE;
+      }
+    if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+      for (int b = 0; b < QT; ++b)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          float mx = top[b][x];
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+          mx = fmaxf(mx == -INFINITY ? -INFINITY : mx * sc, m[b][x]);
+          if (mx == -INFINITY) continue;
+          const float alpha = m[b][x] == -INFINITY ? 0.f : ex2_fast(m[b][x] - mx);
+          m[b][x] = mx;
+          off[b][x] = -mx;
+          l[b][x] *= alpha;
+#pragma unroll
+          for (int e = 0; e < DK; ++e) {
+            acc[b][e][x] *= alpha;
+            acc[b][e][2 + x] *= alpha;
+          }
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < QT; ++b)
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p[b][mt][j] = ex2_fast(fmaf(p[b][mt][j], sc, off[b][j & 1]));
+    if (some)                              // for a scale of 0, whose product with -inf is NaN
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (mt * 16 + (lane >> 2) + (j >> 1) * 8 >= left)
+#pragma unroll
+            for (int b = 0; b < QT; ++b) p[b][mt][j] = 0.f;
+#pragma unroll
+    for (int b = 0; b < QT; ++b)
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) l[b][j & 1] += p[b][mt][j];
+    uint32_t hi[QT][MT][2], lo[QT][P2 ? MT : 1][2];
+#pragma unroll
+    for (int b = 0; b < QT; ++b)
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          uint32_t h, o = 0u;
+          if constexpr (PAIR || P2) ar_split<HALF>(p[b][mt][2 * y], p[b][mt][2 * y + 1], h, o);
+          else h = pack2_prob(p[b][mt][2 * y], p[b][mt][2 * y + 1], HALF ? 1 : 0);
+          hi[b][mt][y] = ar_transpose(PAIR && (lane & 2) ? o : h);
+          if constexpr (P2) lo[b][mt][y] = ar_transpose(o);
+        }
+    if (!some) {
+#pragma unroll
+      for (int dt = 0; dt < DK; ++dt) {
+        const uint32_t at = (vst ^ ((dt & 3) << 5)) + (dt >> 2) * C::BOX;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          uint32_t v[4];
+          ar_ld4t(at + mt * (16 * 128), v);
+#pragma unroll
+          for (int b = 0; b < QT; ++b) {
+            ar_mma<HALF>(acc[b][dt], v, hi[b][mt][0], hi[b][mt][1]);
+            if constexpr (P2) ar_mma<HALF>(acc[b][dt], v, lo[b][mt][0], lo[b][mt][1]);
+          }
         }
       }
-      if (__any_sync(0xffffffffu, raise)) {
-        l[0] *= alpha[0];
-        l[1] *= alpha[1];
+    } else {
+      // values behind the end: a weight of 0 does not hide a NaN
+      uint32_t keep[MT][2];
 #pragma unroll
-        for (int e = 0; e < D / 8; ++e) {
-          acc[e][0] *= alpha[0]; acc[e][1] *= alpha[0];
-          acc[e][2] *= alpha[1]; acc[e][3] *= alpha[1];
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const int k0 = mt * 16 + y * 8 + (lane & 3) * 2;
+          keep[mt][y] = (k0 < left ? 0xffffu : 0u) | (k0 + 1 < left ? 0xffff0000u : 0u);
         }
-      }
-      const float safe[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+#pragma unroll 1
+      for (int dt = 0; dt < DK; ++dt) {
+        const uint32_t at = (vst ^ ((dt & 3) << 5)) + (dt >> 2) * C::BOX;
+        float sum[QT][4];
 #pragma unroll
-      for (int e = 0; e < NT; ++e)
+        for (int b = 0; b < QT; ++b) sum[b][0] = sum[b][1] = sum[b][2] = sum[b][3] = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float p = ex2_fast(fmaf(s[e][j], sc, -safe[j >> 1]));
-          if (some && e * 8 + (lane & 3) * 2 + (j & 1) >= left) p = 0.f;     // also where the scale is 0
-          l[j >> 1] += p;
-          s[e][j] = p;
+        for (int mt = 0; mt < MT; ++mt) {
+          uint32_t v[4];
+          ar_ld4t(at + mt * (16 * 128), v);
+          v[0] &= keep[mt][0]; v[1] &= keep[mt][0];
+          v[2] &= keep[mt][1]; v[3] &= keep[mt][1];
+#pragma unroll
+          for (int b = 0; b < QT; ++b) {
+            ar_mma<HALF>(sum[b], v, hi[b][mt][0], hi[b][mt][1]);
+            if constexpr (P2) ar_mma<HALF>(sum[b], v, lo[b][mt][0], lo[b][mt][1]);
+          }
         }
 #pragma unroll
-      for (int kk = 0; kk < C::KEYS / 16; ++kk) {
-        uint32_t hi[4], lo[4];
-        am_split<HALF>(s[2 * kk][0], s[2 * kk][1], hi[0], lo[0]);
-        am_split<HALF>(s[2 * kk][2], s[2 * kk][3], hi[1], lo[1]);
-        am_split<HALF>(s[2 * kk + 1][0], s[2 * kk + 1][1], hi[2], lo[2]);
-        am_split<HALF>(s[2 * kk + 1][2], s[2 * kk + 1][3], hi[3], lo[3]);
-        const int r = kk * 16 + (lane & 15);
+        for (int e = 0; e < DK; ++e)
+          if (e == dt)
 #pragma unroll
-        for (int dt = 0; dt < DK; ++dt) {
-          uint32_t b[4];
-          am_ld4t(vst + r * (CH * 16) + (((2 * dt + (lane >> 4)) ^ (r & 7)) << 4), b);
-          am_mma<HALF>(acc[2 * dt], hi, b[0], b[1]);
-          am_mma<HALF>(acc[2 * dt + 1], hi, b[2], b[3]);
-          am_mma<HALF>(acc[2 * dt], lo, b[0], b[1]);
-          am_mma<HALF>(acc[2 * dt + 1], lo, b[2], b[3]);
-        }
+            for (int b = 0; b < QT; ++b)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) acc[b][e][j] += sum[b][j];
       }
     }
-    // the unit's part of the result
+  }
+  // The unit's part of the result: eight lanes have eight neighbouring value columns of a query.
+  const bool whole = a.plan.parts == 1;
+#pragma unroll
+  for (int b = 0; b < QT; ++b) {
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
-      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
-      const int r = (lane >> 2) + 8 * x, R = cur.r0 + r;
-      if (r >= cur.rows) continue;
-      const int item = cur.item0 + R / a.rep;
-      const long long ih = (long long)item * a.n_heads + cur.kvh * a.rep + R % a.rep;
-      if (whole) {
-        const bool none = l[x] == 0.f || (a.item_skip && a.item_skip[item]);
-        const float inv = 1.f / l[x];
+      if (b * 8 + x >= w.rows) continue;
 #pragma unroll
-        for (int e = 0; e < D / 8; ++e)
-          ap_store2(a.out, (size_t)ih * D + e * 8 + (lane & 3) * 2, none ? 0.f : acc[e][2 * x] * inv, none ? 0.f : acc[e][2 * x + 1] * inv, a.act_fmt);
-      } else {
-        float* to = ap_record(a, ih, cur.part);
-        if (tiles > 0)
+      for (int o = 4; o <= 16; o <<= 1) l[b][x] += __shfl_xor_sync(0xffffffffu, l[b][x], o);
+      const int r = b * 8 + (lane & (PAIR ? 1 : 3)) * 2 + x;
+      const bool in = r < w.rows && !(PAIR && (lane & 2));
+      const int R = w.r0 + (in ? r : 0), item = w.item0 + R / a.rep;
+      const long long ih = (long long)item * a.n_heads + w.kvh * a.rep + R % a.rep;
+      const float inv = l[b][x] == 0.f || (whole && in && a.item_skip && a.item_skip[item]) ? 0.f : 1.f / l[b][x];
+      float* to = whole ? nullptr : ap_record(a, ih, w.part) + (lane >> 2);
 #pragma unroll
-          for (int e = 0; e < D / 8; ++e) *reinterpret_cast<float2*>(to + e * 8 + (lane & 3) * 2) = make_float2(acc[e][2 * x], acc[e][2 * x + 1]);
-        if ((lane & 3) == 0) *reinterpret_cast<float2*>(to + D) = make_float2(m[x], l[x]);
-      }
-    }
-    if (i + 1 < n) {
-      if (ahead_i == i) {
-        ahead = unit(++ahead_i);
-        ahead_t = 0;
-      }
-      cur = ahead;
+      for (int e = 0; e < DK; ++e)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          float v = acc[b][e][2 * y + x];
+          if constexpr (PAIR) v += __shfl_xor_sync(0xffffffffu, v, 2);
+          if (!in) continue;
+          if (whole) ap_store1(a.out, (size_t)ih * D + e * 16 + y * 8 + (lane >> 2), inv == 0.f ? 0.f : v * inv, a.act_fmt);
+          else if (tiles > 0) to[e * 16 + y * 8] = v;
+        }
+      if (in && !whole && lane < 4) *reinterpret_cast<float2*>(to + D) = make_float2(m[b][x], l[b][x]);
     }
   }
 }
 
-template <int D, bool HALF, bool QS>
-cudaError_t ar_launch(const AttnPrefixArgs& a, long long units, cudaStream_t stream) {
+template <int D, int MOST, bool HALF, bool QS>
+__global__ void __launch_bounds__(AR_WARPS * 32, (ArCfg<D, MOST>::CTAS))
+attn_prefix_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, AttnPrefixArgs a, long long n_units) {
+  using C = ArCfg<D, MOST>;
+  pdl_launch_dependents();
+  pdl_wait();
+  extern __shared__ __align__(1024) uint8_t ar_smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long stride = (long long)gridDim.x * AR_WARPS, first = (long long)warp * gridDim.x + blockIdx.x;
+  if (first >= n_units) return;
+  const uint32_t base = smem_u32(ar_smem), ring = base + warp * C::WARP, bars = base + AR_WARPS * C::WARP + warp * (8 * C::STAGES);
+  if (base & 1023u) {
+    arcb_set_error(a.status, ARCB_DEV_BAD_INDEX);
+    return;
+  }
+  if (lane == 0) {
+    for (int i = 0; i < C::STAGES; ++i) mbar_init(bars + 8 * i, 1);
+    mbar_fence_init();
+  }
+  __syncwarp();
+  ArWarp<D, MOST> s{a, {&tmap_k, &tmap_v}, first, stride, n_units, (int)((n_units - first + stride - 1) / stride), lane, ring, ring + C::STAGES * C::STAGE, bars};
+  s.batch_of = -1;
+  s.flight = s.put = s.get = s.ahead_i = 0;
+  s.phase = 0;
+  s.ok = true;
+  ApWork w = s.unit(0);
+  s.look_at(w);
+  for (int i = 0; i < s.n && s.ok; ++i) {
+    if (w.rows <= 4) ar_unit<D, MOST, HALF, QS, 1, true>(s, w, i);
+    else if (MOST == 1 || w.rows <= 8) ar_unit<D, MOST, HALF, QS, 1, false>(s, w, i);
+    else if constexpr (MOST > 1) {
+      if (w.rows <= 16) ar_unit<D, MOST, HALF, QS, 2, false>(s, w, i);
+      else if constexpr (!(QS && D == 128)) ar_unit<D, MOST, HALF, QS, 3, false>(s, w, i);
+    }
+    if (i + 1 < s.n) {
+      if (s.ahead_i == i) s.look_at(s.unit(++s.ahead_i));
+      w = s.ahead;
+    }
+  }
+}
+
+template <int D, int MOST, bool HALF, bool QS>
+int ar_launch(const AttnPrefixArgs& a, long long units, cudaStream_t stream) {
+  using C = ArCfg<D, MOST>;
   static std::atomic<unsigned long long> done{0};
-  const cudaError_t e = arcb_opt_in_smem(attn_prefix_rows_kernel<D, HALF, QS>, ArCfg<D>::SMEM, done);
-  if (e != cudaSuccess) return e;
-  const long long most = 2LL * arcb_num_sms();
-  return arcb_launch(attn_prefix_rows_kernel<D, HALF, QS>, dim3((unsigned)(units < most ? units : most)), dim3(AR_WARPS * 32), ArCfg<D>::SMEM, stream, a, units);
+  const cudaError_t e = arcb_opt_in_smem(attn_prefix_rows_kernel<D, MOST, HALF, QS>, C::SMEM, done);
+  if (e != cudaSuccess) return (int)e;
+  CUtensorMap tk, tv;
+  const uint64_t rows = (uint64_t)a.n_seqs * a.n_kv * a.t_max;
+  int r = arcb_make_tmap_2d_16b(&tk, a.k, rows, D, C::KEYS, 64, HALF);
+  if (!r) r = arcb_make_tmap_2d_16b(&tv, a.v, rows, D, C::KEYS, 64, HALF);
+  if (r) return 1000 + r;
+  const long long most = (long long)C::CTAS * arcb_num_sms();
+  return (int)arcb_launch(attn_prefix_rows_kernel<D, MOST, HALF, QS>, dim3((unsigned)(units < most ? units : most)), dim3(AR_WARPS * 32), C::SMEM, stream, tk, tv,
+                          a, units);
+}
+template <int D, bool HALF, bool QS>
+int ar_launch(const AttnPrefixArgs& a, long long units, bool eight, cudaStream_t stream) {
+  return eight ? ar_launch<D, 1, HALF, QS>(a, units, stream) : ar_launch<D, 3, HALF, QS>(a, units, stream);
 }
 
 }  // namespace
 
-cudaError_t arcb_attn_prefix_rows(const AttnPrefixArgs& a, long long units, cudaStream_t stream) {
-  if (a.kv_fmt == 1) return a.dim == 64 ? ar_launch<64, true, false>(a, units, stream) : ar_launch<128, true, false>(a, units, stream);
-  if (a.act_fmt == 1) return a.dim == 64 ? ar_launch<64, false, true>(a, units, stream) : ar_launch<128, false, true>(a, units, stream);
-  return a.dim == 64 ? ar_launch<64, false, false>(a, units, stream) : ar_launch<128, false, false>(a, units, stream);
+int arcb_attn_prefix_rows(const AttnPrefixArgs& a, long long units, cudaStream_t stream) {
+  const bool eight = a.plan.rows <= 8;
+  if (a.kv_fmt == 1) return a.dim == 64 ? ar_launch<64, true, false>(a, units, eight, stream) : ar_launch<128, true, false>(a, units, eight, stream);
+  if (a.act_fmt == 1) return a.dim == 64 ? ar_launch<64, false, true>(a, units, eight, stream) : ar_launch<128, false, true>(a, units, eight, stream);
+  return a.dim == 64 ? ar_launch<64, false, false>(a, units, eight, stream) : ar_launch<128, false, false>(a, units, eight, stream);
 }

@@ -4,9 +4,9 @@
 // 128 at a time.  With up to 128 rows B has the same queries as A and takes every other key tile, so that there are always two
 // chains (scores, softmax, weights, values) of which one is in the tensor core while the other is at its exponentials; A's and
 // B's sums are then two parts of the result.
-//   warp 0        TMA: key and value tiles as 128 x 64 boxes with the 128-byte swizzle, rings shared by A and B
+//   warp 0        TMA: key and value tiles as 128 x 64 boxes with the 128-byte swizzle, rings shared by A and B; value rows
+//                 behind the end of the last tile are set to zero: a weight of 0 does not hide a NaN
 //   warps 1, 2    products of A and of B: S = Q K^T (128 TMEM columns), O += P V with P read from TMEM
-//   warp 3        sets the value rows behind the end of the last tile to zero: a weight of 0 does not hide a NaN
 //   warps 4-19    two threads a query row, 64 keys of every tile each: maxima (exchanged), exponentials, row sums, P over the
 //                 thread's own score columns
 // Maxima, sums and results are fp32.  The reference maximum of a row is raised only when it grows by 2^8.  Half queries over a
@@ -161,6 +161,21 @@ attn_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
           for (int c = 0; c < C::BOXES; ++c) tma_load_2d(v_smem + s * C::KV_BYTES + c * AT_BOX, &tmap_v, c * 64, row + j * AT_KEYS, b_vfull + 8 * s);
         }
       }
+      if (ok && n_tiles > 0 && left < AT_KEYS) {
+        // this warp has seen the slot's earlier tiles go, so that the barrier's parity can only mean this one
+        const int s = (n_tiles - 1) % C::STAGES;
+        if (__all_sync(0xffffffffu, mbar_wait_bounded(b_vfull + 8 * s, ((n_tiles - 1) / C::STAGES) & 1))) {
+          uint8_t* v = base_ptr + 2 * C::Q_BYTES + (C::STAGES + s) * C::KV_BYTES;
+#pragma unroll
+          for (int c = 0; c < C::BOXES; ++c)
+            for (int i = left * 8 + lane; i < AT_KEYS * 8; i += 32) *reinterpret_cast<uint4*>(v + c * AT_BOX + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(b_clean);
+        } else if (lane == 0) {
+          arcb_set_error(a.status, ARCB_DEV_WAIT_TIMEOUT_TMA);
+        }
+      }
       if (!ok)        // gave up at tile j: the copies under way end before the CTA does
         for (int i = j > C::STAGES ? j - C::STAGES : 0; i <= j; ++i) {
           mbar_wait_bounded(b_kfull + 8 * (i % C::STAGES), (i / C::STAGES) & 1);
@@ -212,19 +227,6 @@ attn_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
         umma_commit_if(el, b_kempty + 8 * s);
       }
       if (ok && n_x > 0) umma_commit_if(el, b_o + 8 * x);
-    } else if (n_tiles > 0 && left < AT_KEYS) {
-      const int s = (n_tiles - 1) % C::STAGES;
-      if (__all_sync(0xffffffffu, mbar_wait_bounded(b_vfull + 8 * s, ((n_tiles - 1) / C::STAGES) & 1))) {
-        uint8_t* v = base_ptr + 2 * C::Q_BYTES + (C::STAGES + s) * C::KV_BYTES;
-#pragma unroll
-        for (int c = 0; c < C::BOXES; ++c)
-          for (int i = left * 8 + lane; i < AT_KEYS * 8; i += 32) *reinterpret_cast<uint4*>(v + c * AT_BOX + i * 16) = make_uint4(0u, 0u, 0u, 0u);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(b_clean);
-      } else if (lane == 0) {
-        arcb_set_error(a.status, ARCB_DEV_WAIT_TIMEOUT_TMA);
-      }
     }
   } else {
     reg_alloc_112();

@@ -3,7 +3,7 @@
 Tolerance of a value o = sum_t p_t v_t, from the arithmetic alone: the output's rounding, u |o| with u half a step of its type, and
 errors of the weights, each relative to p_t, so that their sum is bounded by a factor of A = sum_t p_t |v_t|.  The factor: a weight
 rounded to the products' operand type in two pieces is 2^-16 off, in one half a step of the type (half: 2^-11; bfloat16, where
-max_group, by default the number of items, allows more than 64 query rows a key head: 2^-8); a score is a sum of dim products in 32
+max_group, by default the number of items, allows more than 16 query rows a key head, 2^-8); a score is a sum of dim products in 32
 bits whose every addition is off by 2^-23 of the partial sums, at most (dim + 4) 2^-23 S with S = scale sum_d |q_d k_d|, and the
 exponential turns an absolute error of a score into a relative one of the weight, twice (numerator and denominator); sums over the
 rows and joins of parts in 32 bits: 2^-23 for each of the chain's additions, at most (rows + 128) of them.
@@ -78,7 +78,7 @@ class Case:
             spread = torch.matmul(weights, values.abs()).view(heads, dim)
             size = (torch.matmul(q.abs(), keys.abs().transpose(1, 2)) * abs(scale)).amax(-1).view(heads, 1)
             u = torch.finfo(out.dtype).eps / 2
-            many = n * rep > 64 and self.q.dtype == BF16
+            many = n * rep > 16 and self.q.dtype == BF16
             pieces = {F32: 0.0, BF16: 2.0 ** -8 if many else 2.0 ** -16, F16: 2.0 ** -11}[self.k.dtype]
             tol = u * want.abs() + (pieces + 2 * (dim + 4) * 2.0 ** -23 * size + (p + o + 128) * 2.0 ** -23) * spread + 2.0 ** -24
             err = (out[i].double() - want).abs()
