@@ -198,8 +198,18 @@ attn_prefix_join_kernel(AttnPrefixArgs a) {
 void fill_plan(AttnPrefixArgs& a) {
   a.rep = a.n_heads / a.n_kv;
   const bool tc = a.kv_fmt != 2 && (a.act_fmt == a.kv_fmt || a.dim == 64) && a.scale != 0.f;
-  a.plan = prefix_plan(a.n_groups, a.max_group, a.max_prefix, a.n_items, a.item_end ? a.max_own : 0, a.n_kv, a.rep,
-                       a.act_fmt != a.kv_fmt && a.dim == 128 ? 16 : 24, a.kv_fmt == 2, tc, arcb_num_sms());
+  a.plan = prefix_plan(a.n_groups, a.max_group, a.max_prefix, a.n_items, a.item_end ? a.max_own : 0, a.n_kv, a.rep, a.kv_fmt == 2, tc, arcb_num_sms());
+}
+
+int launch_part(const AttnPrefixArgs& a, int kernel, long long units, cudaStream_t stream) {
+  arcb_count_launch(1);
+  switch (kernel) {
+    case AP_ROWS: return arcb_attn_prefix_rows(a, units, stream);
+    case AP_TILES: return arcb_attn_prefix_mma(a, units, stream);
+    case AP_TC: return arcb_attn_prefix_tc(a, units, stream);
+  }
+  return (int)(a.dim == 64 ? arcb_launch(attn_prefix_simple_kernel<64>, dim3((unsigned)units), dim3(128), 0, stream, a)
+                           : arcb_launch(attn_prefix_simple_kernel<128>, dim3((unsigned)units), dim3(128), 0, stream, a));
 }
 
 }  // namespace
@@ -221,38 +231,21 @@ int arcb_launch_attn_prefix(AttnPrefixArgs a, cudaStream_t stream) {
   fill_plan(a);
   const PrefixPlan& p = a.plan;
   if (p.parts < 1 || (p.parts > 1 && !a.scratch)) return -1;
-  const long long shared = (long long)a.n_groups * a.n_kv * p.tiles1 * p.splits1, own = (long long)a.n_items * a.n_kv * p.tiles2 * p.splits2;
   const long long joins = ((long long)a.n_items * a.n_heads + 3) / 4;
-  if (shared + own > 0x7fffffffLL || joins > 0x7fffffffLL) return -1;
+  if (p.shared.units + p.own.units > 0x7fffffffLL || joins > 0x1fffffffLL) return -1;
   a.first_block = 0;
-  cudaError_t e = cudaSuccess;
-  if (p.shared == AP_SHARED_PLAIN) {
-    e = a.dim == 64 ? arcb_launch(attn_prefix_simple_kernel<64>, dim3((unsigned)(shared + own)), dim3(128), 0, stream, a)
-                    : arcb_launch(attn_prefix_simple_kernel<128>, dim3((unsigned)(shared + own)), dim3(128), 0, stream, a);
-    arcb_count_launch(1);
-  } else {
-    long long units = shared + own;
-    if (p.shared == AP_SHARED_TC && shared > 0) {
-      const int r = arcb_attn_prefix_tc(a, (unsigned)shared, stream);
-      arcb_count_launch(1);
-      if (r) return r;
-      a.first_block = shared;
-      units = own;
-    }
-    if (units > 0) {
-      const int r = arcb_attn_prefix_rows(a, units, stream);
-      arcb_count_launch(1);
-      if (r) return r;
-    }
+  int r = 0;
+  if (p.shared.units > 0) r = launch_part(a, p.shared.kernel, p.shared.units + (p.together ? p.own.units : 0), stream);
+  if (r == 0 && p.own.units > 0 && !p.together) {
+    a.first_block = p.shared.units;
+    r = launch_part(a, p.own.kernel, p.own.units, stream);
   }
-  if (e == cudaSuccess && p.parts > 1) {
-    // four warps a result where a warp each would leave SMs without work
-    const bool few = p.parts >= 8 && joins < 4LL * arcb_num_sms();
-    e = few ? arcb_launch(attn_prefix_join_kernel<4>, dim3((unsigned)((long long)a.n_items * a.n_heads)), dim3(128), 0, stream, a)
-            : arcb_launch(attn_prefix_join_kernel<1>, dim3((unsigned)joins), dim3(128), 0, stream, a);
-    arcb_count_launch(1);
-  }
-  return (int)e;
+  if (r || p.parts == 1) return r;
+  // four warps a result where a warp each would leave SMs without work
+  const bool few = p.parts >= 8 && joins < 4LL * arcb_num_sms();
+  arcb_count_launch(1);
+  return (int)(few ? arcb_launch(attn_prefix_join_kernel<4>, dim3((unsigned)((long long)a.n_items * a.n_heads)), dim3(128), 0, stream, a)
+                   : arcb_launch(attn_prefix_join_kernel<1>, dim3((unsigned)joins), dim3(128), 0, stream, a));
 }
 
 static int to_fmt(int act_format) { return act_format == ARCB_ACT_F16 ? 1 : act_format == ARCB_ACT_BF16 ? 0 : 2; }

@@ -34,10 +34,11 @@ struct AttnPrefixArgs {
 
 constexpr int AP_PAD = 4;     // of a partial result: the sums of a row's values, its maximum (log2 units), its sum, two spare
 
-// 16-bit formats; `a` as the launcher has filled it.  Units of warps (attn_prefix_rows.cu); the shared part for many query rows
-// (attn_prefix_tc.cu).
+// 16-bit formats; `a` as the launcher has filled it, units from a.first_block on.  Warps for up to 8 query rows
+// (attn_prefix_rows.cu), CTAs for up to 64 (attn_prefix_mma.cu), or 256 with tcgen05 (attn_prefix_tc.cu).
 int arcb_attn_prefix_rows(const AttnPrefixArgs& a, long long units, cudaStream_t stream);
-int arcb_attn_prefix_tc(const AttnPrefixArgs& a, unsigned blocks, cudaStream_t stream);
+int arcb_attn_prefix_mma(const AttnPrefixArgs& a, long long units, cudaStream_t stream);
+int arcb_attn_prefix_tc(const AttnPrefixArgs& a, long long units, cudaStream_t stream);
 
 bool arcb_attn_prefix_supported(int n_heads, int n_kv, int dim, int act_fmt, int kv_fmt);
 // bytes of a.scratch for these sizes

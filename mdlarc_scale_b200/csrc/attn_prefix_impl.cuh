@@ -17,11 +17,11 @@ struct ApWork {
 __device__ __forceinline__ ApWork ap_work(const AttnPrefixArgs& a, long long block, bool report) {
   ApWork k;
   unsigned w = (unsigned)block;       // fewer than 2^31 (the launcher's check)
-  const unsigned n1 = (unsigned)(a.n_groups * a.n_kv * a.plan.tiles1 * a.plan.splits1);
+  const unsigned n1 = (unsigned)a.plan.shared.units;
   int len, at0, split, splits, grain = 15;
   if (w < n1) {
-    const int t = (int)(w % a.plan.tiles1); w /= a.plan.tiles1;
-    splits = a.plan.splits1;
+    const int t = (int)(w % a.plan.shared.tiles); w /= a.plan.shared.tiles;
+    splits = a.plan.shared.splits;
     split = (int)(w % splits); w /= splits;
     k.kvh = (int)(w % a.n_kv);
     const int g = (int)(w / a.n_kv);
@@ -46,20 +46,20 @@ __device__ __forceinline__ ApWork ap_work(const AttnPrefixArgs& a, long long blo
       len = 0;
     }
     k.item0 = first;
-    k.r0 = t * a.plan.tile1;
-    k.rows = min(a.plan.tile1, (last - first) * a.rep - k.r0);
+    k.r0 = t * a.plan.shared.tile;
+    k.rows = min(a.plan.shared.tile, (last - first) * a.rep - k.r0);
     at0 = 0;
-    grain = a.plan.shared == AP_SHARED_TC ? 127 : 15;
+    grain = a.plan.shared.kernel == AP_TC ? 127 : a.plan.shared.kernel == AP_TILES ? 63 : 15;
     k.part = split;
   } else {
     w -= n1;
-    splits = a.plan.splits2;
+    splits = a.plan.own.splits;
     split = (int)(w % splits); w /= splits;
-    const int t = (int)(w % a.plan.tiles2); w /= a.plan.tiles2;
+    const int t = (int)(w % a.plan.own.tiles); w /= a.plan.own.tiles;
     k.kvh = (int)(w % a.n_kv);
     k.item0 = (int)(w / a.n_kv);
-    k.r0 = t * a.plan.tile2;
-    k.rows = min(a.plan.tile2, a.rep - k.r0);
+    k.r0 = t * a.plan.own.tile;
+    k.rows = min(a.plan.own.tile, a.rep - k.r0);
     k.seq = a.item_seq ? a.item_seq[k.item0] : k.item0;
     at0 = a.item_begin ? a.item_begin[k.item0] : 0;
     len = a.item_end[k.item0] - at0;
@@ -68,7 +68,8 @@ __device__ __forceinline__ ApWork ap_work(const AttnPrefixArgs& a, long long blo
       len = 0;
     }
     if (len < 0 || (a.item_skip && a.item_skip[k.item0])) len = 0;
-    k.part = a.plan.parts1 + split;
+    grain = a.plan.own.kernel == AP_TILES ? 63 : 15;
+    k.part = a.plan.shared_parts + split;
   }
   int chunk = (len + splits - 1) / splits;
   chunk = (chunk + grain) & ~grain;

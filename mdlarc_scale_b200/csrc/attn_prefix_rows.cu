@@ -17,7 +17,7 @@
 // weights' pieces are columns of their own and cost nothing; with more than 16 in equal formats weights are one piece (sqrt 2 of the
 // output's own rounding error in all), where a second one would bind the kernel to its products.  Maxima, sums and all partial
 // results are fp32; a range's reference maximum is raised only when it grows by 2^8.
-#include "attn_prefix_impl.cuh"
+#include "attn_prefix_frag.cuh"
 #include "flash_common.cuh"
 #include "gemm.cuh"
 #include "launch.cuh"
@@ -29,53 +29,15 @@ namespace {
 constexpr float AR_RESCALE = 8.f;      // log2 units
 constexpr int AR_WARPS = 4;
 
-template <bool HALF>
-__device__ __forceinline__ void ar_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (HALF)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void ar_ld4(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
-}
-__device__ __forceinline__ void ar_ld4t(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
-}
-__device__ __forceinline__ uint32_t ar_transpose(uint32_t v) {
-  uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
-  return r;
-}
-// two values as pairs of 16-bit pieces
-template <bool HALF>
-__device__ __forceinline__ void ar_split(float x, float y, uint32_t& hi, uint32_t& lo) {
-  if constexpr (HALF) {
-    const __half2 h = __floats2half2_rn(x, y);
-    const float2 f = __half22float2(h);
-    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
-    hi = *reinterpret_cast<const uint32_t*>(&h);
-    lo = *reinterpret_cast<const uint32_t*>(&l);
-  } else {
-    hi = pack2_bf16(x, y);
-    const float2 f = unpack2_bf16(hi);
-    lo = pack2_bf16(x - f.x, y - f.y);
-  }
-}
-
-// MOST: the most query rows of a unit of the launch, in eights.
-template <int D, int MOST>
+template <int D>
 struct ArCfg {
-  static constexpr int CTAS = MOST == 1 ? 3 : 2;           // of an SM
+  static constexpr int CTAS = 3;           // of an SM
   static constexpr int KEYS = D == 64 ? 32 : 16;           // of a tile
-  static constexpr int STAGES = MOST == 1 ? 2 : 3;
+  static constexpr int STAGES = 2;
   static constexpr int BOX = KEYS * 128;
   static constexpr int PLANE = KEYS * D * 2;
   static constexpr int STAGE = 2 * PLANE;
-  static constexpr int Q_ROWS = MOST == 1 ? 8 : 16;        // that travel with a unit's first tile; more are read when it starts
-  static constexpr int Q_BYTES = Q_ROWS * D * 2;
+  static constexpr int Q_BYTES = 8 * D * 2;
   static constexpr int WARP = STAGES * STAGE + Q_BYTES;    // a multiple of 1 KB: the swizzle goes by the address
   static_assert(WARP % 1024 == 0 && STAGE % 1024 == 0, "swizzled boxes");
   static constexpr int SMEM = AR_WARPS * (WARP + 8 * STAGES);      // no room to align: without static shared memory it starts aligned
@@ -83,9 +45,9 @@ struct ArCfg {
 };
 
 // What a warp keeps from unit to unit.
-template <int D, int MOST>
+template <int D>
 struct ArWarp {
-  using C = ArCfg<D, MOST>;
+  using C = ArCfg<D>;
   const AttnPrefixArgs& a;
   const CUtensorMap* maps[2];
   long long first, stride, n_units;        // this warp's units
@@ -134,7 +96,7 @@ struct ArWarp {
     const uint32_t bar = bars + 8 * put, st = ring + put * C::STAGE;
     const bool first_tile = ahead_left == tiles_of(ahead);
     uint32_t bytes = C::STAGE;
-    if (first_tile && ahead.rows <= C::Q_ROWS) {
+    if (first_tile) {
       bytes += ahead.rows * D * 2;
       if (lane < ahead.rows)
         asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(q_slot + lane * D * 2),
@@ -166,34 +128,30 @@ struct ArWarp {
   }
 };
 
-// One unit for 8 QT query rows.  PAIR: up to four rows; columns 4 to 7 of the products are second pieces of weights.
-template <int D, int MOST, bool HALF, bool QS, int QT, bool PAIR>
-__device__ __forceinline__ void ar_unit(ArWarp<D, MOST>& s, const ApWork& w, int i) {
-  using C = ArCfg<D, MOST>;
+// One unit.  PAIR: up to four query rows; columns 4 to 7 of the products are second pieces of weights.
+template <int D, bool HALF, bool QS, bool PAIR>
+__device__ __forceinline__ void ar_unit(ArWarp<D>& s, const ApWork& w, int i) {
+  using C = ArCfg<D>;
   constexpr int DK = D / 16, MT = C::KEYS / 16;
-  constexpr bool P2 = !PAIR && (QS || QT <= 2);          // second pieces of weights as products of their own
   const AttnPrefixArgs& a = s.a;
   const int lane = s.lane;
-  const float sc = fabsf(a.scale) * AP_LOG2E;
-  const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;        // a negative scale turns the queries, so that maxima are maxima
+  // A negative scale turns the queries, so that maxima are maxima; one of 0 makes them 0, since 0 times -inf is no score.
+  const float sc = a.scale == 0.f ? 1.f : fabsf(a.scale) * AP_LOG2E;
+  const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u, kept = a.scale == 0.f ? 0u : 0xffffffffu;
   const int tiles = s.tiles_of(w);
-  // A lane has queries (lane % 4) * 2 and the next one of every eight (PAIR: of the first four), and keys or value columns lane / 4
-  // and that plus 8 of every 16.
-  uint32_t q[QT][DK][2], q2[QS ? QT : 1][QS ? DK : 1][2];
-  float acc[QT][DK][4], m[QT][2], off[QT][2], l[QT][2];          // off: what is taken off a score, -m or 0
+  // A lane has queries (lane % 4) * 2 and the next one (PAIR: of the first four), and keys or value columns lane / 4 and that plus 8 of
+  // every 16.
+  uint32_t q[DK][2], q2[QS ? DK : 1][2];
+  float acc[DK][4], m[2] = {-INFINITY, -INFINITY}, off[2] = {0.f, 0.f}, l[2] = {0.f, 0.f};     // off: what is taken off a score, -m or 0
 #pragma unroll
-  for (int b = 0; b < QT; ++b) {
-    m[b][0] = m[b][1] = -INFINITY;
-    off[b][0] = off[b][1] = l[b][0] = l[b][1] = 0.f;
-#pragma unroll
-    for (int e = 0; e < DK; ++e) acc[b][e][0] = acc[b][e][1] = acc[b][e][2] = acc[b][e][3] = 0.f;
-  }
-  auto keep_query = [&](int b, int ks, int y, uint32_t raw) {
+  for (int e = 0; e < DK; ++e) acc[e][0] = acc[e][1] = acc[e][2] = acc[e][3] = 0.f;
+  auto keep_query = [&](int ks, int y, uint32_t raw) {
+    raw = (raw ^ flip) & kept;
     if constexpr (QS) {
-      const float2 f = unpack2_act(raw ^ flip, 1);
-      ar_split<false>(f.x, f.y, q[b][ks][y], q2[b][ks][y]);
+      const float2 f = unpack2_act(raw, 1);
+      am_split<false>(f.x, f.y, q[ks][y], q2[ks][y]);
     } else {
-      q[b][ks][y] = raw ^ flip;
+      q[ks][y] = raw;
     }
   };
   // Pieces of matrix loads: row (lane % 16) and row (lane % 8) + 8 (lane / 16) of 16; 16-byte piece 2 ks + h lies at (2 ks + h) ^ row % 8,
@@ -209,218 +167,140 @@ __device__ __forceinline__ void ar_unit(ArWarp<D, MOST>& s, const ApWork& w, int
       return;
     }
     if (t == 0) {
+      const int r = min(lane & (PAIR ? 3 : 7), w.rows - 1);      // rows that do not exist are as the last one
 #pragma unroll
-      for (int b = 0; b < QT; ++b) {
-        if constexpr (8 * QT <= C::Q_ROWS) {
-          const int r = min(b * 8 + (lane & (PAIR ? 3 : 7)), w.rows - 1);      // rows that do not exist are as the last one
-#pragma unroll
-          for (int ks = 0; ks < DK; ks += 2) {
-            uint32_t in[4];
-            ar_ld4(s.q_slot + r * (D * 2) + ((2 * ks + (lane >> 3)) << 4), in);
-            keep_query(b, ks, 0, in[0]);
-            keep_query(b, ks, 1, in[1]);
-            keep_query(b, ks + 1, 0, in[2]);
-            keep_query(b, ks + 1, 1, in[3]);
-          }
-        } else {
-          const char* src = s.query(w, min(b * 8 + (lane >> 2), w.rows - 1)) + (lane & 3) * 4;
-#pragma unroll
-          for (int ks = 0; ks < DK; ++ks)
-#pragma unroll
-            for (int y = 0; y < 2; ++y) keep_query(b, ks, y, *reinterpret_cast<const uint32_t*>(src + ks * 32 + y * 16));
-        }
+      for (int ks = 0; ks < DK; ks += 2) {
+        uint32_t in[4];
+        am_ld4(s.q_slot + r * (D * 2) + ((2 * ks + (lane >> 3)) << 4), in);
+        keep_query(ks, 0, in[0]);
+        keep_query(ks, 1, in[1]);
+        keep_query(ks + 1, 0, in[2]);
+        keep_query(ks + 1, 1, in[3]);
       }
       __syncwarp();
       s.ask(i, true);
     }
-    const uint32_t kst = s.ring + s.get * C::STAGE + k_at, vst = s.ring + s.get * C::STAGE + C::PLANE + v_at;
+    const uint32_t slot = s.ring + s.get * C::STAGE, kst = slot + k_at, vst = slot + C::PLANE + v_at;
     s.get = s.get + 1 == C::STAGES ? 0 : s.get + 1;
     s.phase ^= s.get == 0;
     --s.flight;
     const int left = w.end - w.begin - t * C::KEYS;        // keys of the tile
     const bool some = left < C::KEYS;
-    float p[QT][MT][4];
+    float p[MT][4];
 #pragma unroll
-    for (int b = 0; b < QT; ++b)
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) p[b][mt][0] = p[b][mt][1] = p[b][mt][2] = p[b][mt][3] = 0.f;
+    for (int mt = 0; mt < MT; ++mt) p[mt][0] = p[mt][1] = p[mt][2] = p[mt][3] = 0.f;
 #pragma unroll
     for (int ks = 0; ks < DK; ++ks) {
       const uint32_t at = (kst ^ ((ks & 3) << 5)) + (ks >> 2) * C::BOX;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         uint32_t k[4];
-        ar_ld4(at + mt * (16 * 128), k);
-#pragma unroll
-        for (int b = 0; b < QT; ++b) {
-          ar_mma<HALF>(p[b][mt], k, q[b][ks][0], q[b][ks][1]);
-          if constexpr (QS) ar_mma<HALF>(p[b][mt], k, q2[b][ks][0], q2[b][ks][1]);
-        }
+        am_ld4(at + mt * (16 * 128), k);
+        am_mma<HALF>(p[mt], k, q[ks][0], q[ks][1]);
+        if constexpr (QS) am_mma<HALF>(p[mt], k, q2[ks][0], q2[ks][1]);
       }
     }
-    if (some)
+    if (some) {
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (mt * 16 + (lane >> 2) + (j >> 1) * 8 >= left)
+          if (mt * 16 + (lane >> 2) + (j >> 1) * 8 >= left) p[mt][j] = -INFINITY;
+      // values behind the end: a weight of 0 does not hide a NaN
+      for (int e = left * 8 + lane; e < C::KEYS * 8; e += 32)
 #pragma unroll
-            for (int b = 0; b < QT; ++b) p[b][mt][j] = -INFINITY;
+        for (int c = 0; c < D / 64; ++c)
+          asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(slot + C::PLANE + c * C::BOX + e * 16), "r"(0u) : "memory");
+      fence_proxy_async_smem();            // the slot's next tile comes by the other proxy
+      __syncwarp();
+    }
     // the lanes' own maxima tell whether any reference has to be raised; only then are they exchanged
-    float top[QT][2];
+    float top[2];
     bool raise = t == 0;
 #pragma unroll
-    for (int b = 0; b < QT; ++b)
+    for (int x = 0; x < 2; ++x) {
+      float mx = fmaxf(p[0][x], p[0][2 + x]);
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        float mx = fmaxf(p[b][0][x], p[b][0][2 + x]);
-#pragma unroll
-        for (int mt = 1; mt < MT; ++mt) mx = max3_f32(mx, p[b][mt][x], p[b][mt][2 + x]);
-        top[b][x] = mx;
-        raise |= mx * sc > m[b][x] + AR_RESCALE;
-      }
+      for (int mt = 1; mt < MT; ++mt) mx = max3_f32(mx, p[mt][x], p[mt][2 + x]);
+      top[x] = mx;
+      raise |= mx * sc > m[x] + AR_RESCALE;
+    }
     if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
-      for (int b = 0; b < QT; ++b)
+      for (int x = 0; x < 2; ++x) {
+        float mx = top[x];
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        mx = fmaxf(mx * sc, m[x]);
+        if (mx == -INFINITY) continue;
+        const float alpha = m[x] == -INFINITY ? 0.f : ex2_fast(m[x] - mx);
+        m[x] = mx;
+        off[x] = -mx;
+        l[x] *= alpha;
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          float mx = top[b][x];
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-          mx = fmaxf(mx == -INFINITY ? -INFINITY : mx * sc, m[b][x]);
-          if (mx == -INFINITY) continue;
-          const float alpha = m[b][x] == -INFINITY ? 0.f : ex2_fast(m[b][x] - mx);
-          m[b][x] = mx;
-          off[b][x] = -mx;
-          l[b][x] *= alpha;
-#pragma unroll
-          for (int e = 0; e < DK; ++e) {
-            acc[b][e][x] *= alpha;
-            acc[b][e][2 + x] *= alpha;
-          }
-        }
-    }
-#pragma unroll
-    for (int b = 0; b < QT; ++b)
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) p[b][mt][j] = ex2_fast(fmaf(p[b][mt][j], sc, off[b][j & 1]));
-    if (some)                              // for a scale of 0, whose product with -inf is NaN
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (mt * 16 + (lane >> 2) + (j >> 1) * 8 >= left)
-#pragma unroll
-            for (int b = 0; b < QT; ++b) p[b][mt][j] = 0.f;
-#pragma unroll
-    for (int b = 0; b < QT; ++b)
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) l[b][j & 1] += p[b][mt][j];
-    uint32_t hi[QT][MT][2], lo[QT][P2 ? MT : 1][2];
-#pragma unroll
-    for (int b = 0; b < QT; ++b)
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          uint32_t h, o = 0u;
-          if constexpr (PAIR || P2) ar_split<HALF>(p[b][mt][2 * y], p[b][mt][2 * y + 1], h, o);
-          else h = pack2_prob(p[b][mt][2 * y], p[b][mt][2 * y + 1], HALF ? 1 : 0);
-          hi[b][mt][y] = ar_transpose(PAIR && (lane & 2) ? o : h);
-          if constexpr (P2) lo[b][mt][y] = ar_transpose(o);
-        }
-    if (!some) {
-#pragma unroll
-      for (int dt = 0; dt < DK; ++dt) {
-        const uint32_t at = (vst ^ ((dt & 3) << 5)) + (dt >> 2) * C::BOX;
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          uint32_t v[4];
-          ar_ld4t(at + mt * (16 * 128), v);
-#pragma unroll
-          for (int b = 0; b < QT; ++b) {
-            ar_mma<HALF>(acc[b][dt], v, hi[b][mt][0], hi[b][mt][1]);
-            if constexpr (P2) ar_mma<HALF>(acc[b][dt], v, lo[b][mt][0], lo[b][mt][1]);
-          }
+        for (int e = 0; e < DK; ++e) {
+          acc[e][x] *= alpha;
+          acc[e][2 + x] *= alpha;
         }
       }
-    } else {
-      // values behind the end: a weight of 0 does not hide a NaN
-      uint32_t keep[MT][2];
+    }
+    uint32_t hi[MT][2], lo[PAIR ? 1 : MT][2];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          const int k0 = mt * 16 + y * 8 + (lane & 3) * 2;
-          keep[mt][y] = (k0 < left ? 0xffffu : 0u) | (k0 + 1 < left ? 0xffff0000u : 0u);
-        }
-#pragma unroll 1
-      for (int dt = 0; dt < DK; ++dt) {
-        const uint32_t at = (vst ^ ((dt & 3) << 5)) + (dt >> 2) * C::BOX;
-        float sum[QT][4];
+      for (int y = 0; y < 2; ++y) {
+        const float e0 = ex2_fast(fmaf(p[mt][2 * y], sc, off[0])), e1 = ex2_fast(fmaf(p[mt][2 * y + 1], sc, off[1]));
+        l[0] += e0;
+        l[1] += e1;
+        uint32_t h, o;
+        am_split<HALF>(e0, e1, h, o);
+        hi[mt][y] = am_transpose(PAIR && (lane & 2) ? o : h);
+        if constexpr (!PAIR) lo[mt][y] = am_transpose(o);
+      }
 #pragma unroll
-        for (int b = 0; b < QT; ++b) sum[b][0] = sum[b][1] = sum[b][2] = sum[b][3] = 0.f;
+    for (int dt = 0; dt < DK; ++dt) {
+      const uint32_t at = (vst ^ ((dt & 3) << 5)) + (dt >> 2) * C::BOX;
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          uint32_t v[4];
-          ar_ld4t(at + mt * (16 * 128), v);
-          v[0] &= keep[mt][0]; v[1] &= keep[mt][0];
-          v[2] &= keep[mt][1]; v[3] &= keep[mt][1];
-#pragma unroll
-          for (int b = 0; b < QT; ++b) {
-            ar_mma<HALF>(sum[b], v, hi[b][mt][0], hi[b][mt][1]);
-            if constexpr (P2) ar_mma<HALF>(sum[b], v, lo[b][mt][0], lo[b][mt][1]);
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < DK; ++e)
-          if (e == dt)
-#pragma unroll
-            for (int b = 0; b < QT; ++b)
-#pragma unroll
-              for (int j = 0; j < 4; ++j) acc[b][e][j] += sum[b][j];
+      for (int mt = 0; mt < MT; ++mt) {
+        uint32_t v[4];
+        am_ld4t(at + mt * (16 * 128), v);
+        am_mma<HALF>(acc[dt], v, hi[mt][0], hi[mt][1]);
+        if constexpr (!PAIR) am_mma<HALF>(acc[dt], v, lo[mt][0], lo[mt][1]);
       }
     }
   }
   // The unit's part of the result: eight lanes have eight neighbouring value columns of a query.
   const bool whole = a.plan.parts == 1;
 #pragma unroll
-  for (int b = 0; b < QT; ++b) {
+  for (int x = 0; x < 2; ++x) {
+    if (x >= w.rows) break;
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      if (b * 8 + x >= w.rows) continue;
+    for (int o = 4; o <= 16; o <<= 1) l[x] += __shfl_xor_sync(0xffffffffu, l[x], o);
+    const int r = (lane & (PAIR ? 1 : 3)) * 2 + x;
+    const bool in = r < w.rows && !(PAIR && (lane & 2));
+    const int R = w.r0 + (in ? r : 0), item = w.item0 + R / a.rep;
+    const long long ih = (long long)item * a.n_heads + w.kvh * a.rep + R % a.rep;
+    const float inv = l[x] == 0.f || (whole && in && a.item_skip && a.item_skip[item]) ? 0.f : 1.f / l[x];
+    float* to = whole ? nullptr : ap_record(a, ih, w.part) + (lane >> 2);
 #pragma unroll
-      for (int o = 4; o <= 16; o <<= 1) l[b][x] += __shfl_xor_sync(0xffffffffu, l[b][x], o);
-      const int r = b * 8 + (lane & (PAIR ? 1 : 3)) * 2 + x;
-      const bool in = r < w.rows && !(PAIR && (lane & 2));
-      const int R = w.r0 + (in ? r : 0), item = w.item0 + R / a.rep;
-      const long long ih = (long long)item * a.n_heads + w.kvh * a.rep + R % a.rep;
-      const float inv = l[b][x] == 0.f || (whole && in && a.item_skip && a.item_skip[item]) ? 0.f : 1.f / l[b][x];
-      float* to = whole ? nullptr : ap_record(a, ih, w.part) + (lane >> 2);
+    for (int e = 0; e < DK; ++e)
 #pragma unroll
-      for (int e = 0; e < DK; ++e)
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          float v = acc[b][e][2 * y + x];
-          if constexpr (PAIR) v += __shfl_xor_sync(0xffffffffu, v, 2);
-          if (!in) continue;
-          if (whole) ap_store1(a.out, (size_t)ih * D + e * 16 + y * 8 + (lane >> 2), inv == 0.f ? 0.f : v * inv, a.act_fmt);
-          else if (tiles > 0) to[e * 16 + y * 8] = v;
-        }
-      if (in && !whole && lane < 4) *reinterpret_cast<float2*>(to + D) = make_float2(m[b][x], l[b][x]);
-    }
+      for (int y = 0; y < 2; ++y) {
+        float v = acc[e][2 * y + x];
+        if constexpr (PAIR) v += __shfl_xor_sync(0xffffffffu, v, 2);
+        if (!in) continue;
+        if (whole) ap_store1(a.out, (size_t)ih * D + e * 16 + y * 8 + (lane >> 2), inv == 0.f ? 0.f : v * inv, a.act_fmt);
+        else if (tiles > 0) to[e * 16 + y * 8] = v;
+      }
+    if (in && !whole && lane < 4) *reinterpret_cast<float2*>(to + D) = make_float2(m[x], l[x]);
   }
 }
 
-template <int D, int MOST, bool HALF, bool QS>
-__global__ void __launch_bounds__(AR_WARPS * 32, (ArCfg<D, MOST>::CTAS))
+template <int D, bool HALF, bool QS>
+__global__ void __launch_bounds__(AR_WARPS * 32, ArCfg<D>::CTAS)
 attn_prefix_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, AttnPrefixArgs a, long long n_units) {
-  using C = ArCfg<D, MOST>;
+  using C = ArCfg<D>;
   pdl_launch_dependents();
   pdl_wait();
   extern __shared__ __align__(1024) uint8_t ar_smem[];
@@ -437,7 +317,7 @@ attn_prefix_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
     mbar_fence_init();
   }
   __syncwarp();
-  ArWarp<D, MOST> s{a, {&tmap_k, &tmap_v}, first, stride, n_units, (int)((n_units - first + stride - 1) / stride), lane, ring, ring + C::STAGES * C::STAGE, bars};
+  ArWarp<D> s{a, {&tmap_k, &tmap_v}, first, stride, n_units, (int)((n_units - first + stride - 1) / stride), lane, ring, ring + C::STAGES * C::STAGE, bars};
   s.batch_of = -1;
   s.flight = s.put = s.get = s.ahead_i = 0;
   s.phase = 0;
@@ -445,12 +325,8 @@ attn_prefix_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
   ApWork w = s.unit(0);
   s.look_at(w);
   for (int i = 0; i < s.n && s.ok; ++i) {
-    if (w.rows <= 4) ar_unit<D, MOST, HALF, QS, 1, true>(s, w, i);
-    else if (MOST == 1 || w.rows <= 8) ar_unit<D, MOST, HALF, QS, 1, false>(s, w, i);
-    else if constexpr (MOST > 1) {
-      if (w.rows <= 16) ar_unit<D, MOST, HALF, QS, 2, false>(s, w, i);
-      else if constexpr (!(QS && D == 128)) ar_unit<D, MOST, HALF, QS, 3, false>(s, w, i);
-    }
+    if (w.rows <= 4) ar_unit<D, HALF, QS, true>(s, w, i);
+    else ar_unit<D, HALF, QS, false>(s, w, i);
     if (i + 1 < s.n) {
       if (s.ahead_i == i) s.look_at(s.unit(++s.ahead_i));
       w = s.ahead;
@@ -458,11 +334,11 @@ attn_prefix_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
   }
 }
 
-template <int D, int MOST, bool HALF, bool QS>
+template <int D, bool HALF, bool QS>
 int ar_launch(const AttnPrefixArgs& a, long long units, cudaStream_t stream) {
-  using C = ArCfg<D, MOST>;
+  using C = ArCfg<D>;
   static std::atomic<unsigned long long> done{0};
-  const cudaError_t e = arcb_opt_in_smem(attn_prefix_rows_kernel<D, MOST, HALF, QS>, C::SMEM, done);
+  const cudaError_t e = arcb_opt_in_smem(attn_prefix_rows_kernel<D, HALF, QS>, C::SMEM, done);
   if (e != cudaSuccess) return (int)e;
   CUtensorMap tk, tv;
   const uint64_t rows = (uint64_t)a.n_seqs * a.n_kv * a.t_max;
@@ -470,19 +346,13 @@ int ar_launch(const AttnPrefixArgs& a, long long units, cudaStream_t stream) {
   if (!r) r = arcb_make_tmap_2d_16b(&tv, a.v, rows, D, C::KEYS, 64, HALF);
   if (r) return 1000 + r;
   const long long most = (long long)C::CTAS * arcb_num_sms();
-  return (int)arcb_launch(attn_prefix_rows_kernel<D, MOST, HALF, QS>, dim3((unsigned)(units < most ? units : most)), dim3(AR_WARPS * 32), C::SMEM, stream, tk, tv,
+  return (int)arcb_launch(attn_prefix_rows_kernel<D, HALF, QS>, dim3((unsigned)(units < most ? units : most)), dim3(AR_WARPS * 32), C::SMEM, stream, tk, tv,
                           a, units);
 }
-template <int D, bool HALF, bool QS>
-int ar_launch(const AttnPrefixArgs& a, long long units, bool eight, cudaStream_t stream) {
-  return eight ? ar_launch<D, 1, HALF, QS>(a, units, stream) : ar_launch<D, 3, HALF, QS>(a, units, stream);
-}
-
 }  // namespace
 
 int arcb_attn_prefix_rows(const AttnPrefixArgs& a, long long units, cudaStream_t stream) {
-  const bool eight = a.plan.rows <= 8;
-  if (a.kv_fmt == 1) return a.dim == 64 ? ar_launch<64, true, false>(a, units, eight, stream) : ar_launch<128, true, false>(a, units, eight, stream);
-  if (a.act_fmt == 1) return a.dim == 64 ? ar_launch<64, false, true>(a, units, eight, stream) : ar_launch<128, false, true>(a, units, eight, stream);
-  return a.dim == 64 ? ar_launch<64, false, false>(a, units, eight, stream) : ar_launch<128, false, false>(a, units, eight, stream);
+  if (a.kv_fmt == 1) return a.dim == 64 ? ar_launch<64, true, false>(a, units, stream) : ar_launch<128, true, false>(a, units, stream);
+  if (a.act_fmt == 1) return a.dim == 64 ? ar_launch<64, false, true>(a, units, stream) : ar_launch<128, false, true>(a, units, stream);
+  return a.dim == 64 ? ar_launch<64, false, false>(a, units, stream) : ar_launch<128, false, false>(a, units, stream);
 }

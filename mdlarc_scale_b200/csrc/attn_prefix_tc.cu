@@ -421,8 +421,8 @@ int at_launch(const AttnPrefixArgs& a, unsigned blocks, cudaStream_t stream) {
 
 }  // namespace
 
-int arcb_attn_prefix_tc(const AttnPrefixArgs& a, unsigned blocks, cudaStream_t stream) {
-  if (a.kv_fmt == 1) return a.dim == 64 ? at_launch<64, true, false, 1>(a, blocks, stream) : at_launch<128, true, false, 1>(a, blocks, stream);
-  if (a.act_fmt == 1) return a.dim == 64 ? at_launch<64, false, true, 2>(a, blocks, stream) : -1;
-  return a.dim == 64 ? at_launch<64, false, false, 1>(a, blocks, stream) : at_launch<128, false, false, 1>(a, blocks, stream);
+int arcb_attn_prefix_tc(const AttnPrefixArgs& a, long long units, cudaStream_t stream) {
+  if (a.kv_fmt == 1) return a.dim == 64 ? at_launch<64, true, false, 1>(a, (unsigned)units, stream) : at_launch<128, true, false, 1>(a, (unsigned)units, stream);
+  if (a.act_fmt == 1) return a.dim == 64 ? at_launch<64, false, true, 2>(a, (unsigned)units, stream) : -1;
+  return a.dim == 64 ? at_launch<64, false, false, 1>(a, (unsigned)units, stream) : at_launch<128, false, false, 1>(a, (unsigned)units, stream);
 }

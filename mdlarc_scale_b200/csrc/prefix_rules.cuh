@@ -2,57 +2,72 @@
 #pragma once
 #include <algorithm>
 
-// What goes through the shared rows, by the query rows that a group's items have at a key head: a warp for up to 24, a CTA with
-// tcgen05 products for more.  Own rows are a warp's.  32-bit formats: a CTA for 16 query rows of either part.
-enum : int { AP_SHARED_ROWS = 0, AP_SHARED_TC = 1, AP_SHARED_PLAIN = 2 };
-constexpr int AP_WARPS_PER_SM = 8;      // that go through cached rows
+// Kernels, by the query rows of a unit: a warp for up to 8, a CTA for up to 64, a CTA with tcgen05 products for up to 256; a CTA of
+// multiply-adds for 16 in 32-bit formats.
+enum : int { AP_ROWS = 0, AP_TILES = 1, AP_TC = 2, AP_PLAIN = 3 };
 
-struct PrefixPlan {
-  int shared;               // AP_SHARED_*
-  int tile1, tile2;         // query rows of a unit: shared part, own part
-  int rows;                 // the most that a warp's unit has
-  int tiles1, splits1;      // shared rows: query tiles of a group and head, ranges that its rows are cut into
-  int tiles2, splits2;      // own rows: query tiles of an item and head, ranges
-  int parts1, parts;        // of a result: of the shared part, and all
+struct PrefixPart {
+  int kernel;               // AP_*
+  int tile;                 // query rows of a unit
+  int tiles;                // of a group (an item) and key head
+  int splits;               // ranges that the cached rows are cut into
+  long long units;
 };
 
-// max_group items of `rep` heads share a group's rows; `most`: query rows a warp may have; `wide`: 32-bit formats; `tc`: tcgen05 may be
-// used.
+struct PrefixPlan {
+  PrefixPart shared, own;
+  int together;             // both parts in one launch
+  int shared_parts, parts;  // of a result: of the shared rows, and all
+};
+
+// `rows` query rows at each of `heads` (groups or items) x n_kv; `tc`: tcgen05 may be used.
+inline PrefixPart prefix_part(long long heads, long long rows, int n_kv, bool wide, bool tc) {
+  PrefixPart p{};
+  p.kernel = wide ? AP_PLAIN : rows <= 8 ? AP_ROWS : rows <= 64 || !tc ? AP_TILES : AP_TC;
+  p.tile = p.kernel == AP_PLAIN ? 16 : p.kernel == AP_ROWS ? 8 : p.kernel == AP_TC ? 256 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+  p.tiles = (int)((rows + p.tile - 1) / p.tile);
+  p.units = heads * n_kv * p.tiles;
+  return p;
+}
+inline int prefix_cut(long long rows, long long chunk, long long most) {
+  return (int)std::min(most, std::max(1LL, (rows + chunk - 1) / chunk));
+}
+// What runs at once is given about equal shares of `total` cached rows; four units each where they are long, so that lengths that
+// differ even out.
+inline long long prefix_chunk(long long total, long long at_once, long long least) {
+  const long long each = total / at_once;
+  return each < 4 * least ? std::max(least, each) : std::max(4 * least, each / 4);
+}
+
+// max_group items of `rep` heads share a group's rows.
 inline PrefixPlan prefix_plan(long long n_groups, long long max_group, long long max_prefix, long long n_items, long long max_own, int n_kv,
-                              int rep, int most, bool wide, bool tc, int sms) {
+                              int rep, bool wide, bool tc, int sms) {
   PrefixPlan p{};
-  const long long rows = max_group * rep;
-  p.shared = wide ? AP_SHARED_PLAIN : rows <= 24 || !tc ? AP_SHARED_ROWS : AP_SHARED_TC;
-  p.tile1 = p.shared == AP_SHARED_TC ? 256 : wide ? 16 : most;
-  p.tile2 = wide ? 16 : most;
-  p.tiles1 = n_groups > 0 ? (int)((rows + p.tile1 - 1) / p.tile1) : 0;
-  p.tiles2 = max_own > 0 ? (rep + p.tile2 - 1) / p.tile2 : 0;
-  const long long units1 = n_groups * n_kv * p.tiles1, units2 = max_own > 0 ? n_items * n_kv * p.tiles2 : 0;
-  const auto cut = [](long long n, long long chunk, long long most) { return (int)std::min(most, std::max(1LL, (n + chunk - 1) / chunk)); };
-  const bool together = p.shared != AP_SHARED_TC;
-  // cached rows of a warp's unit: all of them divided by the warps; four units a warp where they are long
-  const long long each = ((together ? units1 * max_prefix : 0) + units2 * max_own) / ((long long)AP_WARPS_PER_SM * sms);
-  const long long chunk = each < 256 ? std::max(64LL, each) : std::max(256LL, each / 4);
-  p.splits2 = max_own > 0 ? cut(max_own, chunk, 32) : 0;
-  if (n_groups > 0) {
-    if (together) {
-      p.splits1 = cut(max_prefix, chunk, 128);
-    } else {
-      // one CTA an SM: the number of ranges whose waves take the fewest steps of 128 rows; a CTA's start and end count as three
-      long long best = 0;
-      for (int s = 1; s <= 32; ++s) {
-        const long long waves = (units1 * s + sms - 1) / sms, steps = ((max_prefix + s - 1) / s + 127) / 128;
-        const long long cost = waves * (steps + 3);
-        if (s == 1 || cost < best) {
-          best = cost;
-          p.splits1 = s;
-        }
+  p.shared = prefix_part(n_groups, n_groups > 0 ? max_group * rep : 0, n_kv, wide, tc);
+  p.own = prefix_part(n_items, max_own > 0 ? rep : 0, n_kv, wide, false);
+  const bool any1 = n_groups > 0, any2 = max_own > 0;
+  p.together = any1 && any2 && p.shared.kernel == p.own.kernel;
+  const long long total1 = p.shared.units * max_prefix, total2 = p.own.units * max_own;
+  const auto at_once = [&](int kernel) { return (long long)sms * (kernel == AP_ROWS ? 12 : 4); };
+  const auto least = [](int kernel) { return kernel == AP_ROWS ? 64LL : 128LL; };
+  if (any2) p.own.splits = prefix_cut(max_own, prefix_chunk(total2 + (p.together ? total1 : 0), at_once(p.own.kernel), least(p.own.kernel)), 32);
+  if (any1 && p.shared.kernel != AP_TC) {
+    p.shared.splits = prefix_cut(max_prefix, prefix_chunk(total1 + (p.together ? total2 : 0), at_once(p.shared.kernel), least(p.shared.kernel)), 128);
+  } else if (any1) {
+    // one CTA an SM: the number of ranges whose waves take the fewest steps of 128 rows; a CTA's start and end count as three
+    long long best = 0;
+    for (int s = 1; s <= 32; ++s) {
+      const long long waves = (p.shared.units * s + sms - 1) / sms, steps = ((max_prefix + s - 1) / s + 127) / 128;
+      const long long cost = waves * (steps + 3);
+      if (s == 1 || cost < best) {
+        best = cost;
+        p.shared.splits = s;
       }
     }
   }
-  const long long own = max_own > 0 ? std::min<long long>(rep, p.tile2) : 0;
-  p.rows = (int)std::max(own, p.shared == AP_SHARED_ROWS && n_groups > 0 ? std::min<long long>(rows, p.tile1) : 0LL);
-  p.parts1 = p.shared == AP_SHARED_TC ? 2 * p.splits1 : p.splits1;      // two chains a CTA
-  p.parts = p.parts1 + p.splits2;
+  p.shared.units *= p.shared.splits;
+  p.own.units *= p.own.splits;
+  p.shared_parts = p.shared.kernel == AP_TC ? 2 * p.shared.splits : p.shared.splits;      // two chains a CTA
+  p.parts = p.shared_parts + p.own.splits;
   return p;
 }
