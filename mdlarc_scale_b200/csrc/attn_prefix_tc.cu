@@ -7,8 +7,8 @@
 //   warp 0        TMA: key and value tiles as 128 x 64 boxes with the 128-byte swizzle, rings shared by A and B; value rows
 //                 behind the end of the last tile are set to zero: a weight of 0 does not hide a NaN
 //   warps 1, 2    products of A and of B: S = Q K^T (128 TMEM columns), O += P V with P read from TMEM
-//   warps 4-19    two threads a query row, 64 keys of every tile each: maxima (exchanged), exponentials, row sums, P over the
-//                 thread's own score columns
+//   warps 4-11    a thread a query row: maxima, exponentials, row sums, P over the row's own score columns.  (Two threads a row
+//                 had to exchange maxima in every tile and took twice the instructions.)
 // Maxima, sums and results are fp32.  The reference maximum of a row is raised only when it grows by 2^8.  Half queries over a
 // bfloat16 cache are two bfloat16 pieces (exact), and their weights too (2^-16 of a weight off).  In equal formats a weight is one
 // 16-bit value: its error, half a step, adds to an output that is rounded by as much itself (sqrt 2 of that error alone), and a
@@ -24,7 +24,7 @@ using namespace sm100;
 
 namespace {
 
-constexpr int AT_ROWS = 128, AT_KEYS = 128, AT_THREADS = 640;
+constexpr int AT_ROWS = 128, AT_KEYS = 128, AT_THREADS = 384;
 constexpr float AT_RESCALE = 8.f;          // log2 units
 constexpr int AT_BOX = 128 * 64 * 2;
 
@@ -39,8 +39,7 @@ struct AtCfg {
   static_assert(STAGES >= 2, "two tiles of keys and values");
   static constexpr int TILES = 2 * Q_BYTES + 2 * STAGES * KV_BYTES;
   static constexpr int BARS = 256;
-  static constexpr int XCHG = 2 * 2 * 2 * AT_ROWS * 4;
-  static constexpr int SMEM = TILES + BARS + XCHG + 1024;
+  static constexpr int SMEM = TILES + BARS + 1024;
   static_assert(SMEM <= 227 * 1024, "shared memory of one CTA");
 };
 
@@ -61,16 +60,25 @@ attn_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
   uint8_t* base_ptr = at_smem + (base - raw);
   const uint32_t q_smem = base, k_smem = base + 2 * C::Q_BYTES, v_smem = k_smem + C::STAGES * C::KV_BYTES, bar0 = base + C::TILES;
   const uint32_t b_kfull = bar0, b_kempty = b_kfull + 8 * C::STAGES, b_vfull = b_kempty + 8 * C::STAGES, b_vempty = b_vfull + 8 * C::STAGES,
-                 b_clean = b_vempty + 8 * C::STAGES, b_s = b_clean + 8, b_p = b_s + 16, b_o = b_p + 16, b_x = b_o + 16;
-  static_assert(32 * C::STAGES + 8 + 48 + 64 <= C::BARS - 8, "barriers");
+                 b_clean = b_vempty + 8 * C::STAGES, b_s = b_clean + 8, b_p = b_s + 16, b_o = b_p + 16;
+  static_assert(32 * C::STAGES + 8 + 48 <= C::BARS - 8, "barriers");
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(base_ptr + C::TILES + C::BARS - 8);
-  float (*s_xchg)[2][2][AT_ROWS] = reinterpret_cast<float (*)[2][2][AT_ROWS]>(base_ptr + C::TILES + C::BARS);   // [parity][tile][half][row]
 
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const bool wide = w.rows > AT_ROWS;
   const int n_tiles = (w.end - w.begin + AT_KEYS - 1) / AT_KEYS;
   const auto tiles_of = [&](int x) { return wide ? n_tiles : (n_tiles + 1 - x) / 2; };          // key tiles of A and B
   const int left = w.end - w.begin - (n_tiles - 1) * AT_KEYS;                                   // rows of the last one
+  // key and value tile j into its slots, by one thread
+  const int cache_row = (w.seq * a.n_kv + w.kvh) * a.t_max + w.begin;
+  auto load_tile = [&](int j, bool value) {
+    const int s = j % C::STAGES;
+    const uint32_t bar = (value ? b_vfull : b_kfull) + 8 * s;
+    mbar_expect_tx(bar, C::KV_BYTES);
+#pragma unroll
+    for (int c = 0; c < C::BOXES; ++c)
+      tma_load_2d((value ? v_smem : k_smem) + s * C::KV_BYTES + c * AT_BOX, value ? &tmap_v : &tmap_k, c * 64, cache_row + j * AT_KEYS, bar);
+  };
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
       mbar_init(b_kfull + 8 * s, 1);
@@ -81,13 +89,14 @@ attn_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
     mbar_init(b_clean, 1);
     for (int x = 0; x < 2; ++x) {
       mbar_init(b_s + 8 * x, 1);
-      mbar_init(b_p + 8 * x, 256);
+      mbar_init(b_p + 8 * x, 128);
       mbar_init(b_o + 8 * x, 1);
     }
-    for (int i = 0; i < 8; ++i) mbar_init(b_x + 8 * i, 64);
     mbar_fence_init();
-    tma_prefetch_desc(&tmap_k);
-    tma_prefetch_desc(&tmap_v);
+    for (int j = 0; j < C::STAGES && j < n_tiles; ++j) {      // on their way while the queries are fetched
+      load_tile(j, false);
+      load_tile(j, true);
+    }
   }
   if (warp == 1) {
     tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
@@ -132,9 +141,7 @@ attn_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
   // S_A [0, 128), S_B [128, 256), O_A [256, 256 + D), O_B
 
   if (warp < 4) {
-    reg_dealloc_32();
     if (warp == 0) {
-      const int row = (w.seq * a.n_kv + w.kvh) * a.t_max + w.begin;
       bool ok = true;
       auto wait = [&](uint32_t bar, uint32_t parity) {
         if (ok && !__all_sync(0xffffffffu, mbar_wait_bounded(bar, parity))) {
@@ -142,24 +149,16 @@ attn_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
           ok = false;
         }
       };
-      int j = 0;
+      int j = C::STAGES;
       for (; j < n_tiles; ++j) {
         const int s = j % C::STAGES;
         const uint32_t parity = ((j / C::STAGES) & 1) ^ 1;
         wait(b_kempty + 8 * s, parity);
         if (!ok) break;
-        if (lane == 0) {
-          mbar_expect_tx(b_kfull + 8 * s, C::KV_BYTES);
-#pragma unroll
-          for (int c = 0; c < C::BOXES; ++c) tma_load_2d(k_smem + s * C::KV_BYTES + c * AT_BOX, &tmap_k, c * 64, row + j * AT_KEYS, b_kfull + 8 * s);
-        }
+        if (lane == 0) load_tile(j, false);
         wait(b_vempty + 8 * s, parity);
         if (!ok) break;
-        if (lane == 0) {
-          mbar_expect_tx(b_vfull + 8 * s, C::KV_BYTES);
-#pragma unroll
-          for (int c = 0; c < C::BOXES; ++c) tma_load_2d(v_smem + s * C::KV_BYTES + c * AT_BOX, &tmap_v, c * 64, row + j * AT_KEYS, b_vfull + 8 * s);
-        }
+        if (lane == 0) load_tile(j, true);
       }
       if (ok && n_tiles > 0 && left < AT_KEYS) {
         // this warp has seen the slot's earlier tiles go, so that the barrier's parity can only mean this one
@@ -177,7 +176,7 @@ attn_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
         }
       }
       if (!ok)        // gave up at tile j: the copies under way end before the CTA does
-        for (int i = j > C::STAGES ? j - C::STAGES : 0; i <= j; ++i) {
+        for (int i = j - C::STAGES; i <= j && i < n_tiles; ++i) {
           mbar_wait_bounded(b_kfull + 8 * (i % C::STAGES), (i / C::STAGES) & 1);
           if (i < j) mbar_wait_bounded(b_vfull + 8 * (i % C::STAGES), (i / C::STAGES) & 1);
         }
@@ -206,7 +205,7 @@ attn_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
           for (int piece = 0; piece < WP; ++piece)
 #pragma unroll
             for (int ks = 0; ks < AT_KEYS / 16; ++ks)
-              umma_f16_ts_if(el, t_o, t_s + (ks >> 2) * 64 + piece * 32 + (ks & 3) * 8, dv + (uint64_t)(ks * (2048 >> 4)), idesc_pv, (i > 1 || piece || ks) ? 1u : 0u);
+              umma_f16_ts_if(el, t_o, t_s + piece * 64 + ks * 8, dv + (uint64_t)(ks * (2048 >> 4)), idesc_pv, (i > 1 || piece || ks) ? 1u : 0u);
           umma_commit_if(el, b_vempty + 8 * s);
         }
         if (i == n_x) break;
@@ -229,29 +228,36 @@ attn_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
       if (ok && n_x > 0) umma_commit_if(el, b_o + 8 * x);
     }
   } else {
-    reg_alloc_112();
-    const int x = (warp - 4) >> 3, half = ((warp >> 2) - 1) & 1, quarter = warp & 3;
-    const int r = quarter * 32 + lane, n_x = tiles_of(x);
+    const int x = (warp - 4) >> 2, quarter = warp & 3, n_x = tiles_of(x);
     const uint32_t t_lane = tmem_base + ((uint32_t)(quarter * 32) << 16);
-    const uint32_t t_s = t_lane + x * 128 + half * 64, t_o = t_lane + 256 + x * D + half * (D / 2);
-    const uint32_t xbar = b_x + 8 * (x * 4 + quarter);
+    const uint32_t t_s = t_lane + x * 128, t_o = t_lane + 256 + x * D;
     const float sc = fabsf(a.scale) * AP_LOG2E;
+    const uint64_t sc2 = pack_f32x2(sc, sc);
     const int first_row = (wide ? x * AT_ROWS : 0) + quarter * 32;         // of the warp, among the CTA's
     const bool idle = first_row >= w.rows;
     bool ok = true;
-    uint32_t xphase = 0;
-    // hands `mine` to the row's other thread; consecutive exchanges use the buffer's two parts in turn
-    auto swap = [&](float mine, float& theirs) -> bool {
-      s_xchg[xphase][x][half][r] = mine;
-      tc_fence_before();
-      mbar_arrive(xbar);
-      const bool good = mbar_wait_bounded(xbar, xphase);
-      tc_fence_after();
-      theirs = s_xchg[xphase][x][half ^ 1][r];
-      xphase ^= 1u;
-      return good;
-    };
     float m_ref = -INFINITY, l = 0.f;
+    // 64 of the row's scores; hidden keys become -inf, whose exp2 is exactly 0
+    auto load_scores = [&](int c, int seen, uint32_t (&sv)[2][32]) {
+      tmem_ld_32x32(t_s + c * 64, sv[0]);
+      tmem_ld_32x32(t_s + c * 64 + 32, sv[1]);
+      tmem_wait_ld_dep(sv[0]);
+      tmem_wait_ld_dep(sv[1]);
+      if (seen < AT_KEYS) {
+#pragma unroll
+        for (int e = 0; e < 64; ++e)
+          if (c * 64 + e >= seen) sv[e >> 5][e & 31] = 0xff800000u;
+      }
+    };
+    auto most = [&](const uint32_t (&sv)[2][32], float mx) {
+      float m0 = mx, m1 = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 32; e += 2) {
+        m0 = max3_f32(m0, __uint_as_float(sv[0][e]), __uint_as_float(sv[0][e + 1]));
+        m1 = max3_f32(m1, __uint_as_float(sv[1][e]), __uint_as_float(sv[1][e + 1]));
+      }
+      return fmaxf(m0, m1);
+    };
     for (int i = 0; i < n_x; ++i) {
       if (!__all_sync(0xffffffffu, mbar_wait_bounded(b_s + 8 * x, i & 1))) {
         if (lane == 0) arcb_set_error(a.status, ARCB_DEV_WAIT_TIMEOUT_ACC);
@@ -265,131 +271,118 @@ attn_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
         continue;
       }
       const int j = wide ? i : 2 * i + x;
-      const int seen = (j == n_tiles - 1 ? left : AT_KEYS) - half * 64;    // of the thread's 64 keys
-      auto load_scores = [&](int c, uint32_t (&sv)[32]) {
-        tmem_ld_32x32(t_s + c * 32, sv);
-        tmem_wait_ld_dep(sv);
-        if (seen < 64)
+      const int seen = j == n_tiles - 1 ? left : AT_KEYS;
+      uint32_t pr[2][32], second[WP > 1 ? 2 : 1][WP > 1 ? 32 : 1];
+      float mx, total;
+      // weights against the reference as it is, and the scores' maximum on the way
+      auto weights = [&]() {
+        const float m_safe = m_ref == -INFINITY ? 0.f : m_ref;
+        const uint64_t nm2 = pack_f32x2(-m_safe, -m_safe);
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        mx = -INFINITY;
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (c * 32 + e >= seen) sv[e] = 0xff800000u;
-      };
-      // the scores are read twice (maximum, then exponentials): tensor memory is quicker to read again than 64 registers are
-      // to hold
-      float mine = -INFINITY;
+        for (int c = 0; c < 2; ++c) {
+          uint32_t sv[2][32];
+          load_scores(c, seen, sv);
+          mx = most(sv, mx);
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t sv[32];
-        load_scores(c, sv);
-        float mx = fmaxf(__uint_as_float(sv[0]), __uint_as_float(sv[1]));
-#pragma unroll
-        for (int e = 2; e < 32; e += 2) mx = max3_f32(mx, __uint_as_float(sv[e]), __uint_as_float(sv[e + 1]));
-        mine = fmaxf(mine, mx);
-      }
-      mine *= sc;
-      float other;
-      const bool good = swap(mine, other);
-      if (!good) arcb_set_error(a.status, ARCB_DEV_WAIT_TIMEOUT_ACC);
-      ok = __all_sync(0xffffffffu, good);
-      if (!ok) break;
-      const float mx = fmaxf(mine, other);
-      float alpha = 1.f;
-      if (mx > m_ref + AT_RESCALE) {     // also the first tile (m_ref = -inf)
-        alpha = m_ref == -INFINITY ? 0.f : ex2_fast(m_ref - mx);
-        m_ref = mx;
-      }
-      l *= alpha;
-      const float m_safe = m_ref == -INFINITY ? 0.f : m_ref;
-      const uint64_t sc2 = pack_f32x2(sc, sc), nm2 = pack_f32x2(-m_safe, -m_safe);
-      if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-        // these scores were asked for behind the last product of values: its sums are complete
-#pragma unroll
-        for (int c = 0; c < D / 64; ++c) {
-          uint32_t o[32];
-          tmem_ld_32x32(t_o + c * 32, o);
-          tmem_wait_ld_dep(o);
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-          tmem_st_32x32(t_o + c * 32, o);
-        }
-      }
-      float ls0 = 0.f, ls1 = 0.f;
-      uint32_t lo[WP > 1 ? 16 : 1];
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t sv[32];
-        load_scores(c, sv);
-        if constexpr (WP > 1) {
-          if (c == 1) tmem_st_32x16(t_s + 32, lo);        // the first half's second pieces, over scores read by now
-        }
-        uint32_t hi[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float t0, t1;
-          shift2_f32(sv[2 * e], sv[2 * e + 1], sc2, nm2, t0, t1);
-          t0 = ex2_fast(t0);
-          t1 = ex2_fast(t1);
-          ls0 += t0;
-          ls1 += t1;
-          hi[e] = pack2_prob(t0, t1, HALF ? 1 : 0);
-          if constexpr (WP > 1) {
-            const float2 f = unpack2_act(hi[e], HALF ? 1 : 0);
-            lo[e] = pack2_prob(t0 - f.x, t1 - f.y, HALF ? 1 : 0);
+          for (int e = 0; e < 32; ++e) {
+            float t0, t1;
+            shift2_f32(sv[e >> 4][2 * (e & 15)], sv[e >> 4][2 * (e & 15) + 1], sc2, nm2, t0, t1);
+            t0 = ex2_fast(t0);
+            t1 = ex2_fast(t1);
+            sum[2 * (e & 1)] += t0;
+            sum[2 * (e & 1) + 1] += t1;
+            pr[c][e] = pack2_prob(t0, t1, HALF ? 1 : 0);
+            if constexpr (WP > 1) {
+              const float2 f = unpack2_act(pr[c][e], HALF ? 1 : 0);
+              second[c][e] = pack2_prob(t0 - f.x, t1 - f.y, HALF ? 1 : 0);
+            }
           }
         }
-        tmem_st_32x16(t_s + c * 16, hi);
-        if constexpr (WP > 1) {
-          if (c == 1) tmem_st_32x16(t_s + 48, lo);
+        total = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        mx *= sc;
+      };
+      if (i == 0) {
+        uint32_t sv[2][32];
+        load_scores(0, seen, sv);
+        mx = most(sv, -INFINITY);
+        load_scores(1, seen, sv);
+        m_ref = most(sv, mx) * sc;
+        weights();
+      } else {
+        // Nearly always the reference stays; where it has to be raised, the scores are still there.
+        weights();
+        const bool raise = mx > m_ref + AT_RESCALE;
+        if (__any_sync(0xffffffffu, raise)) {
+          float alpha = 1.f;
+          if (raise) {
+            alpha = m_ref == -INFINITY ? 0.f : ex2_fast(m_ref - mx);
+            m_ref = mx;
+            l *= alpha;
+          }
+          // these scores were asked for behind the last product of values: its sums are complete
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld_32x32(t_o + c * 32, o);
+            tmem_wait_ld_dep(o);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st_32x32(t_o + c * 32, o);
+          }
+          weights();
         }
       }
-      l += ls0 + ls1;
+      l += total;
+      // over scores that have all been read
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        tmem_st_32x32(t_s + c * 32, pr[c]);
+        if constexpr (WP > 1) tmem_st_32x32(t_s + 64 + c * 32, second[c]);
+      }
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(b_p + 8 * x);
     }
     // results: a quad of lanes writes 64 consecutive bytes of each of its four rows
     if (!idle) {
-      float l_other = 0.f;
-      if (ok && n_x > 0) {
-        bool good = swap(l, l_other);
-        good = mbar_wait_bounded(b_o + 8 * x, 0) && good;
-        if (!good) arcb_set_error(a.status, ARCB_DEV_WAIT_TIMEOUT_ACC);
-        ok = __all_sync(0xffffffffu, good);
+      if (ok && n_x > 0 && !__all_sync(0xffffffffu, mbar_wait_bounded(b_o + 8 * x, 0))) {
+        if (lane == 0) arcb_set_error(a.status, ARCB_DEV_WAIT_TIMEOUT_ACC);
+        ok = false;
       }
       const bool any = ok && n_x > 0;
-      const float l_row = half ? l_other + l : l + l_other;
       const int piece = lane & 3, quad_row = first_row + lane - piece;
       auto record = [&](int row, int part) {
         const int R = w.r0 + row;
         return ap_record(a, (long long)(w.item0 + R / a.rep) * a.n_heads + w.kvh * a.rep + R % a.rep, part);
       };
       const int part = 2 * w.part + (wide ? 0 : x);
-      if (any) tc_fence_after();
+      if (any) {
+        tc_fence_after();
+        float* to[4];
 #pragma unroll
-      for (int c = 0; c < D / 64; ++c) {
-        uint32_t o[32];
-        if (any) {
+        for (int e = 0; e < 4; ++e) to[e] = quad_row + e < w.rows ? record(quad_row + e, part) + piece * 4 : nullptr;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
           tmem_ld_32x32(t_o + c * 32, o);
           tmem_wait_ld_dep(o);
-        } else {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0u;
-        }
+          for (int g = 0; g < 2; ++g) {
+            uint4 v[4];
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          uint4 v[4];
+            for (int e = 0; e < 4; ++e) v[e] = make_uint4(o[g * 16 + e * 4], o[g * 16 + e * 4 + 1], o[g * 16 + e * 4 + 2], o[g * 16 + e * 4 + 3]);
+            quad_transpose(v, lane);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = make_uint4(o[g * 16 + e * 4], o[g * 16 + e * 4 + 1], o[g * 16 + e * 4 + 2], o[g * 16 + e * 4 + 3]);
-          quad_transpose(v, lane);
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (quad_row + e < w.rows)
-              *reinterpret_cast<uint4*>(record(quad_row + e, part) + half * (D / 2) + c * 32 + g * 16 + piece * 4) = v[e];
+            for (int e = 0; e < 4; ++e)
+              if (to[e]) *reinterpret_cast<uint4*>(to[e] + c * 32 + g * 16) = v[e];
+          }
         }
       }
       const int row = first_row + lane;
-      if (half == 0 && row < w.rows) {
-        *reinterpret_cast<float2*>(record(row, part) + D) = any ? make_float2(m_ref, l_row) : make_float2(-INFINITY, 0.f);
+      if (row < w.rows) {
+        *reinterpret_cast<float2*>(record(row, part) + D) = any ? make_float2(m_ref, l) : make_float2(-INFINITY, 0.f);
         if (wide) *reinterpret_cast<float2*>(record(row, part + 1) + D) = make_float2(-INFINITY, 0.f);     // one part where B has rows of its own
       }
     }
