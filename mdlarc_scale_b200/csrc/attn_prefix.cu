@@ -136,19 +136,15 @@ attn_prefix_simple_kernel(AttnPrefixArgs a) {
   }
 }
 
-// Joins the parts of an (item, head), W warps of a CTA for each; warp j adds parts j, j + W, ... in order, the warps' sums are
-// added in order.  With few results of many parts one warp alone would wait for memory a dozen times.
-template <int W>
+// Joins the parts of an (item, head) in order, a warp for each: the maximum of all, then their sums with lane s at the factor of
+// every 32nd part.
 __global__ void __launch_bounds__(128)
 attn_prefix_join_kernel(AttnPrefixArgs a) {
   pdl_launch_dependents();
   pdl_wait();
-  __shared__ float4 s_sum[W > 1 ? W : 1][32];
-  __shared__ float s_l[W > 1 ? W : 1];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, mine = warp % W;
-  const long long ih = (long long)blockIdx.x * (4 / W) + warp / W;
-  const bool out_of_range = ih >= (long long)a.n_items * a.n_heads;
-  if (W == 1 && out_of_range) return;
+  const int lane = threadIdx.x & 31;
+  const long long ih = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (ih >= (long long)a.n_items * a.n_heads) return;
   const int n = a.plan.parts, rec = a.dim + AP_PAD, c = lane * 4;
   const float* r0 = a.scratch + (size_t)ih * n * rec;
   float m = -INFINITY;
@@ -158,38 +154,87 @@ attn_prefix_join_kernel(AttnPrefixArgs a) {
   const float safe = m == -INFINITY ? 0.f : m;
   float l = 0.f;
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int base = 0; base < n; base += 32 * W) {
-    const int s = base + mine + lane * W;
+  for (int base = 0; base < n; base += 32) {
     float f = 0.f;
-    if (s < n) {
-      const float2 ml = *reinterpret_cast<const float2*>(r0 + (size_t)s * rec + a.dim);
+    if (base + lane < n) {
+      const float2 ml = *reinterpret_cast<const float2*>(r0 + (size_t)(base + lane) * rec + a.dim);
       f = exp2f(ml.x - safe);
       l += ml.y * f;
     }
-    const int here = min(32, (n - base - mine + W - 1) / W);
+    const int here = min(32, n - base);
 #pragma unroll 8
     for (int i = 0; i < here; ++i) {
       const float fi = __shfl_sync(0xffffffffu, f, i);
       if (c < a.dim && fi != 0.f) {        // an empty part's sums count for nothing, whatever they are
-        const float4 v = *reinterpret_cast<const float4*>(r0 + (size_t)(base + mine + i * W) * rec + c);
+        const float4 v = *reinterpret_cast<const float4*>(r0 + (size_t)(base + i) * rec + c);
         sum.x += v.x * fi; sum.y += v.y * fi; sum.z += v.z * fi; sum.w += v.w * fi;
       }
     }
   }
   l = warp_sum(l);
-  if (W > 1) {
-    s_sum[mine][lane] = sum;
-    if (lane == 0) s_l[mine] = l;
-    __syncthreads();
-    if (mine != 0) return;
-#pragma unroll
-    for (int j = 1; j < W; ++j) {
-      const float4 v = s_sum[j][lane];
-      sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
-      l += s_l[j];
-    }
-  }
   if (c >= a.dim) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  sum = a.item_skip && a.item_skip[ih / a.n_heads] ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+  ap_store4(a.out, (size_t)ih * a.dim + c, sum, a.act_fmt);
+}
+
+// Few results of many parts: a CTA for each; warp j takes parts j, j + 4, ... in order, eight at a time, so that their sums and
+// maxima travel together; the warps' results are joined in order.
+__global__ void __launch_bounds__(128)
+attn_prefix_join_cta_kernel(AttnPrefixArgs a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  constexpr int AHEAD = 8, W = 4;
+  __shared__ float4 s_sum[W][32];
+  __shared__ float2 s_ml[W];
+  const int lane = threadIdx.x & 31, mine = threadIdx.x >> 5;
+  const long long ih = blockIdx.x;
+  const int n = a.plan.parts, rec = a.dim + AP_PAD, c = min(lane * 4, a.dim - 4);
+  const float* r0 = a.scratch + (size_t)ih * n * rec;
+  float m = -INFINITY, l = 0.f;
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto join = [&](const float2* ml, const float4* v, int count) {
+    float top = m;
+#pragma unroll
+    for (int i = 0; i < count; ++i) top = fmaxf(top, ml[i].x);
+    const float safe = top == -INFINITY ? 0.f : top;
+    const float f0 = exp2f(m - safe);
+    l *= f0;
+    sum.x *= f0; sum.y *= f0; sum.z *= f0; sum.w *= f0;
+#pragma unroll
+    for (int i = 0; i < count; ++i) {
+      const float f = exp2f(ml[i].x - safe);
+      l += ml[i].y * f;
+      if (ml[i].x != -INFINITY) {        // an empty part's sums count for nothing, whatever they are
+        sum.x += v[i].x * f; sum.y += v[i].y * f; sum.z += v[i].z * f; sum.w += v[i].w * f;
+      }
+    }
+    m = top;
+  };
+  for (int base = mine; base < n; base += AHEAD * W) {
+    float2 ml[AHEAD];
+    float4 v[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int s = base + i * W;
+      ml[i] = s < n ? *reinterpret_cast<const float2*>(r0 + (size_t)s * rec + a.dim) : make_float2(-INFINITY, 0.f);
+      v[i] = s < n ? *reinterpret_cast<const float4*>(r0 + (size_t)s * rec + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    join(ml, v, AHEAD);
+  }
+  s_sum[mine][lane] = sum;
+  if (lane == 0) s_ml[mine] = make_float2(m, l);
+  __syncthreads();
+  if (mine != 0) return;
+  float2 ml[W - 1];
+  float4 v[W - 1];
+#pragma unroll
+  for (int i = 1; i < W; ++i) {
+    ml[i - 1] = s_ml[i];
+    v[i - 1] = s_sum[i][lane];
+  }
+  join(ml, v, W - 1);
+  if (lane * 4 >= a.dim) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;
   sum = a.item_skip && a.item_skip[ih / a.n_heads] ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
   ap_store4(a.out, (size_t)ih * a.dim + c, sum, a.act_fmt);
@@ -242,10 +287,10 @@ int arcb_launch_attn_prefix(AttnPrefixArgs a, cudaStream_t stream) {
   }
   if (r || p.parts == 1) return r;
   // four warps a result where a warp each would leave SMs without work
-  const bool few = p.parts >= 8 && joins < 4LL * arcb_num_sms();
+  const bool few = p.parts > 8 && joins < 4LL * arcb_num_sms();
   arcb_count_launch(1);
-  return (int)(few ? arcb_launch(attn_prefix_join_kernel<4>, dim3((unsigned)((long long)a.n_items * a.n_heads)), dim3(128), 0, stream, a)
-                   : arcb_launch(attn_prefix_join_kernel<1>, dim3((unsigned)joins), dim3(128), 0, stream, a));
+  return (int)(few ? arcb_launch(attn_prefix_join_cta_kernel, dim3((unsigned)((long long)a.n_items * a.n_heads)), dim3(128), 0, stream, a)
+                   : arcb_launch(attn_prefix_join_kernel, dim3((unsigned)joins), dim3(128), 0, stream, a));
 }
 
 static int to_fmt(int act_format) { return act_format == ARCB_ACT_F16 ? 1 : act_format == ARCB_ACT_BF16 ? 0 : 2; }

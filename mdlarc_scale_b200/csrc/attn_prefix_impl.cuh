@@ -69,7 +69,7 @@ __device__ __forceinline__ ApWork ap_work(const AttnPrefixArgs& a, long long blo
     }
     if (len < 0 || (a.item_skip && a.item_skip[k.item0])) len = 0;
     grain = a.plan.own.kernel == AP_TILES ? 63 : 15;
-    k.part = a.plan.shared_parts + split;
+    k.part = a.plan.shared.splits + split;
   }
   int chunk = (len + splits - 1) / splits;
   chunk = (chunk + grain) & ~grain;

@@ -2,8 +2,7 @@
 //
 // A CTA has up to 256 query rows of one (group, key head) as two tiles of 128, A and B, and goes through a range of cached rows
 // 128 at a time.  With up to 128 rows B has the same queries as A and takes every other key tile, so that there are always two
-// chains (scores, softmax, weights, values) of which one is in the tensor core while the other is at its exponentials; A's and
-// B's sums are then two parts of the result.
+// chains (scores, softmax, weights, values) of which one is in the tensor core while the other is at its exponentials.
 //   warp 0        TMA: key and value tiles as 128 x 64 boxes with the 128-byte swizzle, rings shared by A and B; value rows
 //                 behind the end of the last tile are set to zero: a weight of 0 does not hide a NaN
 //   warps 1, 2    products of A and of B: S = Q K^T (128 TMEM columns), O += P V with P read from TMEM
@@ -345,29 +344,67 @@ attn_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
       tc_fence_before();
       mbar_arrive(b_p + 8 * x);
     }
-    // results: a quad of lanes writes 64 consecutive bytes of each of its four rows
-    if (!idle) {
-      if (ok && n_x > 0 && !__all_sync(0xffffffffu, mbar_wait_bounded(b_o + 8 * x, 0))) {
-        if (lane == 0) arcb_set_error(a.status, ARCB_DEV_WAIT_TIMEOUT_ACC);
-        ok = false;
+    if (!idle && ok && n_x > 0 && !__all_sync(0xffffffffu, mbar_wait_bounded(b_o + 8 * x, 0))) {
+      if (lane == 0) arcb_set_error(a.status, ARCB_DEV_WAIT_TIMEOUT_ACC);
+      ok = false;
+    }
+    const bool any = ok && n_x > 0;
+    tc_fence_after();
+    // With one tile of queries B's sums are handed to A's threads through the ring, which nothing reads any more.
+    constexpr int REC = D + 4;
+    static_assert(AT_ROWS * REC * 4 <= 2 * C::STAGES * C::KV_BYTES, "the ring holds B's sums");
+    float* theirs = reinterpret_cast<float*>(base_ptr + 2 * C::Q_BYTES) + (quarter * 32 + lane) * REC;
+    float fa = 1.f, fb = 0.f;
+    if (!wide) {
+      named_bar_sync(1, 256);
+      if (x == 1 && !idle) {
+        if (any)
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld_32x32(t_o + c * 32, o);
+            tmem_wait_ld_dep(o);
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(theirs + c * 32 + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          }
+        *reinterpret_cast<float2*>(theirs + D) = any ? make_float2(m_ref, l) : make_float2(-INFINITY, 0.f);
       }
-      const bool any = ok && n_x > 0;
+      named_bar_sync(1, 256);
+      if (x == 0 && !idle) {
+        const float2 ml = *reinterpret_cast<const float2*>(theirs + D);
+        const float top = fmaxf(m_ref, ml.x), safe = top == -INFINITY ? 0.f : top;
+        fa = exp2f(m_ref - safe);
+        fb = ml.x == -INFINITY ? 0.f : exp2f(ml.x - safe);
+        m_ref = top;
+        l = l * fa + ml.y * fb;
+      }
+    }
+    // results: a quad of lanes writes 64 consecutive bytes of each of its four rows
+    if (!idle && (wide || x == 0)) {
       const int piece = lane & 3, quad_row = first_row + lane - piece;
-      auto record = [&](int row, int part) {
+      auto record = [&](int row) {
         const int R = w.r0 + row;
-        return ap_record(a, (long long)(w.item0 + R / a.rep) * a.n_heads + w.kvh * a.rep + R % a.rep, part);
+        return ap_record(a, (long long)(w.item0 + R / a.rep) * a.n_heads + w.kvh * a.rep + R % a.rep, w.part);
       };
-      const int part = 2 * w.part + (wide ? 0 : x);
       if (any) {
-        tc_fence_after();
+        const bool both = __any_sync(0xffffffffu, fb != 0.f);
         float* to[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) to[e] = quad_row + e < w.rows ? record(quad_row + e, part) + piece * 4 : nullptr;
+        for (int e = 0; e < 4; ++e) to[e] = quad_row + e < w.rows ? record(quad_row + e) + piece * 4 : nullptr;
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
           tmem_ld_32x32(t_o + c * 32, o);
           tmem_wait_ld_dep(o);
+          if (both)
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+              const float4 v = *reinterpret_cast<const float4*>(theirs + c * 32 + e);
+              o[e] = __float_as_uint(__uint_as_float(o[e]) * fa + v.x * fb);
+              o[e + 1] = __float_as_uint(__uint_as_float(o[e + 1]) * fa + v.y * fb);
+              o[e + 2] = __float_as_uint(__uint_as_float(o[e + 2]) * fa + v.z * fb);
+              o[e + 3] = __float_as_uint(__uint_as_float(o[e + 3]) * fa + v.w * fb);
+            }
 #pragma unroll
           for (int g = 0; g < 2; ++g) {
             uint4 v[4];
@@ -381,10 +418,7 @@ attn_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
         }
       }
       const int row = first_row + lane;
-      if (row < w.rows) {
-        *reinterpret_cast<float2*>(record(row, part) + D) = any ? make_float2(m_ref, l) : make_float2(-INFINITY, 0.f);
-        if (wide) *reinterpret_cast<float2*>(record(row, part + 1) + D) = make_float2(-INFINITY, 0.f);     // one part where B has rows of its own
-      }
+      if (row < w.rows) *reinterpret_cast<float2*>(record(row) + D) = any ? make_float2(m_ref, l) : make_float2(-INFINITY, 0.f);
     }
   }
   tc_fence_before();

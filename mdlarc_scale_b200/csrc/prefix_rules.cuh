@@ -17,7 +17,7 @@ struct PrefixPart {
 struct PrefixPlan {
   PrefixPart shared, own;
   int together;             // both parts in one launch
-  int shared_parts, parts;  // of a result: of the shared rows, and all
+  int parts;                // of a result
 };
 
 // `rows` query rows at each of `heads` (groups or items) x n_kv; `tc`: tcgen05 may be used.
@@ -67,7 +67,6 @@ inline PrefixPlan prefix_plan(long long n_groups, long long max_group, long long
   }
   p.shared.units *= p.shared.splits;
   p.own.units *= p.own.splits;
-  p.shared_parts = p.shared.kernel == AP_TC ? 2 * p.shared.splits : p.shared.splits;      // two chains a CTA
-  p.parts = p.shared_parts + p.own.splits;
+  p.parts = p.shared.splits + p.own.splits;
   return p;
 }
