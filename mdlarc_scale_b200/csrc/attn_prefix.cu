@@ -279,18 +279,22 @@ int arcb_launch_attn_prefix(AttnPrefixArgs a, cudaStream_t stream) {
   const long long joins = ((long long)a.n_items * a.n_heads + 3) / 4;
   if (p.shared.units + p.own.units > 0x7fffffffLL || joins > 0x1fffffffLL) return -1;
   a.first_block = 0;
+  a.beside = 0;
   int r = 0;
   if (p.shared.units > 0) r = launch_part(a, p.shared.kernel, p.shared.units + (p.together ? p.own.units : 0), stream);
   if (r == 0 && p.own.units > 0 && !p.together) {
     a.first_block = p.shared.units;
+    // Beside the shared part, which it does not depend on.  What came before that one is over when it starts, unless the library
+    // launches everything programmatically.
+    a.beside = p.shared.units > 0 && !arcb_pdl_enabled();
     r = launch_part(a, p.own.kernel, p.own.units, stream);
   }
   if (r || p.parts == 1) return r;
-  // four warps a result where a warp each would leave SMs without work
+  // Its CTAs come while the last ones of the parts are at work, and wait.  Four warps a result where a warp each would leave SMs without work
   const bool few = p.parts > 8 && joins < 4LL * arcb_num_sms();
   arcb_count_launch(1);
-  return (int)(few ? arcb_launch(attn_prefix_join_cta_kernel, dim3((unsigned)((long long)a.n_items * a.n_heads)), dim3(128), 0, stream, a)
-                   : arcb_launch(attn_prefix_join_kernel, dim3((unsigned)joins), dim3(128), 0, stream, a));
+  return (int)(few ? ap_launch_beside(attn_prefix_join_cta_kernel, dim3((unsigned)((long long)a.n_items * a.n_heads)), dim3(128), 0, stream, a)
+                   : ap_launch_beside(attn_prefix_join_kernel, dim3((unsigned)joins), dim3(128), 0, stream, a));
 }
 
 static int to_fmt(int act_format) { return act_format == ARCB_ACT_F16 ? 1 : act_format == ARCB_ACT_BF16 ? 0 : 2; }

@@ -30,6 +30,7 @@ struct AttnPrefixArgs {
   int rep;
   PrefixPlan plan;
   long long first_block;      // of the launch, in the numbering of the whole work
+  int beside;                 // the launch runs beside the one ahead of it, whose end it waits for at its own
 };
 
 constexpr int AP_PAD = 4;     // of a partial result: the sums of a row's values, its maximum (log2 units), its sum, two spare

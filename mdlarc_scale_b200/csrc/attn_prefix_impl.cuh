@@ -2,10 +2,29 @@
 // results go, how outputs are rounded.
 #pragma once
 #include "attn_prefix.cuh"
+#include "launch.cuh"
 
 namespace {
 
 constexpr float AP_LOG2E = 1.4426950408889634f;
+
+// Launch with the programmatic attribute: the kernel's CTAs may come when all of the kernel ahead have started.
+template <typename... KArgs, typename... Args>
+inline cudaError_t ap_launch_beside(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+  if (e != cudaSuccess) cudaGetLastError();
+  return e;
+}
 
 // A CTA's part of the work: query rows (row r is item item0 + (r0 + r) / rep, head kvh * rep + (r0 + r) % rep), cached rows
 // [begin, end) of a sequence, and which part of the results it is.

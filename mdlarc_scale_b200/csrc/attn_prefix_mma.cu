@@ -248,13 +248,13 @@ template <int D, bool HALF, bool QS>
 __global__ void __launch_bounds__(128, AmCfg<D>::MIN_CTAS)
 attn_prefix_mma_kernel(AttnPrefixArgs a) {
   pdl_launch_dependents();
-  pdl_wait();
+  if (!a.beside) pdl_wait();
   extern __shared__ __align__(128) uint8_t am_smem[];
   const ApWork w = ap_work(a, a.first_block + blockIdx.x, threadIdx.x == 0);
-  if (w.rows <= 0) return;
-  if (w.rows <= 16) am_body<D, HALF, QS, 4>(a, w, am_smem);
-  else if (w.rows <= 32) am_body<D, HALF, QS, 2>(a, w, am_smem);
-  else am_body<D, HALF, QS, 1>(a, w, am_smem);
+  if (w.rows > 32) am_body<D, HALF, QS, 1>(a, w, am_smem);
+  else if (w.rows > 16) am_body<D, HALF, QS, 2>(a, w, am_smem);
+  else if (w.rows > 0) am_body<D, HALF, QS, 4>(a, w, am_smem);
+  if (a.beside) pdl_wait();      // this launch's end is the other's too
 }
 
 template <int D, bool HALF, bool QS>
@@ -262,7 +262,8 @@ int am_launch(const AttnPrefixArgs& a, unsigned blocks, cudaStream_t stream) {
   static std::atomic<unsigned long long> done{0};
   const cudaError_t e = arcb_opt_in_smem(attn_prefix_mma_kernel<D, HALF, QS>, AmCfg<D>::SMEM, done);
   if (e != cudaSuccess) return (int)e;
-  return (int)arcb_launch(attn_prefix_mma_kernel<D, HALF, QS>, dim3(blocks), dim3(128), AmCfg<D>::SMEM, stream, a);
+  return (int)(a.beside ? ap_launch_beside(attn_prefix_mma_kernel<D, HALF, QS>, dim3(blocks), dim3(128), AmCfg<D>::SMEM, stream, a)
+                        : arcb_launch(attn_prefix_mma_kernel<D, HALF, QS>, dim3(blocks), dim3(128), AmCfg<D>::SMEM, stream, a));
 }
 
 }  // namespace

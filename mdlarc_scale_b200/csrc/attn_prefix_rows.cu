@@ -302,14 +302,18 @@ __global__ void __launch_bounds__(AR_WARPS * 32, ArCfg<D>::CTAS)
 attn_prefix_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, AttnPrefixArgs a, long long n_units) {
   using C = ArCfg<D>;
   pdl_launch_dependents();
-  pdl_wait();
+  if (!a.beside) pdl_wait();
   extern __shared__ __align__(1024) uint8_t ar_smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long stride = (long long)gridDim.x * AR_WARPS, first = (long long)warp * gridDim.x + blockIdx.x;
-  if (first >= n_units) return;
+  if (first >= n_units) {
+    if (a.beside) pdl_wait();
+    return;
+  }
   const uint32_t base = smem_u32(ar_smem), ring = base + warp * C::WARP, bars = base + AR_WARPS * C::WARP + warp * (8 * C::STAGES);
   if (base & 1023u) {
     arcb_set_error(a.status, ARCB_DEV_BAD_INDEX);
+    if (a.beside) pdl_wait();
     return;
   }
   if (lane == 0) {
@@ -332,6 +336,7 @@ attn_prefix_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid
       w = s.ahead;
     }
   }
+  if (a.beside) pdl_wait();      // this launch's end is the other's too
 }
 
 template <int D, bool HALF, bool QS>
@@ -346,8 +351,9 @@ int ar_launch(const AttnPrefixArgs& a, long long units, cudaStream_t stream) {
   if (!r) r = arcb_make_tmap_2d_16b(&tv, a.v, rows, D, C::KEYS, 64, HALF);
   if (r) return 1000 + r;
   const long long most = (long long)C::CTAS * arcb_num_sms();
-  return (int)arcb_launch(attn_prefix_rows_kernel<D, HALF, QS>, dim3((unsigned)(units < most ? units : most)), dim3(AR_WARPS * 32), C::SMEM, stream, tk, tv,
-                          a, units);
+  const dim3 grid((unsigned)(units < most ? units : most));
+  return (int)(a.beside ? ap_launch_beside(attn_prefix_rows_kernel<D, HALF, QS>, grid, dim3(AR_WARPS * 32), C::SMEM, stream, tk, tv, a, units)
+                        : arcb_launch(attn_prefix_rows_kernel<D, HALF, QS>, grid, dim3(AR_WARPS * 32), C::SMEM, stream, tk, tv, a, units));
 }
 }  // namespace
 

@@ -7,6 +7,7 @@
 // keeps the call free of device memory of its own (and a captured one independent of later calls).
 #include "../../include/arcb200.h"
 #include "cache_copy.cuh"
+#include "gemm.cuh"
 #include "launch.cuh"
 
 int arcb_fail(int code, const char* msg);
@@ -15,69 +16,103 @@ int arcb_fail_cuda(cudaError_t e, const char* where);
 namespace {
 
 constexpr int CC_THREADS = 256;
-constexpr int CC_UNROLL = 4;
 
 template <int STEPS>
 struct CopyArgs {
   CopyGeometry g;
-  int n_programs, row_vecs;
+  int row_vecs, turns;        // vectors of a row; times that a CTA goes on by its threads' places
   CopyStep step[STEPS];
-  // of each program: first step and rows, packed where there is room for as many programs as steps / 2
-  unsigned short first[STEPS / 2 + 1];
+  unsigned short first[STEPS / 2 + 1];      // step of each program (which has two at least)
 };
 
+// place i of a program: its address in a sequence at 0, and its row (-1: there is none)
+struct CopyPlace {
+  char* at;
+  int row;
+};
+template <typename VEC, int STEPS>
+__device__ __forceinline__ CopyPlace cc_place(const CopyArgs<STEPS>& a, unsigned i, unsigned total, unsigned run, int lo) {
+  CopyPlace p;
+  const unsigned pb = i / run, off = i - pb * run, plane = pb / a.g.blocks, b = pb - plane * a.g.blocks;
+  p.row = i < total ? lo + (int)(off / a.row_vecs) : -1;
+  p.at = reinterpret_cast<char*>(a.g.base) + plane * a.g.plane_stride + b * a.g.block_stride + ((long long)lo * a.row_vecs + off) * (long long)sizeof(VEC);
+  return p;
+}
+
+// Programs of one source: four places a thread in a turn, the next turn's rows on their way while this one's are written.  (A CTA a
+// turn spent most of its time starting: 77 sequences moved in 475 us, 5.5 TB/s, or 775 us with the registers of the other kernel.)
 template <int STEPS, typename VEC>
 __global__ void __launch_bounds__(CC_THREADS)
-cache_copy_kernel(const __grid_constant__ CopyArgs<STEPS> a) {
+cache_spread_kernel(const __grid_constant__ CopyArgs<STEPS> a) {
   pdl_launch_dependents();
   pdl_wait();
+  constexpr int U = 4;
   const int from = a.first[blockIdx.y], to = a.first[blockIdx.y + 1];
   // the first step is a load: its unused row fields hold the program's rows
   const int lo = a.step[from].begin, hi = a.step[from].end;
-  const unsigned run = (unsigned)(hi - lo) * a.row_vecs;
-  const unsigned total = run * (unsigned)(a.g.planes * a.g.blocks);
-  const unsigned base = blockIdx.x * (unsigned)(CC_THREADS * CC_UNROLL);
+  const unsigned run = (unsigned)(hi - lo) * a.row_vecs, total = run * (unsigned)(a.g.planes * a.g.blocks);
+  const long long src = a.step[from].slot * a.g.seq_stride;
+  unsigned base = blockIdx.x * (unsigned)(CC_THREADS * U) * a.turns;
   if (base >= total) return;
-  char* at[CC_UNROLL];
-  int row[CC_UNROLL];
+  CopyPlace now[U], next[U];
+  VEC v[U], w[U];
+  auto fetch = [&](CopyPlace (&p)[U], VEC (&x)[U]) {
 #pragma unroll
-  for (int u = 0; u < CC_UNROLL; ++u) {
-    const unsigned i = base + u * CC_THREADS + threadIdx.x;
-    const unsigned pb = i / run, off = i - pb * run;
-    const unsigned p = pb / a.g.blocks, b = pb - p * a.g.blocks;
-    row[u] = i < total ? lo + (int)(off / a.row_vecs) : -1;        // -1: no step has it
-    at[u] = reinterpret_cast<char*>(a.g.base) + (i < total ? p * a.g.plane_stride + b * a.g.block_stride +
-                                                             ((long long)lo * a.row_vecs + off) * (long long)sizeof(VEC) : 0);
+    for (int u = 0; u < U; ++u) {
+      p[u] = cc_place<VEC>(a, base + u * CC_THREADS + threadIdx.x, total, run, lo);
+      if (p[u].row >= 0) x[u] = *reinterpret_cast<const VEC*>(p[u].at + src);
+    }
+    base += CC_THREADS * U;
+  };
+  fetch(now, v);
+  for (int t = 1;; ++t) {
+    const bool more = t < a.turns && base < total;
+    if (more) fetch(next, w);
+    for (int s = from + 1; s < to; ++s) {
+      const CopyStep c = a.step[s];
+      const long long d = c.slot * a.g.seq_stride;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (now[u].row >= c.begin && now[u].row < c.end) *reinterpret_cast<VEC*>(now[u].at + d) = v[u];
+    }
+    if (!more) break;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      now[u] = next[u];
+      v[u] = w[u];
+    }
   }
-  VEC v[CC_UNROLL], held[CC_UNROLL];
+}
+
+// Programs of several sources: one place a thread.
+template <int STEPS, typename VEC>
+__global__ void __launch_bounds__(CC_THREADS)
+cache_permute_kernel(const __grid_constant__ CopyArgs<STEPS> a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int from = a.first[blockIdx.y], to = a.first[blockIdx.y + 1];
+  const int lo = a.step[from].begin, hi = a.step[from].end;
+  const unsigned run = (unsigned)(hi - lo) * a.row_vecs, total = run * (unsigned)(a.g.planes * a.g.blocks), i = blockIdx.x * CC_THREADS + threadIdx.x;
+  if (i >= total) return;
+  const CopyPlace p = cc_place<VEC>(a, i, total, run, lo);
+  VEC v[COPY_VALUES + 1];
   for (int s = from; s < to; ++s) {
     const CopyStep c = a.step[s];
-    const long long d = c.slot * a.g.seq_stride;
-    if (c.op == COPY_LOAD) {
+    VEC* at = reinterpret_cast<VEC*>(p.at + c.slot * a.g.seq_stride);
+    const bool mine = p.row >= c.begin && p.row < c.end;
 #pragma unroll
-      for (int u = 0; u < CC_UNROLL; ++u)
-        if (row[u] >= 0) v[u] = *reinterpret_cast<const VEC*>(at[u] + d);
-    } else if (c.op == COPY_STORE) {
-#pragma unroll
-      for (int u = 0; u < CC_UNROLL; ++u)
-        if (row[u] >= c.begin && row[u] < c.end) *reinterpret_cast<VEC*>(at[u] + d) = v[u];
-    } else if (c.op == COPY_HOLD) {
-#pragma unroll
-      for (int u = 0; u < CC_UNROLL; ++u)
-        if (row[u] >= 0) held[u] = *reinterpret_cast<const VEC*>(at[u] + d);
-    } else {
-#pragma unroll
-      for (int u = 0; u < CC_UNROLL; ++u)
-        if (row[u] >= c.begin && row[u] < c.end) *reinterpret_cast<VEC*>(at[u] + d) = held[u];
+    for (int k = 0; k <= COPY_VALUES; ++k) {       // one of them, the same for all threads
+      if (c.op == k) v[k] = *at;
+      else if (c.op == COPY_STORE + k && mine) *at = v[k];
     }
   }
 }
 
 template <int STEPS, typename VEC>
-int launch_programs(const CopyGeometry& g, const CopyProgram* const* progs, int n, cudaStream_t stream) {
+int launch_programs(const CopyGeometry& g, const std::vector<const CopyProgram*>& progs, bool single, cudaStream_t stream) {
   CopyArgs<STEPS> a;
   a.row_vecs = g.row_bytes / (int)sizeof(VEC);
-  a.n_programs = n;
+  const int n = (int)progs.size();
   int steps = 0, rows = 0;
   for (int i = 0; i < n; ++i) {
     const CopyProgram& p = *progs[i];
@@ -98,8 +133,12 @@ int launch_programs(const CopyGeometry& g, const CopyProgram* const* progs, int 
     a.g.base = reinterpret_cast<char*>(g.base) + p * g.plane_stride;
     a.g.planes = g.planes - p < at_once ? g.planes - p : at_once;
     const long long places = per_plane * a.g.planes;
-    const unsigned blocks = (unsigned)((places + CC_THREADS * CC_UNROLL - 1) / (CC_THREADS * CC_UNROLL));
-    const cudaError_t e = arcb_launch(cache_copy_kernel<STEPS, VEC>, dim3(blocks, n), dim3(CC_THREADS), 0, stream, a);
+    // up to eight turns, as long as sixteen CTAs an SM are left; one where a place is written many times anyway
+    const long long turn = single ? CC_THREADS * 4 : CC_THREADS, ctas = (places + turn - 1) / turn * n;
+    a.turns = !single || steps > 4 * n ? 1 : (int)(ctas >= 128LL * arcb_num_sms() ? 8 : ctas >= 32LL * arcb_num_sms() ? 2 : 1);
+    const dim3 grid((unsigned)((places + turn * a.turns - 1) / (turn * a.turns)), n);
+    const cudaError_t e = single ? arcb_launch(cache_spread_kernel<STEPS, VEC>, grid, dim3(CC_THREADS), 0, stream, a)
+                                 : arcb_launch(cache_permute_kernel<STEPS, VEC>, grid, dim3(CC_THREADS), 0, stream, a);
     arcb_count_launch(1);
     if (e != cudaSuccess) return (int)e;
   }
@@ -107,12 +146,11 @@ int launch_programs(const CopyGeometry& g, const CopyProgram* const* progs, int 
 }
 
 template <typename VEC>
-int launch_batch(const CopyGeometry& g, const std::vector<const CopyProgram*>& batch, size_t steps, cudaStream_t stream) {
-  const int n = (int)batch.size();
-  if (!n) return 0;
-  if (steps <= 48) return launch_programs<48, VEC>(g, batch.data(), n, stream);
-  if (steps <= 400) return launch_programs<400, VEC>(g, batch.data(), n, stream);
-  return launch_programs<COPY_MAX_STEPS, VEC>(g, batch.data(), n, stream);
+int launch_batch(const CopyGeometry& g, const std::vector<const CopyProgram*>& batch, size_t steps, bool single, cudaStream_t stream) {
+  if (batch.empty()) return 0;
+  if (steps <= 48) return launch_programs<48, VEC>(g, batch, single, stream);
+  if (steps <= 400) return launch_programs<400, VEC>(g, batch, single, stream);
+  return launch_programs<COPY_MAX_STEPS, VEC>(g, batch, single, stream);
 }
 
 static_assert(sizeof(CopyArgs<COPY_MAX_STEPS>) <= 32764, "launch parameters");
@@ -123,19 +161,22 @@ int arcb_launch_cache_copy(const CopyGeometry& g, const std::vector<CopyProgram>
   const long long any = reinterpret_cast<long long>(g.base) | g.plane_stride | g.seq_stride | g.block_stride | g.row_bytes;
   if (any & 3) return -1;
   const bool wide = !(any & 15);
+  bool single = true;                      // every program has one source
+  for (const CopyProgram& p : programs) {
+    single = single && p.steps[0].op == 0;
+    for (size_t s = 1; s < p.steps.size() && single; ++s) single = p.steps[s].op == COPY_STORE;
+  }
   std::vector<const CopyProgram*> batch;
   size_t steps = 0;
   auto flush = [&]() {
-    const int r = wide ? launch_batch<uint4>(g, batch, steps, stream) : launch_batch<uint32_t>(g, batch, steps, stream);
+    const int r = wide ? launch_batch<uint4>(g, batch, steps, single, stream) : launch_batch<uint32_t>(g, batch, steps, single, stream);
     batch.clear();
     steps = 0;
     return r;
   };
   for (size_t i = 0; i < programs.size(); ++i) {
-    if (steps + programs[i].steps.size() > COPY_MAX_STEPS || serial[i]) {
-      const int r = flush();
-      if (r) return r;
-    }
+    if (serial[i] || steps + programs[i].steps.size() > COPY_MAX_STEPS)
+      if (const int r = flush()) return r;
     batch.push_back(&programs[i]);
     steps += programs[i].steps.size();
   }

@@ -26,7 +26,7 @@ extern "C" int plan(const int* copies, int n, int n_seqs, int t_max, int most, i
   return r;
 }
 """
-LOAD, STORE, HOLD, STORE_HELD = range(4)
+STORE = 8        # op: number of the value, this much more for a store
 
 
 @pytest.fixture(scope="module")
@@ -64,16 +64,14 @@ def carry_out(programs, state, order):
     for launch in launches:
         for i in order(len(launch)):
             steps, lo, hi, _ = launch[i]
-            assert steps[0][3] in (LOAD, HOLD)       # the kernel keeps the program's rows in the first step
+            assert steps[0][3] < STORE               # the kernel keeps the program's rows in the first step
             for r in range(lo, hi):
-                v = held = None
+                v = [None] * 5
                 for slot, b, e, op in steps.tolist():
-                    if op == LOAD:
-                        v = state[slot, r]
-                    elif op == HOLD:
-                        held = state[slot, r]
+                    if op < STORE:
+                        v[op] = state[slot, r]
                     elif b <= r < e:
-                        state[slot, r] = v if op == STORE else held
+                        state[slot, r] = v[op - STORE]
     return state
 
 
@@ -89,7 +87,7 @@ def check(lib, copies, seqs, rows, most=1900):
 
 def test_fork_reads_once(lib):
     programs = check(lib, [(2, d, 0, 3 + d) for d in (0, 1, 3, 4)], 5, 9)
-    assert len(programs) == 1 and sum(s[3] == LOAD for s in programs[0][0].tolist()) == 1
+    assert len(programs) == 1 and sum(s[3] < STORE for s in programs[0][0].tolist()) == 1
 
 
 def test_independent_copies_are_programs_of_their_own(lib):
