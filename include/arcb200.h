@@ -288,11 +288,18 @@ typedef struct arcb_session_desc {
                                      grid model's END is fixed).  d_step_logits is then
                                      [B][max_new][vocab], and the cache buffer holds per layer either
                                      keys and values or the recurrent state of every sequence     */
+  int32_t prefix_group;           /* grid model: n > 1 = rows g n ... g n + n - 1 are samples of one prompt, whose keys and
+                                     values only row g n holds: decode steps read them there once for all of them, and a
+                                     row's own cache from the end of the prompt on.  Prefill the prompts of rows g n alone and
+                                     name the same d_first_row for the n rows.  n divides n_seqs; the workspace grows by
+                                     arcb_session_prefix_bytes.  0 or 1: every row holds its prompt            */
 } arcb_session_desc;
 
 int64_t arcb_session_workspace_bytes(const arcb_engine* eng, int32_t n_seqs,
                                      int32_t max_prefill_tokens, int32_t attn_splits);
 int64_t arcb_kv_cache_bytes(const arcb_engine* eng, int32_t n_seqs, int32_t t_max);
+/* what a session with prefix_group > 1 needs in its workspace on top of arcb_session_workspace_bytes; < 0: not supported */
+int64_t arcb_session_prefix_bytes(const arcb_engine* eng, int32_t n_seqs, int32_t t_max, int32_t max_new, int32_t prefix_group);
 /* Creating a session launches nothing: the session's device state (inside d_workspace) is cleared
  * by the session's FIRST arcb_prefill, on that call's stream, so a workspace recycled from an
  * earlier session is ordered after whatever that stream still has queued on it.  Use one stream
@@ -391,6 +398,11 @@ int arcb_session_step_logits(arcb_session* s, float** d_logits, int32_t* pitch);
 /* Layered engines: synchronises `stream` and copies one flag per sequence to the host: 1 = the sequence has
  * emitted end_token or used up max_new (it is held then). */
 int arcb_session_finished(arcb_session* s, int32_t* h_finished, void* stream);
+
+/* Copies what sequence src holds to the sequences h_dst[n_dst] (host memory, free when the call returns): keys, values or latents of its
+ * first `rows` positions and, on layered engines, recurrent states and the position it continues at, so that `rows` is its
+ * length there.  The targets then continue from there; what they have produced and whether they are armed stays theirs. */
+int arcb_session_fork(arcb_session* s, int32_t src, int32_t rows, const int32_t* h_dst, int32_t n_dst, void* stream);
 
 /* Synchronises `stream`, then reports how many rows have emitted END and the
  * device error word (0 = none). Replaces `finished.all()` (src/inference.py:594). */

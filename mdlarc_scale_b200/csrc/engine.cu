@@ -10,6 +10,7 @@
 
 #include "../../include/arcb200.h"
 #include "attn_prefill.cuh"
+#include "attn_prefix.cuh"
 #include "attn_stream.cuh"
 #include "gemm.cuh"
 #include "gemm_split.cuh"
@@ -253,6 +254,32 @@ extern "C" int64_t arcb_kv_cache_bytes(const arcb_engine* e, int32_t n_seqs, int
   return (int64_t)e->cfg.n_layers * 2 * n_seqs * e->cfg.d_model * (int64_t)t_max * 2;
 }
 
+// Decode attention of rows in groups of `group` that share the first one's prompt; sizes only.
+static AttnPrefixArgs prefix_args(const arcb_engine* e, int n_seqs, int t_max, int max_new, int group) {
+  AttnPrefixArgs a{};
+  a.uniform = a.max_group = group;
+  a.n_groups = n_seqs / group;
+  a.n_items = a.n_seqs = n_seqs;
+  a.n_heads = a.n_kv = e->cfg.n_heads;
+  a.dim = ARCB_HEAD_DIM;
+  a.t_max = t_max;
+  a.max_prefix = t_max > max_new ? t_max - max_new : 1;
+  a.max_own = max_new < t_max ? max_new : t_max;
+  a.scale = 0.125f;
+  a.act_fmt = e->act_f16() ? 1 : 0;
+  a.kv_fmt = 0;
+  static const int any = 0;
+  a.item_end = &any;            // own rows: set when launched
+  return a;
+}
+
+extern "C" int64_t arcb_session_prefix_bytes(const arcb_engine* e, int32_t n_seqs, int32_t t_max, int32_t max_new, int32_t group) {
+  if (!e || n_seqs <= 0 || t_max <= 0 || max_new <= 0) return -1;
+  if (group <= 1) return 0;
+  if (e->lm || n_seqs % group || (int64_t)n_seqs * e->cfg.n_heads * t_max >= (1ll << 31) - 256) return -1;
+  return (int64_t)align_up((size_t)arcb_attn_prefix_scratch(prefix_args(e, n_seqs, t_max, max_new, group)), 256);
+}
+
 extern "C" int arcb_session_create(arcb_engine* e, const arcb_session_desc* dsc, arcb_session** out) {
   if (!e || !dsc || !out) return arcb_fail(ARCB_E_ARG, "null argument");
   if (!engine_complete(e)) return arcb_fail(ARCB_E_STATE, "engine is missing tensors");
@@ -264,6 +291,7 @@ extern "C" int arcb_session_create(arcb_engine* e, const arcb_session_desc* dsc,
   if (((uintptr_t)dsc->d_kv_cache & 255) || ((uintptr_t)dsc->d_workspace & 255))
     return arcb_fail(ARCB_E_ARG, "buffers must be 256-byte aligned");
   if (e->lm) {
+    if (dsc->prefix_group > 1) return arcb_fail(ARCB_E_UNSUPPORTED, "prefix_group is for the grid model: arcb_session_fork copies what a sequence holds");
     if (dsc->workspace_bytes < lm_workspace_bytes(e, dsc->n_seqs, dsc->max_prefill_tokens, dsc->attn_splits))
       return arcb_fail(ARCB_E_ARG, "workspace too small");
     arcb_session* s = new arcb_session();
@@ -280,7 +308,9 @@ extern "C" int arcb_session_create(arcb_engine* e, const arcb_session_desc* dsc,
   }
   const int splits = choose_splits(e, dsc->n_seqs, dsc->attn_splits, dsc->t_max);
   const WsLayout w = ws_layout(e, dsc->n_seqs, dsc->max_prefill_tokens, scratch_splits(e, dsc->n_seqs, dsc->attn_splits));
-  if ((size_t)dsc->workspace_bytes < w.total) return arcb_fail(ARCB_E_ARG, "workspace too small");
+  const int64_t prefix_bytes = arcb_session_prefix_bytes(e, dsc->n_seqs, dsc->t_max, dsc->max_new, dsc->prefix_group);
+  if (prefix_bytes < 0 || dsc->prefix_group < 0) return arcb_fail(ARCB_E_ARG, "prefix_group must divide n_seqs, in a cache of fewer than 2^31 rows");
+  if ((size_t)dsc->workspace_bytes < w.total + (size_t)prefix_bytes) return arcb_fail(ARCB_E_ARG, "workspace too small");
   arcb_session* s = new arcb_session();
   s->eng = e;
   s->desc = *dsc;
@@ -295,6 +325,7 @@ extern "C" int arcb_session_create(arcb_engine* e, const arcb_session_desc* dsc,
   s->v16 = reinterpret_cast<uint16_t*>(base + w.v16);
   s->attn_scratch = scratch_splits(e, dsc->n_seqs, dsc->attn_splits) > 1 ? reinterpret_cast<float*>(base + w.scratch) : nullptr;
   s->gemm_scratch = reinterpret_cast<float*>(base + w.gemm_scratch);
+  s->prefix_scratch = reinterpret_cast<float*>(base + w.total);
   int* ints = reinterpret_cast<int*>(base + w.ints);
   const int B = dsc->n_seqs;
   DecodeState& st = s->st;
@@ -326,7 +357,7 @@ extern "C" int arcb_session_create(arcb_engine* e, const arcb_session_desc* dsc,
   s->n_state_ints = w.n_int;
   s->step_probe = reinterpret_cast<unsigned long long*>(ints + ((13 * (size_t)B + 9) & ~(size_t)1));
   // a caller that chooses kernels or splits gets the separate launches
-  if (dsc->attn_splits <= 0 && e->cfg.gemm_path == ARCB_GEMM_AUTO && e->cfg.attn_path == ARCB_ATTN_AUTO)
+  if (dsc->attn_splits <= 0 && dsc->prefix_group <= 1 && e->cfg.gemm_path == ARCB_GEMM_AUTO && e->cfg.attn_path == ARCB_ATTN_AUTO)
     s->step_cluster = arcb_step_cluster(B, e->cfg.d_model, e->cfg.d_ff, e->cfg.n_layers, dsc->t_max);
   cudaError_t r = cudaStreamCreateWithFlags(&s->capture_stream, cudaStreamNonBlocking);
   if (r != cudaSuccess) { delete s; return arcb_fail_cuda(r, "cudaStreamCreate"); }
@@ -422,7 +453,15 @@ static int run_layer(arcb_session* s, int l, int rows, const int* pos, const int
       plain_edges.on();
       CK(cudaEventRecordWithFlags(s->probe_begin, stream, cudaEventRecordExternal));
     }
-    CKL(arcb_launch_attn_stream(aa, stream), "attention");
+    if (!prefill && s->desc.prefix_group > 1) {
+      AttnPrefixArgs pa = prefix_args(e, B, T, s->desc.max_new, s->desc.prefix_group);
+      pa.q = s->q16; pa.q_pitch = d; pa.k = kbase; pa.v = vbase; pa.out = s->attn16;
+      pa.group_len = pa.item_begin = s->st.len0; pa.item_end = kv_count; pa.item_skip = skip;
+      pa.scratch = s->prefix_scratch; pa.status = e->d_err;
+      CKL(arcb_launch_attn_prefix(pa, stream), "attention over shared prompts");
+    } else {
+      CKL(arcb_launch_attn_stream(aa, stream), "attention");
+    }
     if (probe) { CK(cudaEventRecordWithFlags(s->probe_end, stream, cudaEventRecordExternal)); s->probe_recorded = true; }
   }
 
@@ -593,6 +632,47 @@ extern "C" int arcb_decode(arcb_session* s, int32_t n_steps, void* stream_v) {
   }
   for (int i = 0; i < n_steps; ++i) CK(cudaGraphLaunch(s->graph_exec, stream));
   arcb_count_launch(s->graph_kernels * n_steps);
+  return ARCB_OK;
+}
+
+extern "C" int arcb_session_fork(arcb_session* s, int32_t src, int32_t rows, const int32_t* h_dst, int32_t n_dst, void* stream_v) {
+  if (!s || (n_dst > 0 && !h_dst)) return arcb_fail(ARCB_E_ARG, "null argument");
+  const int B = s->desc.n_seqs, T = s->desc.t_max;
+  if (src < 0 || src >= B || n_dst < 0 || rows < 0 || rows > T) return arcb_fail(ARCB_E_ARG, "a fork names a sequence or rows outside the session");
+  cudaStream_t stream = (cudaStream_t)stream_v;
+  try {
+    std::vector<int32_t> copies;
+    for (int i = 0; i < n_dst; ++i) {
+      if (h_dst[i] < 0 || h_dst[i] >= B) return arcb_fail(ARCB_E_ARG, "a fork names a sequence outside the session");
+      if (h_dst[i] != src) copies.insert(copies.end(), {src, h_dst[i], 0, rows});
+    }
+    const int n = (int)copies.size() / 4;
+    if (!n || !rows) return ARCB_OK;
+    std::vector<CopyProgram> programs, whole;
+    std::vector<char> serial;
+    if (copy_plan(copies.data(), n, B, T, COPY_MAX_STEPS, programs, serial)) return arcb_fail(ARCB_E_ARG, "a fork names a sequence twice");
+    if (s->ls) {
+      whole = programs;           // the same sequences, for states that are one row
+      for (CopyProgram& p : whole) {
+        p.lo = 0;
+        p.hi = 1;
+        for (CopyStep& c : p.steps) c.end = c.op >= COPY_STORE ? 1 : c.end;
+      }
+      return lm_fork(s, programs, whole, serial, stream);
+    }
+    const arcb_config& c = s->eng->cfg;
+    CopyGeometry g{};
+    g.base = s->desc.d_kv_cache;
+    g.row_bytes = ARCB_HEAD_DIM * 2;
+    g.blocks = c.n_heads;
+    g.planes = 2 * c.n_layers;
+    g.block_stride = (long long)T * g.row_bytes;
+    g.seq_stride = g.block_stride * g.blocks;
+    g.plane_stride = g.seq_stride * B;
+    CKL(arcb_launch_cache_copy(g, programs, serial, stream), "fork");
+  } catch (const std::bad_alloc&) {
+    return arcb_fail(ARCB_E_STATE, "out of host memory");
+  }
   return ARCB_OK;
 }
 

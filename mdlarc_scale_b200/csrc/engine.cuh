@@ -7,6 +7,7 @@
 #include "../../include/arcb200.h"
 #include "common.cuh"
 #include "rowops.cuh"
+#include "cache_copy.cuh"
 #include "step_cluster.cuh"
 
 int arcb_fail(int code, const char* msg);
@@ -72,6 +73,7 @@ struct arcb_session {
   uint16_t* k16 = nullptr;  // K/V of one prefill call in the activation format
   uint16_t* v16 = nullptr;
   float* attn_scratch = nullptr;
+  float* prefix_scratch = nullptr; // parts of attention over shared prompts
   float* gemm_scratch = nullptr;   // split-K partials of the decode step's residual GEMMs
   int* example_ids = nullptr;
   bool use_examples = false;
@@ -118,3 +120,4 @@ int lm_prefill(arcb_session* s, const arcb_prefill_args* a, cudaStream_t stream)
 int lm_record_step(arcb_session* s, cudaStream_t stream);
 int* lm_n_finished(arcb_session* s);
 bool lm_armed(const arcb_session* s);
+int lm_fork(arcb_session* s, const std::vector<CopyProgram>& rows, const std::vector<CopyProgram>& whole, const std::vector<char>& serial, cudaStream_t stream);

@@ -1137,6 +1137,52 @@ int lm_prefill(arcb_session* s, const arcb_prefill_args* a, cudaStream_t stream)
   return ARCB_OK;
 }
 
+// Planes of equal geometry, a constant distance apart, are one launch.
+int lm_fork(arcb_session* s, const std::vector<CopyProgram>& rows, const std::vector<CopyProgram>& whole, const std::vector<char>& serial, cudaStream_t stream) {
+  const LayeredModel& m = *s->eng->lm;
+  LayeredSession* ls = s->ls;
+  const int T = s->desc.t_max;
+  std::vector<CopyGeometry> planes;
+  std::vector<char> state;
+  auto add = [&](void* base, int blocks, int n_rows, long long row_bytes, bool is_state) {
+    CopyGeometry g{};
+    g.base = base;
+    g.blocks = blocks;
+    g.row_bytes = (int)row_bytes;
+    g.block_stride = n_rows * row_bytes;
+    g.seq_stride = g.block_stride * blocks;
+    g.planes = 1;
+    for (size_t i = 0; i < planes.size(); ++i) {
+      CopyGeometry& o = planes[i];
+      const long long dist = reinterpret_cast<char*>(base) - reinterpret_cast<char*>(o.base);
+      if (state[i] == is_state && o.blocks == g.blocks && o.row_bytes == g.row_bytes && o.block_stride == g.block_stride && dist > 0 &&
+          (o.planes == 1 || dist == o.planes * o.plane_stride)) {
+        if (o.planes == 1) o.plane_stride = dist;
+        ++o.planes;
+        return;
+      }
+    }
+    planes.push_back(g);
+    state.push_back(is_state);
+  };
+  for (size_t l = 0; l < m.runs.size(); ++l) {
+    const LmLayer& y = m.layers[m.runs[l].layer];
+    if (y.d.mixer == ARCB_MIXER_LATENT) {
+      add(ls->k[l], y.panels(), T, 64 * m.es, false);
+    } else if (y.own_kv) {
+      add(ls->k[l], y.d.kv_heads, T, (long long)y.dimp * m.es, false);
+      add(ls->v[l], y.d.kv_heads, T, (long long)y.vdimp * m.es, false);
+    } else if (y.d.mixer == ARCB_MIXER_MLSTM) {
+      add(ls->S[l], y.d.heads, 1, (long long)y.d.dim * y.vdimp * 4, true);
+      add(ls->n[l], y.d.heads, 1, (long long)y.dimp * 4, true);
+      add(ls->m[l], 1, 1, (long long)y.d.heads * 4, true);
+    }
+  }
+  add(ls->st.cur_len, 1, 1, 4, true);      // where the next decode step continues
+  for (size_t i = 0; i < planes.size(); ++i) CKL(arcb_launch_cache_copy(planes[i], state[i] ? whole : rows, serial, stream), "fork");
+  return ARCB_OK;
+}
+
 int lm_record_step(arcb_session* s, cudaStream_t stream) {
   LayeredSession* ls = s->ls;
   const int B = s->desc.n_seqs;

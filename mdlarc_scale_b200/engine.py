@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import weakref
-from dataclasses import dataclass
+from dataclasses import dataclass, replace
 
 import numpy as np
 import torch
@@ -126,10 +126,10 @@ class EngineBase:
                     stop_on_end: bool = True, attn_splits: int = 0, forced: torch.Tensor | None = None,
                     want_step_logits: bool = False, out_tokens: torch.Tensor | None = None,
                     constraints: dict | None = None, temperature: float = 0.0, top_k: int = 0,
-                    sample_seed: int = 0, sample_stream=None, end_token: int | None = None) -> "Session":
+                    sample_seed: int = 0, sample_stream=None, end_token: int | None = None, prefix_group: int = 0) -> "Session":
         return self.session_class(self, n_seqs, t_max, max_new, max_prefill_tokens, stop_on_end, attn_splits,
                                   forced, want_step_logits, out_tokens, constraints, temperature, top_k,
-                                  sample_seed, sample_stream, self.end_token if end_token is None else end_token)
+                                  sample_seed, sample_stream, self.end_token if end_token is None else end_token, prefix_group)
 
 
 class Engine(EngineBase):
@@ -225,7 +225,7 @@ class Session:
 
     def __init__(self, eng: EngineBase, n_seqs, t_max, max_new, max_prefill_tokens, stop_on_end,
                  attn_splits, forced, want_step_logits, out_tokens=None, constraints=None,
-                 temperature=0.0, top_k=0, sample_seed=0, sample_stream=None, end_token=END_TOKEN_ID):
+                 temperature=0.0, top_k=0, sample_seed=0, sample_stream=None, end_token=END_TOKEN_ID, prefix_group=0):
         self.eng = eng
         self.n_seqs, self.t_max, self.max_new = int(n_seqs), cache_row_pitch(t_max), int(max_new)
         self.t_requested = int(t_max)
@@ -235,8 +235,12 @@ class Session:
         kv_bytes = lib.arcb_kv_cache_bytes(eng._handle, self.n_seqs, self.t_max)
         ws_bytes = lib.arcb_session_workspace_bytes(eng._handle, self.n_seqs, self.max_prefill_tokens,
                                                     int(attn_splits))
-        if kv_bytes <= 0 or ws_bytes <= 0:
+        # rows of the grid model in groups that share the first one's prompt (grid models; decode steps read it once)
+        self.prefix_group = int(prefix_group)
+        shared = lib.arcb_session_prefix_bytes(eng._handle, self.n_seqs, self.t_max, self.max_new, self.prefix_group) if self.prefix_group else 0
+        if kv_bytes <= 0 or ws_bytes <= 0 or shared < 0:
             raise ValueError("bad session sizes")
+        ws_bytes += shared
         # torch owns the memory; the library only borrows the pointers
         self.kv_cache = torch.empty(kv_bytes, dtype=torch.uint8, device=dev)
         self.workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
@@ -287,7 +291,7 @@ class Session:
             d_palette_mask=_ptr(self.palette_mask), d_target_shape=_ptr(self.target_shape),
             palette_penalty=pal_pen, shape_penalty=shp_pen, disallow_token_mask=disallow,
             temperature=float(temperature), top_k=int(top_k or 0), sample_seed=int(sample_seed) & (2 ** 64 - 1),
-            d_sample_stream=_ptr(self.sample_stream), end_token=int(end_token))
+            d_sample_stream=_ptr(self.sample_stream), end_token=int(end_token), prefix_group=self.prefix_group)
         self._handle = C.c_void_p()
         with torch.cuda.device(dev):
             _lib.check(lib.arcb_session_create(eng._handle, C.byref(desc), C.byref(self._handle)))
@@ -323,6 +327,12 @@ class Session:
             d_grid_in_output=_ptr(plan.grid_in_output), d_first_logits=_ptr(first_logits))
         with torch.cuda.device(self.eng.device):
             _lib.check(self.eng.lib.arcb_prefill(self._handle, C.byref(a), _stream_ptr(self.eng.device)))
+
+    def copy_rows(self, src: int, rows: int, targets) -> None:
+        """What sequence ``src`` holds at its first ``rows`` positions, for the sequences ``targets`` as well."""
+        dst = np.ascontiguousarray(targets, dtype=np.int32).reshape(-1)
+        with torch.cuda.device(self.eng.device):
+            _lib.check(self.eng.lib.arcb_session_fork(self._handle, int(src), int(rows), dst.ctypes.data, len(dst), _stream_ptr(self.eng.device)))
 
     def decode(self, n_steps: int) -> None:
         with torch.cuda.device(self.eng.device):
@@ -371,6 +381,15 @@ class PrefillPlan:
     grid_y: torch.Tensor | None = None
     grid_in_output: torch.Tensor | None = None
     kv_row_identity: bool = False   # kv_row[i] == i for i < n_kv_rows and < 0 after
+
+    def for_samples(self, n: int) -> "PrefillPlan":
+        """The same prompts for groups of ``n`` rows that share them: prompt i in cache row i n, read once, and its first token
+        picked for rows i n ... i n + n - 1."""
+        def rep(t):
+            return t.repeat_interleave(n)
+        rows = rep(self.first_seq) * n + torch.arange(n, dtype=torch.int32, device=self.first_seq.device).repeat(self.n_first)
+        return replace(self, seq=self.seq * n, n_first=self.n_first * n, first_row=rep(self.first_row), first_seq=rows, prompt_len=rep(self.prompt_len),
+                       grid_x=rep(self.grid_x), grid_y=rep(self.grid_y), grid_in_output=rep(self.grid_in_output))
 
     def to(self, device) -> "PrefillPlan":
         def mv(t):

@@ -32,6 +32,7 @@ class Request:
     produced: int = 0            # tokens picked so far (host count; an upper bound once the end token is out)
     output: list[int] = field(default_factory=list)
     tokens: np.ndarray | None = field(default=None, compare=False)     # the prompt as one array, from submit()
+    others: list["Request"] = field(default_factory=list, compare=False)   # of the same prompt, forked from this one's sequence
 
 
 def _token_array(prompt) -> np.ndarray:
@@ -50,7 +51,7 @@ class Scheduler:
     def __init__(self, engine: EngineBase, max_new: int, t_max: int, n_slots: int, prefill_tokens: int = DEFAULT_PREFILL_TOKENS,
                  end_token: int | None = None, temperature: float = 0.0, top_k: int | None = None, seed: int = 0,
                  want_logits: bool = False):
-        self.engine, self.max_new = engine, int(max_new)
+        self.engine, self.max_new, self.n_slots = engine, int(max_new), int(n_slots)
         self.end_token = -1 if end_token is None else int(end_token)
         self.session = engine.new_session(
             n_slots, t_max, self.max_new, min(prefill_tokens, n_slots * t_max), stop_on_end=True,
@@ -74,25 +75,46 @@ class Scheduler:
         request.tokens = tokens.astype(np.int64)
         self.waiting.append(request)
 
+    def submit_samples(self, requests: list[Request]) -> None:
+        """Requests for one prompt: it is prefilled once, and the others' sequences are forked from the first one's.  They are admitted
+        together, so there may be no more of them than slots."""
+        if len(requests) > self.n_slots:
+            raise ValueError("more samples of a prompt than the session has slots")
+        self.submit(requests[0])
+        for r in requests[1:]:
+            r.tokens = requests[0].tokens
+        requests[0].others = list(requests[1:])
+
     # The device state of all admitted requests is set, and the results of all ended ones are read, together: with a few
     # launches and copies for each (35 to 90 us) the GPU waited 10 of 68 ms for the host at 150 requests.
     def _admit(self) -> None:
         admitted = []
-        while self.waiting and self.session.free_slots:
+        while self.waiting and self.session.free_slots > len(self.waiting[0].others):
             r = self.waiting.popleft()
-            r.slot = self.session.acquire()
-            admitted.append(r)
+            for x in (r, *r.others):
+                x.slot = self.session.acquire()
+                admitted.append(x)
         if not admitted:
             return
-        self.filling += admitted
+        forked = {id(x) for r in admitted for x in r.others}
+        self.filling += [r for r in admitted if id(r) not in forked]
         at = torch.tensor([[r.slot for r in admitted], [r.rid & 0x7FFFFFFF for r in admitted]]).to(self.engine.device, non_blocking=True)
         self.session.out_tokens.index_fill_(0, at[0], -1)
         self.session.sample_stream.index_copy_(0, at[0], at[1].to(torch.int32))
 
     def _prefill(self) -> None:
         room, call, armed = self.session.max_prefill_tokens, [], []
+        for r in list(self.filling):
+            if r.others and r.fed == len(r.tokens) - 1:
+                # all but the last token are there: the others take them over, and every one feeds the last token itself
+                if r.fed:
+                    self.session.fork(r.slot, [x.slot for x in r.others])
+                for x in r.others:
+                    x.fed = r.fed
+                self.filling += r.others
+                r.others = []
         for r in self.filling:
-            n = min(room, len(r.tokens) - r.fed)
+            n = min(room, len(r.tokens) - bool(r.others) - r.fed)
             if n <= 0:
                 break
             last = r.fed + n == len(r.tokens)
@@ -163,17 +185,26 @@ class Scheduler:
 
 def generate(engine: EngineBase, prompts, max_new: int, end_token: int | None = None, temperature: float = 0.0,
              top_k: int | None = None, seed: int = 0, max_batch: int = 256,
-             prefill_tokens: int = DEFAULT_PREFILL_TOKENS, return_logits: bool = False):
+             prefill_tokens: int = DEFAULT_PREFILL_TOKENS, return_logits: bool = False, samples: int = 1):
     """Continuations of token-id prompts: one list of generated ids per prompt, the end token (if any) included.
-    Greedy unless ``temperature > 0``; a request's random stream depends on ``seed`` and its index only."""
+    Greedy unless ``temperature > 0``; a request's random stream depends on ``seed`` and its index only.
+
+    ``samples`` > 1: that many continuations of every prompt, one after the other in the list (and in the indices of random
+    streams and logits): continuation j of prompt i is number ``i samples + j``.  A prompt is prefilled once, and what its sequence
+    holds is copied to the others' slots; with more samples than ``max_batch`` it is prefilled once for every ``max_batch`` of them."""
+    if samples < 1:
+        raise ValueError("samples must be at least 1")
     if max_new <= 0 or not prompts:
-        return ([[] for _ in prompts], {}) if return_logits else [[] for _ in prompts]
+        none = [[] for _ in range(len(prompts) * samples)]
+        return (none, {}) if return_logits else none
     t_max = max(len(p) for p in prompts) + max_new
-    sched = Scheduler(engine, max_new, t_max, min(len(prompts), max_batch), prefill_tokens, end_token, temperature,
+    sched = Scheduler(engine, max_new, t_max, min(len(prompts) * samples, max_batch), prefill_tokens, end_token, temperature,
                       top_k, seed, return_logits)
     try:
         for i, p in enumerate(prompts):
-            sched.submit(Request(i, p if isinstance(p, list) else [int(t) for t in p]))
+            p = p if isinstance(p, list) else [int(t) for t in p]
+            for j in range(0, samples, max_batch):
+                sched.submit_samples([Request(i * samples + k, p) for k in range(j, min(j + max_batch, samples))])
         out = [r.output for r in sched.run()]
         return (out, sched.step_logits) if return_logits else out
     finally:
@@ -191,12 +222,14 @@ def main(argv=None) -> int:
     ap.add_argument("--top-k", type=int, default=None)
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--max-batch", type=int, default=256)
+    ap.add_argument("--samples", type=int, default=1, help="continuations of every prompt, one a line")
     args = ap.parse_args(argv)
     from .registry import load_model
     engine = load_model(args.model, "cuda:0", args.dtype)
     src = sys.stdin if args.prompts == "-" else open(args.prompts)
     prompts = [json.loads(line) for line in src if line.strip()]
-    for row in generate(engine, prompts, args.max_new, args.end_token, args.temperature, args.top_k, args.seed, args.max_batch):
+    for row in generate(engine, prompts, args.max_new, args.end_token, args.temperature, args.top_k, args.seed, args.max_batch,
+                        samples=args.samples):
         print(json.dumps(row))
     return 0
 

@@ -97,7 +97,7 @@ def generate_tokens(engine: Engine, ids: np.ndarray, pos: np.ndarray, mask: np.n
                     max_prefill_tokens: int = DEFAULT_PREFILL_TOKENS, attn_splits: int = 0,
                     session: Session | None = None, pinned: bool = False,
                     constraints: dict | None = None, temperature: float = 0.0, top_k: int | None = None,
-                    sample_seed: int = 0, freeze_finished: bool = True) -> GenerationTrace:
+                    sample_seed: int = 0, freeze_finished: bool = True, samples: int = 1) -> GenerationTrace:
     """Prefill + greedy decode of a padded batch given as host arrays; returns device tokens.
 
     ``ids`` int [B, S], ``pos`` int [B, S, 3], ``mask`` bool [B, S] (True = real token).  At most
@@ -106,15 +106,23 @@ def generate_tokens(engine: Engine, ids: np.ndarray, pos: np.ndarray, mask: np.n
     that has emitted END is frozen (it emits END from then on and its attention is skipped) unless
     ``freeze_finished`` is False, in which case it keeps decoding until every row has emitted END,
     which is what the reference does.
+
+    ``samples`` > 1: that many rows for every prompt, row ``i samples + j`` the j-th of prompt i (``example_ids`` go by prompt,
+    ``forced`` and ``constraints`` by row).  A prompt is prefilled once, and the decode steps read its keys and values once for all
+    of its rows.
     """
     dev = engine.device
-    B, S = ids.shape
+    P, S = ids.shape
+    samples = int(samples)
+    if samples < 1:
+        raise ValueError("samples must be at least 1")
+    B = P * samples
     lens = mask.sum(axis=1)
     # the plans of the prefill calls are made on the device, unless most of what would have to cross is padding
-    plain = pos.shape == (B, S, 3) and mask.shape == (B, S)
-    batch = PaddedBatch(ids, pos, mask, dev) if plain and 0 < B * S <= 4 * int(lens.sum()) else None
+    plain = pos.shape == (P, S, 3) and mask.shape == (P, S)
+    batch = PaddedBatch(ids, pos, mask, dev) if plain and 0 < P * S <= 4 * int(lens.sum()) else None
     t_max = int(lens.max()) + int(max_new)
-    cap = int(min(max_prefill_tokens, int(lens.sum()) + 2 * B))
+    cap = int(min(max_prefill_tokens, int(lens.sum()) + 2 * P))
     cap = max(cap, int(lens.max()) + 2, B)
     if session is None:
         session = engine.new_session(
@@ -122,11 +130,13 @@ def generate_tokens(engine: Engine, ids: np.ndarray, pos: np.ndarray, mask: np.n
             attn_splits=attn_splits,
             forced=None if forced is None else torch.from_numpy(np.ascontiguousarray(forced, dtype=np.int32)),
             want_step_logits=want_logits, constraints=constraints, temperature=temperature,
-            top_k=top_k or 0, sample_seed=sample_seed)
+            top_k=top_k or 0, sample_seed=sample_seed, prefix_group=samples if samples > 1 else 0)
+    elif session.prefix_group != (samples if samples > 1 else 0):
+        raise ValueError("the session was made for another number of samples")
     ex_dev = None
     h2d = 0
     if example_ids is not None and engine.use_example_embedding:
-        ex_host = torch.from_numpy(np.ascontiguousarray(example_ids, dtype=np.int32))
+        ex_host = torch.from_numpy(np.ascontiguousarray(np.repeat(example_ids, samples), dtype=np.int32))
         if pinned:
             ex_host = ex_host.pin_memory()
         ex_dev = ex_host.to(dev, non_blocking=True)
@@ -141,7 +151,9 @@ def generate_tokens(engine: Engine, ids: np.ndarray, pos: np.ndarray, mask: np.n
             h2d += plan.h2d_bytes()
             plan = plan.to(dev)
         n_prefill += plan.n_tokens
-        fl = None if first_logits is None else first_logits[int(rows[0]):int(rows[-1]) + 1]     # consecutive rows
+        if samples > 1:
+            plan = plan.for_samples(samples)
+        fl = None if first_logits is None else first_logits[int(rows[0]) * samples:(int(rows[-1]) + 1) * samples]     # consecutive rows
         session.prefill(plan, ex_dev, first_logits=fl)
     if batch is not None:
         h2d += batch.h2d_bytes
@@ -370,7 +382,7 @@ def predict_with_augmentations(model, task: dict, test_idx: int, device, example
                                constrain_decoding: bool = False, palette_penalty: float = 2.0,
                                shape_penalty: float = 2.0, batched: bool = True, use_compile: bool = False,
                                max_batch_size: int = 16, merge_chunks: bool = True,
-                               freeze_finished: bool = True):
+                               freeze_finished: bool = True, share_prompts: bool = False):
     """Candidates under all augmentations for AAIVR voting (``src/inference.py:697-920``).
 
     Returns ``[(grid | None, dihedral_idx, colour_perm | None), ...]`` in the reference's order.
@@ -384,15 +396,22 @@ def predict_with_augmentations(model, task: dict, test_idx: int, device, example
     that later emits another IO_SEP yields a different candidate there.  For exactly the reference's
     candidates pass ``freeze_finished=False`` together with ``merge_chunks=False`` (one call per chunk,
     each stopping when its own 16 rows have finished).
+
+    ``share_prompts`` prefills the prompt of a variant once for its ``num_samples`` rows, whose steps read its keys and values
+    once (``generate_tokens(samples=...)``).  The rows then run unpadded in one session, as those of ``batched=False`` do; where
+    ``max_seq_len`` would cut some shorter than others they are not shared.
     """
     device = torch.device(device)
     engine = _resolve_engine(model, device)
+    share_prompts = share_prompts and num_samples > 1
     prompts, positions, info = build_augmented_prompts(task, test_idx, use_train_examples,
                                                        num_color_perms, num_samples)
     palettes = shapes = None
     if constrain_decoding:
         palettes, shapes = augmented_constraints(task, test_idx, info)
-    if not batched:
+    if share_prompts and max((len(p) for p in prompts), default=0) + max_output_tokens > engine.max_seq_len:
+        share_prompts = False
+    if not batched or share_prompts:
         # The reference's sequential path runs every variant alone and unpadded
         # (src/inference.py:923-1003).  A right-padded batch gives each row exactly that (its keys,
         # its last token), so all variants share one session unless max_seq_len would cut some
@@ -400,16 +419,17 @@ def predict_with_augmentations(model, task: dict, test_idx: int, device, example
         lens = [len(p) for p in prompts]
         out = []
         if lens and max(lens) + max_output_tokens <= engine.max_seq_len:
-            ids, pos, mask = pad_prompts(prompts, positions, left=False)
             n = len(prompts)
+            per = num_samples if share_prompts else 1
+            ids, pos, mask = pad_prompts(prompts[::per], positions[::per], left=False)
             cons = None
             if constrain_decoding:
                 cons = _constraints_dict(chunk_constraints(palettes, shapes, palette_penalty, shape_penalty), n)
             seed = int(torch.randint(0, 2 ** 62, (1,)).item()) if sample_temperature > 0 else 0
-            trace = generate_tokens(engine, ids, pos, mask, np.full(n, example_id, dtype=np.int64),
+            trace = generate_tokens(engine, ids, pos, mask, np.full(len(ids), example_id, dtype=np.int64),
                                     max_output_tokens, stop_on_end=True, constraints=cons,
                                     temperature=float(sample_temperature), top_k=sample_top_k, sample_seed=seed,
-                                    freeze_finished=freeze_finished)
+                                    freeze_finished=freeze_finished, samples=per)
             gen = trace.tokens.cpu().tolist()
             for i, (d_idx, tag) in enumerate(info):
                 out.append((_grid_after_last_sep([int(t) for t in prompts[i]] + gen[i]), d_idx, tag))

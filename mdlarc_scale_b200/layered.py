@@ -254,6 +254,20 @@ class LayeredSession(Session):
         self.lens[slot] = 0
         self._free.append(slot)
 
+    def fork(self, slot: int, targets: list[int]) -> None:
+        """The sequences in ``targets`` (slots of the caller's) hold what the one in ``slot`` does, and continue from there."""
+        targets = [int(t) for t in targets]
+        for t in [slot, *targets]:
+            if t < 0 or t >= self.n_seqs:
+                raise ValueError(f"slot {t} outside the session")
+            if t in self._free:
+                raise ValueError(f"slot {t} is not in use")
+        if len(set(targets)) != len(targets) or slot in targets:
+            raise ValueError("a sequence may appear once in a fork")
+        self.copy_rows(slot, self.lens[slot], targets)
+        for t in targets:
+            self.lens[t] = self.lens[slot]
+
     @property
     def free_slots(self) -> int:
         return len(self._free)
