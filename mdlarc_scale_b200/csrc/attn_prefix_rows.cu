@@ -38,9 +38,9 @@ struct ArCfg {
   static constexpr int PLANE = KEYS * D * 2;
   static constexpr int STAGE = 2 * PLANE;
   static constexpr int Q_BYTES = 8 * D * 2;
-  static constexpr int WARP = STAGES * STAGE + Q_BYTES;    // a multiple of 1 KB: the swizzle goes by the address
-  static_assert(WARP % 1024 == 0 && STAGE % 1024 == 0, "swizzled boxes");
-  static constexpr int SMEM = AR_WARPS * (WARP + 8 * STAGES);      // no room to align: without static shared memory it starts aligned
+  static constexpr int WARP = STAGES * STAGE + Q_BYTES;
+  static_assert(WARP % 128 == 0 && BOX % 128 == 0, "an exclusive-or of an address is one of its piece of 128 bytes");
+  static constexpr int SMEM = AR_WARPS * WARP;
   static_assert(CTAS * (SMEM + 1024) <= 228 * 1024, "CTAs of an SM");
 };
 
@@ -48,18 +48,17 @@ struct ArCfg {
 template <int D>
 struct ArWarp {
   using C = ArCfg<D>;
+  static constexpr int CH = D / 8;         // 16-byte pieces of a row
   const AttnPrefixArgs& a;
-  const CUtensorMap* maps[2];
   long long first, stride, n_units;        // this warp's units
   int n, lane;
-  uint32_t ring, q_slot, bars;
+  uint32_t ring, q_slot, to;               // `to`: where a lane's first piece of a tile goes
   ApWork batch;
   int batch_of;
-  ApWork ahead;                            // the unit that tiles are asked for of, its number, its tiles that have not been, and
-  int ahead_i, ahead_left, ahead_row;      // the next one's first row in the cache
+  ApWork ahead;                            // the unit that tiles are asked for of, its number, its tiles that have not been,
+  int ahead_i, ahead_left, rows_left;      // the rows from the next one on, and where they are
+  const char* from[2];
   int flight, put, get;                    // tiles asked for and not used up
-  uint32_t phase;                          // of the slot that is used next
-  bool ok;
 
   __device__ __forceinline__ ApWork unit(int i) {
     if (i >> 5 != batch_of) {
@@ -89,31 +88,45 @@ struct ArWarp {
   __device__ __forceinline__ void look_at(const ApWork& w) {
     ahead = w;
     ahead_left = tiles_of(w);
-    ahead_row = (w.seq * a.n_kv + w.kvh) * a.t_max + w.begin;
+    rows_left = w.end - w.begin;
+    const size_t at = (((size_t)w.seq * a.n_kv + w.kvh) * (size_t)a.t_max + w.begin + lane / CH) * (D * 2) + (lane % CH) * 16;
+    from[0] = reinterpret_cast<const char*>(a.k) + at;
+    from[1] = reinterpret_cast<const char*>(a.v) + at;
   }
-  // the next tile into slot `put`, with the unit's queries when it is the first
+  // the next tile into slot `put`, with the unit's queries when it is the first; rows behind the end become zeros
   __device__ __forceinline__ void issue() {
-    const uint32_t bar = bars + 8 * put, st = ring + put * C::STAGE;
-    const bool first_tile = ahead_left == tiles_of(ahead);
-    uint32_t bytes = C::STAGE;
-    if (first_tile) {
-      bytes += ahead.rows * D * 2;
-      if (lane < ahead.rows)
-        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(q_slot + lane * D * 2),
-                     "l"(query(ahead, lane)), "r"(D * 2), "r"(bar) : "memory");
-    }
-    if (lane == 0) {
-      mbar_expect_tx(bar, bytes);
+    constexpr int STEP = 32 / CH;          // rows of a pass; a lane has one 16-byte piece of each
+    const uint32_t st = ring + put * C::STAGE + to;
+    if (rows_left >= C::KEYS) {
 #pragma unroll
       for (int plane = 0; plane < 2; ++plane)
 #pragma unroll
-        for (int c = 0; c < D / 64; ++c) tma_load_2d(st + plane * C::PLANE + c * C::BOX, maps[plane], c * 64, ahead_row, bar);
+        for (int i = 0; i < C::KEYS / STEP; ++i)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((st ^ piece(i)) + plane * C::PLANE + i * STEP * 128), "l"(from[plane] + i * STEP * (D * 2)) : "memory");
+    } else {
+#pragma unroll
+      for (int plane = 0; plane < 2; ++plane)
+#pragma unroll
+        for (int i = 0; i < C::KEYS / STEP; ++i) {
+          const bool ok = lane / CH + i * STEP < rows_left;
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((st ^ piece(i)) + plane * C::PLANE + i * STEP * 128),
+                       "l"(ok ? from[plane] + i * STEP * (D * 2) : reinterpret_cast<const char*>(a.k)), "r"(ok ? 16 : 0) : "memory");
+        }
     }
-    ahead_row += C::KEYS;
+    if (ahead_left == tiles_of(ahead)) {
+      for (int r = lane / CH; r < ahead.rows; r += STEP)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(q_slot + r * (D * 2) + (lane % CH) * 16), "l"(query(ahead, r) + (lane % CH) * 16) : "memory");
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    from[0] += C::KEYS * D * 2;
+    from[1] += C::KEYS * D * 2;
+    rows_left -= C::KEYS;
     --ahead_left;
     put = put + 1 == C::STAGES ? 0 : put + 1;
     ++flight;
   }
+  // the swizzle of row lane / CH + i STEP beside that of row lane / CH
+  static __device__ __forceinline__ uint32_t piece(int i) { return ((i * (32 / CH)) & 7) << 4; }
   // Asks for tiles while there is room, up to the end of the unit behind unit i; into that (cross) only when the queries of
   // unit i have left their slot.
   __device__ __forceinline__ void ask(int i, bool cross) {
@@ -161,11 +174,11 @@ __device__ __forceinline__ void ar_unit(ArWarp<D>& s, const ApWork& w, int i) {
   for (int t = 0; t < tiles; ++t) {
     __syncwarp();                          // everybody is done with the tile before, whose slot is asked for now
     s.ask(i, t > 0);
-    if (!__all_sync(0xffffffffu, mbar_wait_bounded(s.bars + 8 * s.get, s.phase))) {
-      arcb_set_error(a.status, ARCB_DEV_WAIT_TIMEOUT_TMA);
-      s.ok = false;
-      return;
-    }
+    if (s.flight == 1) asm volatile("cp.async.wait_group 0;" ::: "memory");
+    else if (s.flight == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    else asm volatile("cp.async.wait_group 2;" ::: "memory");
+    static_assert(C::STAGES <= 3, "waits for one to three tiles under way");
+    __syncwarp();
     if (t == 0) {
       const int r = min(lane & (PAIR ? 3 : 7), w.rows - 1);      // rows that do not exist are as the last one
 #pragma unroll
@@ -182,7 +195,6 @@ __device__ __forceinline__ void ar_unit(ArWarp<D>& s, const ApWork& w, int i) {
     }
     const uint32_t slot = s.ring + s.get * C::STAGE, kst = slot + k_at, vst = slot + C::PLANE + v_at;
     s.get = s.get + 1 == C::STAGES ? 0 : s.get + 1;
-    s.phase ^= s.get == 0;
     --s.flight;
     const int left = w.end - w.begin - t * C::KEYS;        // keys of the tile
     const bool some = left < C::KEYS;
@@ -206,13 +218,6 @@ __device__ __forceinline__ void ar_unit(ArWarp<D>& s, const ApWork& w, int i) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           if (mt * 16 + (lane >> 2) + (j >> 1) * 8 >= left) p[mt][j] = -INFINITY;
-      // values behind the end: a weight of 0 does not hide a NaN
-      for (int e = left * 8 + lane; e < C::KEYS * 8; e += 32)
-#pragma unroll
-        for (int c = 0; c < D / 64; ++c)
-          asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(slot + C::PLANE + c * C::BOX + e * 16), "r"(0u) : "memory");
-      fence_proxy_async_smem();            // the slot's next tile comes by the other proxy
-      __syncwarp();
     }
     // the lanes' own maxima tell whether any reference has to be raised; only then are they exchanged
     float top[2];
@@ -299,36 +304,27 @@ __device__ __forceinline__ void ar_unit(ArWarp<D>& s, const ApWork& w, int i) {
 
 template <int D, bool HALF, bool QS>
 __global__ void __launch_bounds__(AR_WARPS * 32, ArCfg<D>::CTAS)
-attn_prefix_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, AttnPrefixArgs a, long long n_units) {
+attn_prefix_rows_kernel(AttnPrefixArgs a, long long n_units) {
   using C = ArCfg<D>;
   pdl_launch_dependents();
   if (!a.beside) pdl_wait();
-  extern __shared__ __align__(1024) uint8_t ar_smem[];
+  extern __shared__ __align__(128) uint8_t ar_smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const long long stride = (long long)gridDim.x * AR_WARPS, first = (long long)warp * gridDim.x + blockIdx.x;
   if (first >= n_units) {
     if (a.beside) pdl_wait();
     return;
   }
-  const uint32_t base = smem_u32(ar_smem), ring = base + warp * C::WARP, bars = base + AR_WARPS * C::WARP + warp * (8 * C::STAGES);
-  if (base & 1023u) {
-    arcb_set_error(a.status, ARCB_DEV_BAD_INDEX);
-    if (a.beside) pdl_wait();
-    return;
-  }
-  if (lane == 0) {
-    for (int i = 0; i < C::STAGES; ++i) mbar_init(bars + 8 * i, 1);
-    mbar_fence_init();
-  }
-  __syncwarp();
-  ArWarp<D> s{a, {&tmap_k, &tmap_v}, first, stride, n_units, (int)((n_units - first + stride - 1) / stride), lane, ring, ring + C::STAGES * C::STAGE, bars};
+  const uint32_t base = smem_u32(ar_smem), ring = base + warp * C::WARP;
+  constexpr int CH = D / 8;
+  const int row = lane / CH, col = lane % CH;
+  ArWarp<D> s{a, first, stride, n_units, (int)((n_units - first + stride - 1) / stride), lane, ring, ring + C::STAGES * C::STAGE,
+              (uint32_t)((col >> 3) * C::BOX + row * 128 + (((col & 7) ^ (row & 7)) << 4))};
   s.batch_of = -1;
   s.flight = s.put = s.get = s.ahead_i = 0;
-  s.phase = 0;
-  s.ok = true;
   ApWork w = s.unit(0);
   s.look_at(w);
-  for (int i = 0; i < s.n && s.ok; ++i) {
+  for (int i = 0; i < s.n; ++i) {
     if (w.rows <= 4) ar_unit<D, HALF, QS, true>(s, w, i);
     else ar_unit<D, HALF, QS, false>(s, w, i);
     if (i + 1 < s.n) {
@@ -345,15 +341,10 @@ int ar_launch(const AttnPrefixArgs& a, long long units, cudaStream_t stream) {
   static std::atomic<unsigned long long> done{0};
   const cudaError_t e = arcb_opt_in_smem(attn_prefix_rows_kernel<D, HALF, QS>, C::SMEM, done);
   if (e != cudaSuccess) return (int)e;
-  CUtensorMap tk, tv;
-  const uint64_t rows = (uint64_t)a.n_seqs * a.n_kv * a.t_max;
-  int r = arcb_make_tmap_2d_16b(&tk, a.k, rows, D, C::KEYS, 64, HALF);
-  if (!r) r = arcb_make_tmap_2d_16b(&tv, a.v, rows, D, C::KEYS, 64, HALF);
-  if (r) return 1000 + r;
   const long long most = (long long)C::CTAS * arcb_num_sms();
   const dim3 grid((unsigned)(units < most ? units : most));
-  return (int)(a.beside ? ap_launch_beside(attn_prefix_rows_kernel<D, HALF, QS>, grid, dim3(AR_WARPS * 32), C::SMEM, stream, tk, tv, a, units)
-                        : arcb_launch(attn_prefix_rows_kernel<D, HALF, QS>, grid, dim3(AR_WARPS * 32), C::SMEM, stream, tk, tv, a, units));
+  return (int)(a.beside ? ap_launch_beside(attn_prefix_rows_kernel<D, HALF, QS>, grid, dim3(AR_WARPS * 32), C::SMEM, stream, a, units)
+                        : arcb_launch(attn_prefix_rows_kernel<D, HALF, QS>, grid, dim3(AR_WARPS * 32), C::SMEM, stream, a, units));
 }
 }  // namespace
 
