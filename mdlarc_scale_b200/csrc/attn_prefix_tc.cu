@@ -51,7 +51,12 @@ attn_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
   using C = AtCfg<D, QS>;
   pdl_launch_dependents();
   pdl_wait();
-  const ApWork w = ap_work(a, a.first_block + blockIdx.x, threadIdx.x == 0);
+  ApWork w = ap_work(a, a.first_block + blockIdx.x, threadIdx.x == 0);
+  // Read from memory, these would be a thread's own to the compiler, and every operand of a product that depends on them a move to
+  // a uniform register.
+  w.rows = __shfl_sync(0xffffffffu, w.rows, 0);
+  w.begin = __shfl_sync(0xffffffffu, w.begin, 0);
+  w.end = __shfl_sync(0xffffffffu, w.end, 0);
   if (w.rows <= 0) return;
   extern __shared__ __align__(1024) uint8_t at_smem[];
   const uint32_t raw = smem_u32(at_smem);
@@ -191,38 +196,40 @@ attn_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
       };
       const uint32_t t_s = tmem_base + x * 128, t_o = tmem_base + 256 + x * D, q_tile = q_smem + (wide ? x * C::Q_BYTES : 0);
       auto tile = [&](int i) { return wide ? i : 2 * i + x; };
+      // The values of a tile and the scores of the next one are issued together, and all that either waits for is waited for ahead:
+      // a wait between them lasted until the values were through (970 of 5450 cycles a tile).
       for (int i = 0; ok && i <= n_x; ++i) {
+        const int j = tile(i), s = j % C::STAGES, j1 = tile(i - 1), s1 = j1 % C::STAGES;
+        if (i < n_x) wait(b_kfull + 8 * s, (j / C::STAGES) & 1, ARCB_DEV_WAIT_TIMEOUT_TMA);
         if (i > 0) {
-          const int j = tile(i - 1), s = j % C::STAGES;
+          wait(b_vfull + 8 * s1, (j1 / C::STAGES) & 1, ARCB_DEV_WAIT_TIMEOUT_TMA);
+          if (j1 == n_tiles - 1 && left < AT_KEYS) wait(b_clean, 0, ARCB_DEV_WAIT_TIMEOUT_TMA);
           wait(b_p + 8 * x, (i - 1) & 1, ARCB_DEV_WAIT_TIMEOUT_ACC);
-          wait(b_vfull + 8 * s, (j / C::STAGES) & 1, ARCB_DEV_WAIT_TIMEOUT_TMA);
-          if (j == n_tiles - 1 && left < AT_KEYS) wait(b_clean, 0, ARCB_DEV_WAIT_TIMEOUT_TMA);
-          if (!ok) break;
-          tc_fence_after();
-          const uint64_t dv = umma_desc_mn_sw128(v_smem + s * C::KV_BYTES, AT_BOX);
+        }
+        if (!ok) break;
+        tc_fence_after();
+        if (i > 0) {
+          const uint64_t dv = umma_desc_mn_sw128(v_smem + s1 * C::KV_BYTES, AT_BOX);
 #pragma unroll
           for (int piece = 0; piece < WP; ++piece)
 #pragma unroll
             for (int ks = 0; ks < AT_KEYS / 16; ++ks)
               umma_f16_ts_if(el, t_o, t_s + piece * 64 + ks * 8, dv + (uint64_t)(ks * (2048 >> 4)), idesc_pv, (i > 1 || piece || ks) ? 1u : 0u);
-          umma_commit_if(el, b_vempty + 8 * s);
         }
-        if (i == n_x) break;
-        const int j = tile(i), s = j % C::STAGES;
-        wait(b_kfull + 8 * s, (j / C::STAGES) & 1, ARCB_DEV_WAIT_TIMEOUT_TMA);
-        if (!ok) break;
-        tc_fence_after();
+        if (i < n_x) {
 #pragma unroll
-        for (int piece = 0; piece < (QS ? 2 : 1); ++piece)
+          for (int piece = 0; piece < (QS ? 2 : 1); ++piece)
 #pragma unroll
-          for (int c = 0; c < C::BOXES; ++c) {
-            const uint64_t dq = umma_desc_k_sw128(q_tile + piece * C::Q_PIECE + c * AT_BOX);
-            const uint64_t dk = umma_desc_k_sw128(k_smem + s * C::KV_BYTES + c * AT_BOX);
+            for (int c = 0; c < C::BOXES; ++c) {
+              const uint64_t dq = umma_desc_k_sw128(q_tile + piece * C::Q_PIECE + c * AT_BOX);
+              const uint64_t dk = umma_desc_k_sw128(k_smem + s * C::KV_BYTES + c * AT_BOX);
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks) umma_f16_if(el, t_s, dq + 2 * ks, dk + 2 * ks, idesc_qk, (piece | c | ks) ? 1u : 0u);
-          }
-        umma_commit_if(el, b_s + 8 * x);
-        umma_commit_if(el, b_kempty + 8 * s);
+              for (int ks = 0; ks < 4; ++ks) umma_f16_if(el, t_s, dq + 2 * ks, dk + 2 * ks, idesc_qk, (piece | c | ks) ? 1u : 0u);
+            }
+          umma_commit_if(el, b_s + 8 * x);
+          umma_commit_if(el, b_kempty + 8 * s);
+        }
+        if (i > 0) umma_commit_if(el, b_vempty + 8 * s1);
       }
       if (ok && n_x > 0) umma_commit_if(el, b_o + 8 * x);
     }
