@@ -5,7 +5,7 @@
 // chains (scores, softmax, weights, values) of which one is in the tensor core while the other is at its exponentials.
 //   warp 0        TMA: key and value tiles as 128 x 64 boxes with the 128-byte swizzle, rings shared by A and B; value rows
 //                 behind the end of the last tile are set to zero: a weight of 0 does not hide a NaN
-//   warps 1, 2    products of A and of B: S = Q K^T (128 TMEM columns), O += P V with P read from TMEM
+//   warp 1        products of A and of B in turn: O += P V with P read from TMEM, then the next S = Q K^T (128 TMEM columns)
 //   warps 4-11    a thread a query row: maxima, exponentials, row sums, P over the row's own score columns.  (Two threads a row
 //                 had to exchange maxima in every tile and took twice the instructions.)
 // Maxima, sums and results are fp32.  The reference maximum of a row is raised only when it grows by 2^8.  Half queries over a
@@ -184,8 +184,9 @@ attn_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
           mbar_wait_bounded(b_kfull + 8 * (i % C::STAGES), (i / C::STAGES) & 1);
           if (i < j) mbar_wait_bounded(b_vfull + 8 * (i % C::STAGES), (i / C::STAGES) & 1);
         }
-    } else if (warp < 3) {
-      const int x = warp - 1, n_x = tiles_of(x);
+    } else if (warp == 1) {
+      // One warp issues for both chains in turn: with a warp each, their products shared the tensor core, both were through at the
+      // same time, and both then met at the exponentials.
       const uint32_t el = elect_one();
       bool ok = true;
       auto wait = [&](uint32_t bar, uint32_t parity, int code) {
@@ -194,11 +195,12 @@ attn_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
           ok = false;
         }
       };
-      const uint32_t t_s = tmem_base + x * 128, t_o = tmem_base + 256 + x * D, q_tile = q_smem + (wide ? x * C::Q_BYTES : 0);
-      auto tile = [&](int i) { return wide ? i : 2 * i + x; };
       // The values of a tile and the scores of the next one are issued together, and all that either waits for is waited for ahead:
       // a wait between them lasted until the values were through (970 of 5450 cycles a tile).
-      for (int i = 0; ok && i <= n_x; ++i) {
+      auto step = [&](int x, int i) {
+        const int n_x = tiles_of(x);
+        const uint32_t t_s = tmem_base + x * 128, t_o = tmem_base + 256 + x * D, q_tile = q_smem + (wide ? x * C::Q_BYTES : 0);
+        auto tile = [&](int i) { return wide ? i : 2 * i + x; };
         const int j = tile(i), s = j % C::STAGES, j1 = tile(i - 1), s1 = j1 % C::STAGES;
         if (i < n_x) wait(b_kfull + 8 * s, (j / C::STAGES) & 1, ARCB_DEV_WAIT_TIMEOUT_TMA);
         if (i > 0) {
@@ -206,7 +208,7 @@ attn_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
           if (j1 == n_tiles - 1 && left < AT_KEYS) wait(b_clean, 0, ARCB_DEV_WAIT_TIMEOUT_TMA);
           wait(b_p + 8 * x, (i - 1) & 1, ARCB_DEV_WAIT_TIMEOUT_ACC);
         }
-        if (!ok) break;
+        if (!ok) return;
         tc_fence_after();
         if (i > 0) {
           const uint64_t dv = umma_desc_mn_sw128(v_smem + s1 * C::KV_BYTES, AT_BOX);
@@ -230,8 +232,12 @@ attn_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
           umma_commit_if(el, b_kempty + 8 * s);
         }
         if (i > 0) umma_commit_if(el, b_vempty + 8 * s1);
+        if (i > 0 && i == n_x) umma_commit_if(el, b_o + 8 * x);
+      };
+      for (int i = 0; ok && i <= tiles_of(0); ++i) {
+        step(0, i);
+        if (ok && i <= tiles_of(1)) step(1, i);
       }
-      if (ok && n_x > 0) umma_commit_if(el, b_o + 8 * x);
     }
   } else {
     const int x = (warp - 4) >> 2, quarter = warp & 3, n_x = tiles_of(x);
