@@ -144,7 +144,10 @@ attn_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   // S_A [0, 128), S_B [128, 256), O_A [256, 256 + D), O_B
 
+  // 12 warps start with 168 registers a thread; the four that move and issue keep 88, the eight that hold scores, weights and their
+  // sums get 208 (88 + 2 * 208 = 3 * 168).
   if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (warp == 0) {
       bool ok = true;
       auto wait = [&](uint32_t bar, uint32_t parity) {
@@ -240,6 +243,7 @@ attn_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
       }
     }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const int x = (warp - 4) >> 2, quarter = warp & 3, n_x = tiles_of(x);
     const uint32_t t_lane = tmem_base + ((uint32_t)(quarter * 32) << 16);
     const uint32_t t_s = t_lane + x * 128, t_o = t_lane + 256 + x * D;
@@ -249,24 +253,21 @@ attn_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
     const bool idle = first_row >= w.rows;
     bool ok = true;
     float m_ref = -INFINITY, l = 0.f;
-    // 64 of the row's scores; hidden keys become -inf, whose exp2 is exactly 0
-    auto load_scores = [&](int c, int seen, uint32_t (&sv)[2][32]) {
-      tmem_ld_32x32(t_s + c * 64, sv[0]);
-      tmem_ld_32x32(t_s + c * 64 + 32, sv[1]);
-      tmem_wait_ld_dep(sv[0]);
-      tmem_wait_ld_dep(sv[1]);
+    // 32 of the row's scores have come: hidden keys become -inf, whose exp2 is exactly 0
+    auto arrived = [&](int c, int seen, uint32_t (&sv)[32]) {
+      tmem_wait_ld_dep(sv);
       if (seen < AT_KEYS) {
 #pragma unroll
-        for (int e = 0; e < 64; ++e)
-          if (c * 64 + e >= seen) sv[e >> 5][e & 31] = 0xff800000u;
+        for (int e = 0; e < 32; ++e)
+          if (c * 32 + e >= seen) sv[e] = 0xff800000u;
       }
     };
-    auto most = [&](const uint32_t (&sv)[2][32], float mx) {
+    auto most = [&](const uint32_t (&sv)[32], float mx) {
       float m0 = mx, m1 = -INFINITY;
 #pragma unroll
-      for (int e = 0; e < 32; e += 2) {
-        m0 = max3_f32(m0, __uint_as_float(sv[0][e]), __uint_as_float(sv[0][e + 1]));
-        m1 = max3_f32(m1, __uint_as_float(sv[1][e]), __uint_as_float(sv[1][e + 1]));
+      for (int e = 0; e < 32; e += 4) {
+        m0 = max3_f32(m0, __uint_as_float(sv[e]), __uint_as_float(sv[e + 1]));
+        m1 = max3_f32(m1, __uint_as_float(sv[e + 2]), __uint_as_float(sv[e + 3]));
       }
       return fmaxf(m0, m1);
     };
@@ -284,56 +285,60 @@ attn_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
       }
       const int j = wide ? i : 2 * i + x;
       const int seen = j == n_tiles - 1 ? left : AT_KEYS;
-      uint32_t pr[2][32], second[WP > 1 ? 2 : 1][WP > 1 ? 32 : 1];
-      float mx, total;
-      // weights against the reference as it is, and the scores' maximum on the way
-      auto weights = [&]() {
+      uint32_t pr[2][32], second[WP > 1 ? 2 : 1][WP > 1 ? 32 : 1];      // pairs of 64 keys each
+      float total;
+      if (i == 0) {
+        float mx = -INFINITY;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t sv[32];
+          tmem_ld_32x32(t_s + c * 32, sv);
+          arrived(c, seen, sv);
+          mx = most(sv, mx);
+        }
+        m_ref = mx * sc;
+      }
+      // Weights against the reference as it is, and the scores' maximum on the way.  Nearly always the reference stays; where it
+      // has to be raised, the scores are still there for a second time.
+      for (;;) {
         const float m_safe = m_ref == -INFINITY ? 0.f : m_ref;
         const uint64_t nm2 = pack_f32x2(-m_safe, -m_safe);
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-        mx = -INFINITY;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f}, mx = -INFINITY;
+        uint32_t sv[2][32];
+        tmem_ld_32x32(t_s, sv[0]);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t sv[2][32];
-          load_scores(c, seen, sv);
-          mx = most(sv, mx);
+        for (int c = 0; c < 4; ++c) {
+          arrived(c, seen, sv[c & 1]);
+          if (c < 3) tmem_ld_32x32(t_s + (c + 1) * 32, sv[(c + 1) & 1]);      // while these are at work
+          mx = most(sv[c & 1], mx);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
+          for (int e = 0; e < 16; ++e) {
             float t0, t1;
-            shift2_f32(sv[e >> 4][2 * (e & 15)], sv[e >> 4][2 * (e & 15) + 1], sc2, nm2, t0, t1);
+            shift2_f32(sv[c & 1][2 * e], sv[c & 1][2 * e + 1], sc2, nm2, t0, t1);
             t0 = ex2_fast(t0);
             t1 = ex2_fast(t1);
             sum[2 * (e & 1)] += t0;
             sum[2 * (e & 1) + 1] += t1;
-            pr[c][e] = pack2_prob(t0, t1, HALF ? 1 : 0);
+            const uint32_t h = pack2_prob(t0, t1, HALF ? 1 : 0);
+            pr[c >> 1][(c & 1) * 16 + e] = h;
             if constexpr (WP > 1) {
-              const float2 f = unpack2_act(pr[c][e], HALF ? 1 : 0);
-              second[c][e] = pack2_prob(t0 - f.x, t1 - f.y, HALF ? 1 : 0);
+              const float2 f = unpack2_act(h, HALF ? 1 : 0);
+              second[c >> 1][(c & 1) * 16 + e] = pack2_prob(t0 - f.x, t1 - f.y, HALF ? 1 : 0);
             }
           }
         }
         total = (sum[0] + sum[1]) + (sum[2] + sum[3]);
         mx *= sc;
-      };
-      if (i == 0) {
-        uint32_t sv[2][32];
-        load_scores(0, seen, sv);
-        mx = most(sv, -INFINITY);
-        load_scores(1, seen, sv);
-        m_ref = most(sv, mx) * sc;
-        weights();
-      } else {
-        // Nearly always the reference stays; where it has to be raised, the scores are still there.
-        weights();
         const bool raise = mx > m_ref + AT_RESCALE;
-        if (__any_sync(0xffffffffu, raise)) {
-          float alpha = 1.f;
-          if (raise) {
-            alpha = m_ref == -INFINITY ? 0.f : ex2_fast(m_ref - mx);
-            m_ref = mx;
-            l *= alpha;
-          }
-          // these scores were asked for behind the last product of values: its sums are complete
+        if (!__any_sync(0xffffffffu, raise)) break;
+        float alpha = 1.f;
+        if (raise) {
+          alpha = m_ref == -INFINITY ? 0.f : ex2_fast(m_ref - mx);
+          m_ref = mx;
+          l *= alpha;
+        }
+        // these scores were asked for behind the last product of values: its sums are complete
+        if (i > 0)
 #pragma unroll 1
           for (int c = 0; c < D / 32; ++c) {
             uint32_t o[32];
@@ -343,8 +348,6 @@ attn_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
             for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
             tmem_st_32x32(t_o + c * 32, o);
           }
-          weights();
-        }
       }
       l += total;
       // over scores that have all been read
