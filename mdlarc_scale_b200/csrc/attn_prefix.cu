@@ -243,7 +243,7 @@ attn_prefix_join_cta_kernel(AttnPrefixArgs a) {
 void fill_plan(AttnPrefixArgs& a) {
   a.rep = a.n_heads / a.n_kv;
   const bool tc = a.kv_fmt != 2 && (a.act_fmt == a.kv_fmt || a.dim == 64) && a.scale != 0.f;
-  a.plan = prefix_plan(a.n_groups, a.max_group, a.max_prefix, a.n_items, a.item_end ? a.max_own : 0, a.n_kv, a.rep, a.kv_fmt == 2, tc, arcb_num_sms());
+  a.plan = prefix_plan(a.n_groups, a.max_group, a.max_prefix, a.n_items, a.item_end ? a.max_own : 0, a.n_kv, a.rep, a.dim, a.kv_fmt == 2, tc, arcb_num_sms());
 }
 
 int launch_part(const AttnPrefixArgs& a, int kernel, long long units, cudaStream_t stream) {
@@ -291,7 +291,7 @@ int arcb_launch_attn_prefix(AttnPrefixArgs a, cudaStream_t stream) {
   }
   if (r || p.parts == 1) return r;
   // Its CTAs come while the last ones of the parts are at work, and wait.  Four warps a result where a warp each would leave SMs without work
-  const bool few = p.parts > 8 && joins < 4LL * arcb_num_sms();
+  const bool few = joins < 4LL * arcb_num_sms();
   arcb_count_launch(1);
   return (int)(few ? ap_launch_beside(attn_prefix_join_cta_kernel, dim3((unsigned)((long long)a.n_items * a.n_heads)), dim3(128), 0, stream, a)
                    : ap_launch_beside(attn_prefix_join_kernel, dim3((unsigned)joins), dim3(128), 0, stream, a));

@@ -29,36 +29,39 @@ inline PrefixPart prefix_part(long long heads, long long rows, int n_kv, bool wi
   p.units = heads * n_kv * p.tiles;
   return p;
 }
-inline int prefix_cut(long long rows, long long chunk, long long most) {
-  return (int)std::min(most, std::max(1LL, (rows + chunk - 1) / chunk));
-}
-// What runs at once is given about equal shares of `total` cached rows; four units each where they are long, so that lengths that
-// differ even out.
-inline long long prefix_chunk(long long total, long long at_once, long long least) {
-  const long long each = total / at_once;
-  return each < 4 * least ? std::max(least, each) : std::max(4 * least, each / 4);
+// Ranges for `rows` cached rows where every slot of the GPU has `each` rows to read.  Up to 1024, what runs at once gets one range each
+// (rounded so that no few are left for a second wave); above, up to four, so that lengths that differ even out.
+inline int prefix_cut(long long rows, long long each, long long least, long long most) {
+  const long long fewest = (rows + least - 1) / least;
+  const long long s = each <= 1024 ? rows / std::max(1LL, each) : (rows + std::max(1024LL, each / 4) - 1) / std::max(1024LL, each / 4);
+  return (int)std::min(most, std::max(1LL, std::min(fewest, s)));
 }
 
 // max_group items of `rep` heads share a group's rows.
 inline PrefixPlan prefix_plan(long long n_groups, long long max_group, long long max_prefix, long long n_items, long long max_own, int n_kv,
-                              int rep, bool wide, bool tc, int sms) {
+                              int rep, int dim, bool wide, bool tc, int sms) {
   PrefixPlan p{};
   p.shared = prefix_part(n_groups, n_groups > 0 ? max_group * rep : 0, n_kv, wide, tc);
   p.own = prefix_part(n_items, max_own > 0 ? rep : 0, n_kv, wide, false);
   const bool any1 = n_groups > 0, any2 = max_own > 0;
   p.together = any1 && any2 && p.shared.kernel == p.own.kernel;
   const long long total1 = p.shared.units * max_prefix, total2 = p.own.units * max_own;
-  const auto at_once = [&](int kernel) { return (long long)sms * (kernel == AP_ROWS ? 12 : 4); };
-  const auto least = [](int kernel) { return kernel == AP_ROWS ? 64LL : 128LL; };
-  if (any2) p.own.splits = prefix_cut(max_own, prefix_chunk(total2 + (p.together ? total1 : 0), at_once(p.own.kernel), least(p.own.kernel)), 32);
+  const auto slots = [&](int kernel) { return (long long)sms * (kernel == AP_ROWS ? 12 : kernel == AP_TILES ? 3 : 4); };
+  const auto least = [](int kernel) { return kernel == AP_TILES ? 256LL : 64LL; };
+  if (any2) p.own.splits = prefix_cut(max_own, (total2 + (p.together ? total1 : 0)) / slots(p.own.kernel), least(p.own.kernel), 32);
   if (any1 && p.shared.kernel != AP_TC) {
-    p.shared.splits = prefix_cut(max_prefix, prefix_chunk(total1 + (p.together ? total2 : 0), at_once(p.shared.kernel), least(p.shared.kernel)), 128);
+    p.shared.splits = prefix_cut(max_prefix, (total1 + (p.together ? total2 : 0)) / slots(p.shared.kernel), least(p.shared.kernel), 128);
   } else if (any1) {
-    // one CTA an SM: the number of ranges whose waves take the fewest steps of 128 rows; a CTA's start and end count as three
-    long long best = 0;
+    // One CTA an SM: the number of ranges whose waves take the fewest steps of 128 rows.  A CTA's start and end count as eight, what a
+    // range's results are written and joined for as their bytes over 10^7.  Groups differ in length: half of the cost is that of
+    // waves that end on the average unit.
+    const double joined = 2.0 * n_items * n_kv * rep * (dim + 4) * 4 / 1e7;
+    double best = 0;
     for (int s = 1; s <= 32; ++s) {
-      const long long waves = (p.shared.units * s + sms - 1) / sms, steps = ((max_prefix + s - 1) / s + 127) / 128;
-      const long long cost = waves * (steps + 3);
+      const long long steps = ((max_prefix + s - 1) / s + 127) / 128;
+      double waves = (double)((p.shared.units * s + sms - 1) / sms);
+      if (n_groups > 1) waves = (waves + (double)(p.shared.units * s) / sms + 0.5) / 2;
+      const double cost = waves * (steps + 8) + s * joined;
       if (s == 1 || cost < best) {
         best = cost;
         p.shared.splits = s;
