@@ -26,7 +26,7 @@ FORM_IDS = ["f16-bf16", "bf16", "f16", "f32"]
 class Case:
     """Ragged groups over one cache; every row that no item may see holds NaN."""
 
-    def __init__(self, sizes, prefix, own, heads, kv, dim, form, seed=0, own_in_group=False, sharp=1.0, spread=1.0):
+    def __init__(self, sizes, prefix, own, heads, kv, dim, form, seed=0, own_in_group=False, sharp=1.0, spread=1.0, rows=0):
         g = torch.Generator(device="cuda").manual_seed(seed)
         r = np.random.default_rng(seed)
         n = sum(sizes)
@@ -34,11 +34,11 @@ class Case:
         first = np.concatenate([[0], np.cumsum(sizes)]).astype(int)
         group_of = np.repeat(np.arange(len(sizes)), sizes)
         self.begin = [prefix[x] if own_in_group else int(r.integers(0, 20)) for x in group_of]
-        seqs = len(sizes) + n
+        seqs = len(sizes) if rows else len(sizes) + n
         places = r.permutation(seqs)
         self.group_seq = places[:len(sizes)].tolist()
         self.item_seq = [self.group_seq[x] for x in group_of] if own_in_group else places[len(sizes):].tolist()
-        rows = max([*prefix, *[b + o for b, o in zip(self.begin, own)], 1]) + int(r.integers(0, 3))
+        rows = rows or max([*prefix, *[b + o for b, o in zip(self.begin, own)], 1]) + int(r.integers(0, 3))
         q_type, kv_type = form
         self.q = (torch.randn((n, heads, dim), device="cuda", generator=g) * sharp).to(q_type)
         k = torch.randn((seqs, kv, rows, dim), device="cuda", generator=g) * spread
@@ -119,6 +119,26 @@ def test_query_tiles(form, items, heads, kv):
 
 
 @pytest.mark.parametrize("form", FORMS, ids=FORM_IDS)
+@pytest.mark.parametrize("items,heads,kv", [(17, 4, 1), (65, 2, 2), (43, 3, 1), (128, 1, 1), (129, 1, 1), (70, 8, 2), (257, 1, 1), (300, 2, 1)])
+def test_query_tiles_of_a_long_cache(form, items, heads, kv):
+    """Without hints the plan is made for groups as long as a cache: most ranges of these are short or empty."""
+    for dim in (64, 128):
+        for prefix in (3, 1153):
+            c = Case([items, 2], [prefix, 130], [i % 5 for i in range(items + 2)], heads, kv, dim, form, items, own_in_group=True, rows=4144)
+            c.check(c())
+
+
+@pytest.mark.parametrize("form", FORMS, ids=FORM_IDS)
+@pytest.mark.parametrize("prefix", [0, 1, 127, 128, 129, 255, 257, 1025, 4097, 4140])
+def test_lengths_in_a_long_cache(form, prefix):
+    for dim in (64, 128):
+        for items in (33, 70):
+            c = Case([items], [prefix], [i % 3 for i in range(items)], 4, 2, dim, form, prefix, own_in_group=True, rows=4144)
+            c.check(c())
+            c.check(prefix_attention(c.q, c.k, c.v, *c.groups), mine=False)
+
+
+@pytest.mark.parametrize("form", FORMS, ids=FORM_IDS)
 @pytest.mark.parametrize("dim", [64, 128])
 def test_long_rows_in_many_ranges(form, dim):
     """Rows cut into as many ranges as the plan makes; all kinds of lengths in one call, some empty."""
@@ -131,6 +151,8 @@ def test_many_queries_over_a_long_prefix(form):
     c = Case([90, 70], [2900, 1031], [i * 7 % 40 for i in range(160)], 8, 2, 128, form, 5)
     c.check(c())
     c = Case([150, 3], [1500, 2100], [i * 7 % 40 for i in range(153)], 3, 3, 64, form, 6)
+    c.check(c())
+    c = Case([100, 71], [4600, 9003], [i % 4 for i in range(171)], 2, 1, 64, form, 7, own_in_group=True, rows=9008, sharp=3.0)
     c.check(c())
 
 
