@@ -16,126 +16,6 @@ int arcb_fail_cuda(cudaError_t e, const char* where);
 
 namespace {
 
-// ---- 32-bit formats: multiply-adds ----
-// Four warps of four query rows; 32 cached rows at a time in shared memory.  Scores: a lane has a cached row; sums: a lane has
-// every 32nd value column.
-constexpr int AS_ROWS = 16, AS_KEYS = 32;
-
-template <int D>
-__global__ void __launch_bounds__(128)
-attn_prefix_simple_kernel(AttnPrefixArgs a) {
-  pdl_launch_dependents();
-  pdl_wait();
-  __shared__ __align__(16) float s_q[AS_ROWS][D];
-  __shared__ __align__(16) float s_k[AS_KEYS][D + 4];
-  __shared__ __align__(16) float s_v[AS_KEYS][D];
-  const int lane = threadIdx.x & 31, wj = threadIdx.x >> 5;
-  const ApWork w = ap_work(a, a.first_block + blockIdx.x, threadIdx.x == 0);
-  if (w.rows <= 0) return;
-  for (int i = threadIdx.x; i < AS_ROWS * D / 4; i += 128) {
-    const int r = i / (D / 4), c = i % (D / 4) * 4;
-    float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (r < w.rows) {
-      const int R = w.r0 + r;
-      q = ld_act4(a.q, (size_t)(w.item0 + R / a.rep) * a.q_pitch + (size_t)(w.kvh * a.rep + R % a.rep) * D + c, a.act_fmt);
-    }
-    *reinterpret_cast<float4*>(&s_q[r][c]) = q;
-  }
-  const size_t row0 = ((size_t)w.seq * a.n_kv + w.kvh) * (size_t)a.t_max;
-  const float sc = a.scale * AP_LOG2E;
-  float m[4], l[4], acc[4][D / 32];
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    m[r] = -INFINITY;
-    l[r] = 0.f;
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) acc[r][i] = 0.f;
-  }
-  for (int t = w.begin; t < w.end; t += AS_KEYS) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < AS_KEYS * D / 4; i += 128) {
-      const int r = i / (D / 4), c = i % (D / 4) * 4;
-      float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
-      if (t + r < w.end) {
-        k = ld_act4(a.k, (row0 + t + r) * D + c, a.kv_fmt);
-        v = ld_act4(a.v, (row0 + t + r) * D + c, a.kv_fmt);
-      }
-      *reinterpret_cast<float4*>(&s_k[r][c]) = k;
-      *reinterpret_cast<float4*>(&s_v[r][c]) = v;
-    }
-    __syncthreads();
-    if (wj * 4 >= w.rows) continue;
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int c = 0; c < D; c += 4) {
-      const float4 k = *reinterpret_cast<const float4*>(&s_k[lane][c]);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float4 q = *reinterpret_cast<const float4*>(&s_q[wj * 4 + r][c]);
-        s[r] = fmaf(q.x, k.x, s[r]);
-        s[r] = fmaf(q.y, k.y, s[r]);
-        s[r] = fmaf(q.z, k.z, s[r]);
-        s[r] = fmaf(q.w, k.w, s[r]);
-      }
-    }
-    float p[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      s[r] = t + lane < w.end ? s[r] * sc : -INFINITY;
-      float mx = s[r];
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      mx = fmaxf(mx, m[r]);
-      const float safe = mx == -INFINITY ? 0.f : mx;
-      const float alpha = exp2f(m[r] - safe);
-      m[r] = mx;
-      p[r] = exp2f(s[r] - safe);
-      l[r] = l[r] * alpha + p[r];
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i) acc[r][i] *= alpha;
-    }
-    const int n = min(AS_KEYS, w.end - t);
-#pragma unroll 4
-    for (int j = 0; j < n; ++j) {
-      float v[D / 32];
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i) v[i] = s_v[j][lane + 32 * i];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float pr = __shfl_sync(0xffffffffu, p[r], j);
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) acc[r][i] = fmaf(pr, v[i], acc[r][i]);
-      }
-    }
-  }
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int R = w.r0 + wj * 4 + r;
-    if (wj * 4 + r >= w.rows) break;
-    const int item = w.item0 + R / a.rep;
-    const long long ih = (long long)item * a.n_heads + w.kvh * a.rep + R % a.rep;
-    const float sum = warp_sum(l[r]);
-    if (a.plan.parts == 1) {
-      const bool none = sum == 0.f || (a.item_skip && a.item_skip[item]);
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i) {
-        const float o = none ? 0.f : acc[r][i] / sum;
-        const size_t at = (size_t)ih * D + lane + 32 * i;
-        if (a.act_fmt == 1 && isnan(o)) reinterpret_cast<__half*>(a.out)[at] = __float2half_rn(o);
-        else st_act(a.out, at, o, a.act_fmt);
-      }
-    } else {
-      float* rec = ap_record(a, ih, w.part);
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i) rec[lane + 32 * i] = acc[r][i];
-      if (lane == 0) {
-        rec[D] = m[r];
-        rec[D + 1] = sum;
-      }
-    }
-  }
-}
-
 // Joins the parts of an (item, head) in order, a warp for each: the maximum of all, then their sums with lane s at the factor of
 // every 32nd part.
 __global__ void __launch_bounds__(128)
@@ -250,15 +130,14 @@ void fill_plan(AttnPrefixArgs& a) {
   a.plan = prefix_plan(a.n_groups, a.max_group, a.max_prefix, a.n_items, a.item_end ? a.max_own : 0, a.n_kv, a.rep, a.dim, a.kv_fmt == 2, tc, arcb_num_sms());
 }
 
-int launch_part(const AttnPrefixArgs& a, int kernel, long long units, cudaStream_t stream) {
+int launch_part(const AttnPrefixArgs& a, const PrefixPart& p, long long units, cudaStream_t stream) {
   arcb_count_launch(1);
-  switch (kernel) {
+  switch (p.kernel) {
     case AP_ROWS: return arcb_attn_prefix_rows(a, units, stream);
     case AP_TILES: return arcb_attn_prefix_mma(a, units, stream);
     case AP_TC: return arcb_attn_prefix_tc(a, units, stream);
   }
-  return (int)(a.dim == 64 ? arcb_launch(attn_prefix_simple_kernel<64>, dim3((unsigned)units), dim3(128), 0, stream, a)
-                           : arcb_launch(attn_prefix_simple_kernel<128>, dim3((unsigned)units), dim3(128), 0, stream, a));
+  return arcb_attn_prefix_f32(a, p.tile, units, stream);
 }
 
 }  // namespace
@@ -285,13 +164,13 @@ int arcb_launch_attn_prefix(AttnPrefixArgs a, cudaStream_t stream) {
   a.first_block = 0;
   a.beside = 0;
   int r = 0;
-  if (p.shared.units > 0) r = launch_part(a, p.shared.kernel, p.shared.units + (p.together ? p.own.units : 0), stream);
+  if (p.shared.units > 0) r = launch_part(a, p.shared, p.shared.units + (p.together ? p.own.units : 0), stream);
   if (r == 0 && p.own.units > 0 && !p.together) {
     a.first_block = p.shared.units;
     // Beside the shared part, which it does not depend on.  What came before that one is over when it starts, unless the library
     // launches everything programmatically.
     a.beside = p.shared.units > 0 && !arcb_pdl_enabled();
-    r = launch_part(a, p.own.kernel, p.own.units, stream);
+    r = launch_part(a, p.own, p.own.units, stream);
   }
   if (r || p.parts == 1) return r;
   // Its CTAs come while the last ones of the parts are at work, and wait.  Four warps a result where a warp each would leave SMs without work

@@ -40,6 +40,8 @@ constexpr int AP_PAD = 4;     // of a partial result: the sums of a row's values
 int arcb_attn_prefix_rows(const AttnPrefixArgs& a, long long units, cudaStream_t stream);
 int arcb_attn_prefix_mma(const AttnPrefixArgs& a, long long units, cudaStream_t stream);
 int arcb_attn_prefix_tc(const AttnPrefixArgs& a, long long units, cudaStream_t stream);
+// 32-bit formats, units of `tile` rows (attn_prefix_f32.cu)
+int arcb_attn_prefix_f32(const AttnPrefixArgs& a, int tile, long long units, cudaStream_t stream);
 
 bool arcb_attn_prefix_supported(int n_heads, int n_kv, int dim, int act_fmt, int kv_fmt);
 // bytes of a.scratch for these sizes

@@ -68,7 +68,7 @@ __device__ __forceinline__ ApWork ap_work(const AttnPrefixArgs& a, long long blo
     k.r0 = t * a.plan.shared.tile;
     k.rows = min(a.plan.shared.tile, (last - first) * a.rep - k.r0);
     at0 = 0;
-    grain = a.plan.shared.kernel == AP_TC ? 127 : a.plan.shared.kernel == AP_TILES ? 63 : 15;
+    grain = a.plan.shared.kernel == AP_TC ? 127 : a.plan.shared.kernel == AP_ROWS ? 15 : 63;
     k.part = split;
   } else {
     w -= n1;
@@ -87,7 +87,7 @@ __device__ __forceinline__ ApWork ap_work(const AttnPrefixArgs& a, long long blo
       len = 0;
     }
     if (len < 0 || (a.item_skip && a.item_skip[k.item0])) len = 0;
-    grain = a.plan.own.kernel == AP_TILES ? 63 : 15;
+    grain = a.plan.own.kernel == AP_ROWS ? 15 : 63;
     k.part = a.plan.shared.splits + split;
   }
   int chunk = (len + splits - 1) / splits;

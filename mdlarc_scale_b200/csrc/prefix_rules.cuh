@@ -2,9 +2,9 @@
 #pragma once
 #include <algorithm>
 
-// Kernels, by the query rows of a unit: a warp for up to 8, a CTA for up to 64, a CTA with tcgen05 products for up to 256; a CTA of
-// multiply-adds for 16 in 32-bit formats.
-enum : int { AP_ROWS = 0, AP_TILES = 1, AP_TC = 2, AP_PLAIN = 3 };
+// Kernels, by the query rows of a unit: a warp for up to 8, a CTA for up to 64, a CTA with tcgen05 products for up to 256; in 32-bit
+// formats a warp for up to 4, a CTA for up to 64.
+enum : int { AP_ROWS = 0, AP_TILES = 1, AP_TC = 2, AP_F32_FEW = 3, AP_F32 = 4 };
 
 struct PrefixPart {
   int kernel;               // AP_*
@@ -23,8 +23,8 @@ struct PrefixPlan {
 // `rows` query rows at each of `heads` (groups or items) x n_kv; `tc`: tcgen05 may be used.
 inline PrefixPart prefix_part(long long heads, long long rows, int n_kv, bool wide, bool tc) {
   PrefixPart p{};
-  p.kernel = wide ? AP_PLAIN : rows <= 8 ? AP_ROWS : rows <= 64 || !tc ? AP_TILES : AP_TC;
-  p.tile = p.kernel == AP_PLAIN ? 16 : p.kernel == AP_ROWS ? 8 : p.kernel == AP_TC ? 256 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+  p.kernel = wide ? (rows <= 4 ? AP_F32_FEW : AP_F32) : rows <= 8 ? AP_ROWS : rows <= 64 || !tc ? AP_TILES : AP_TC;
+  p.tile = p.kernel == AP_F32_FEW ? (rows <= 2 ? (int)std::max(1LL, rows) : 4) : p.kernel == AP_ROWS ? 8 : p.kernel == AP_TC ? 256 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
   p.tiles = (int)((rows + p.tile - 1) / p.tile);
   p.units = heads * n_kv * p.tiles;
   return p;
@@ -44,13 +44,16 @@ inline PrefixPlan prefix_plan(long long n_groups, long long max_group, long long
   p.shared = prefix_part(n_groups, n_groups > 0 ? max_group * rep : 0, n_kv, wide, tc);
   p.own = prefix_part(n_items, max_own > 0 ? rep : 0, n_kv, wide, false);
   const bool any1 = n_groups > 0, any2 = max_own > 0;
-  p.together = any1 && any2 && p.shared.kernel == p.own.kernel;
+  p.together = any1 && any2 && p.shared.kernel == p.own.kernel && (!wide || p.shared.tile == p.own.tile);
   const long long total1 = p.shared.units * max_prefix, total2 = p.own.units * max_own;
-  const auto slots = [&](int kernel) { return (long long)sms * (kernel == AP_ROWS ? 12 : kernel == AP_TILES ? 3 : 4); };
+  const auto slots = [&](const PrefixPart& part) {
+    const int k = part.kernel;
+    return (long long)sms * (k == AP_ROWS ? 12 : k == AP_F32_FEW ? 8 : k == AP_TILES ? 3 : dim == 128 || part.tile == 64 ? 2 : 4);
+  };
   const auto least = [](int kernel) { return kernel == AP_TILES ? 256LL : 64LL; };
-  if (any2) p.own.splits = prefix_cut(max_own, (total2 + (p.together ? total1 : 0)) / slots(p.own.kernel), least(p.own.kernel), 32);
+  if (any2) p.own.splits = prefix_cut(max_own, (total2 + (p.together ? total1 : 0)) / slots(p.own), least(p.own.kernel), 32);
   if (any1 && p.shared.kernel != AP_TC) {
-    p.shared.splits = prefix_cut(max_prefix, (total1 + (p.together ? total2 : 0)) / slots(p.shared.kernel), least(p.shared.kernel), 128);
+    p.shared.splits = prefix_cut(max_prefix, (total1 + (p.together ? total2 : 0)) / slots(p.shared), least(p.shared.kernel), 128);
   } else if (any1) {
     // One CTA an SM: the number of ranges whose waves take the fewest steps of 128 rows.  A CTA's start and end count as eight, what a
     // range's results are written and joined for as their bytes over 10^7.  Groups differ in length: half of the cost is that of
