@@ -226,8 +226,8 @@ def load() -> C.CDLL:
     lib.arcb_op_decode_attention.argtypes = [vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, vp, i32, vp]
     lib.arcb_op_decode_attention_static.argtypes = [vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, vp]
     lib.arcb_prefix_attention_scratch_bytes.restype = i64
-    lib.arcb_prefix_attention_scratch_bytes.argtypes = [C.POINTER(PrefixAttentionArgs)]
-    lib.arcb_op_prefix_attention.argtypes = [C.POINTER(PrefixAttentionArgs), vp]
+    lib.arcb_prefix_attention_scratch_bytes.argtypes = [vp]        # PrefixAttentionArgs by reference, or packed
+    lib.arcb_op_prefix_attention.argtypes = [vp, vp]
     lib.arcb_op_cache_copy.argtypes = [vp, i32, i32, i32, i32, i32, vp, i32, vp]
     lib.arcb_op_head.argtypes = [vp, vp, vp, vp, vp, vp, i32, i32, f32, vp]
     _lib = lib

@@ -2,7 +2,7 @@
 between sequences."""
 from __future__ import annotations
 
-import ctypes as C
+import struct
 
 import numpy as np
 import torch
@@ -13,6 +13,9 @@ _FORMATS = {torch.float16: _lib.ACT_F16, torch.bfloat16: _lib.ACT_BF16, torch.fl
 
 
 _I32, _U8 = torch.int32, torch.uint8
+# The fields of _lib.PrefixAttentionArgs: packing them takes a sixth of filling the ctypes structure, which a call's time shows.
+_ARGS = struct.Struct("@13P2q10if3i")
+_SCRATCH, _SCRATCH_AT = struct.Struct("@Pq"), _lib.PrefixAttentionArgs.d_scratch.offset
 _raw_stream = torch._C._cuda_getCurrentRawStream      # the current stream's handle; torch.cuda.current_stream() takes 2 us
 
 
@@ -55,7 +58,7 @@ def prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, group_fi
             raise ValueError("an item's heads must be consecutive")
         pitch = q.stride(0) if n > 1 else 0
     if out is None:
-        out = torch.empty((n, heads, dim), dtype=q.dtype, device=q.device)
+        out = q.new_empty((n, heads, dim)) if pitch else torch.empty_like(q)
     elif out.shape != q.shape or out.dtype != q.dtype or out.get_device() != dev or not out.is_contiguous():
         raise ValueError("out must be a contiguous tensor like the queries")
     if n == 0:
@@ -63,12 +66,12 @@ def prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, group_fi
 
     def index(t, size, name, dtype=_I32):
         if t is None:
-            return None
+            return 0
         if t.dtype is not dtype or t.numel() != size or t.get_device() != dev or not t.is_contiguous():
             _refuse_index(name, size)
         return t.data_ptr()
 
-    groups, first, seq, length = 0, None, None, None
+    groups = first = seq = length = 0
     if group_first is not None:
         groups = group_first.numel() - 1
         if groups < 1 or group_seq is None or group_len is None:
@@ -77,26 +80,30 @@ def prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, group_fi
     max_group, max_prefix, max_own = max_group or 0, max_prefix or 0, max_own or 0
     if max_group < 0 or max_prefix < 0 or max_own < 0:
         raise ValueError("max_group, max_prefix and max_own must not be negative")
-    a = _lib.PrefixAttentionArgs(
+    fields = (
         q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), first, seq, length, index(item_seq, n, "item_seq"), index(item_begin, n, "item_begin"),
-        index(item_end, n, "item_end"), index(skip, n, "skip", _U8), index(status, 1, "status"), None, 0, pitch, groups, n, heads, kv, dim, seqs, rows,
+        index(item_end, n, "item_end"), index(skip, n, "skip", _U8), index(status, 1, "status"), 0, 0, pitch, groups, n, heads, kv, dim, seqs, rows,
         max_group, max_prefix, max_own, dim ** -0.5 if scale is None else scale, act, form, 0)
+    try:
+        a = _ARGS.pack(*fields)
+    except (struct.error, OverflowError):
+        raise ValueError("scale, max_group, max_prefix and max_own must be numbers of 32 bits") from None
     if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):
-            _attend(a, dev)
+            _attend(a, out, dev)
     else:
-        _attend(a, dev)
+        _attend(a, out, dev)
     return out
 
 
-def _attend(a, dev: int) -> None:
-    lib, ref = _lib.load(), C.byref(a)
-    need = lib.arcb_prefix_attention_scratch_bytes(ref)
+def _attend(a: bytes, out: torch.Tensor, dev: int) -> None:
+    lib = _lib.load()
+    need = lib.arcb_prefix_attention_scratch_bytes(a)
     if need > 0:
         # from the current stream's pool: free for the next call on it when this one's kernels are done
-        scratch = torch.empty(need, dtype=_U8, device=f"cuda:{dev}")
-        a.d_scratch, a.scratch_bytes = scratch.data_ptr(), need
-    code = need if need < 0 else lib.arcb_op_prefix_attention(ref, _raw_stream(dev))
+        scratch = torch.empty(need, dtype=_U8, device=out.device)
+        a = a[:_SCRATCH_AT] + _SCRATCH.pack(scratch.data_ptr(), need) + a[_SCRATCH_AT + _SCRATCH.size:]
+    code = need if need < 0 else lib.arcb_op_prefix_attention(a, _raw_stream(dev))
     if code:
         _lib.check(code)
 

@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 import torch
 
-from mdlarc_scale_b200 import _lib
+from mdlarc_scale_b200 import _lib, prefix
 from mdlarc_scale_b200.engine import plan_prefill
 from mdlarc_scale_b200.generation import Request, Scheduler, generate
 from test_vodavik_host import _CpuEngine, _CpuSession, _Lens
@@ -104,6 +104,9 @@ def test_argument_layout_is_the_headers(tmp_path):
     got = [int(v) for v in subprocess.run([str(tmp_path / "p")], capture_output=True, text=True, check=True).stdout.split()]
     want = [C.sizeof(_lib.PrefixAttentionArgs)] + [getattr(_lib.PrefixAttentionArgs, f).offset for f in fields]
     assert got == want + [C.sizeof(_lib.SessionDesc), _lib.SessionDesc.prefix_group.offset]
+    values = [0.5 if f == "scale" else 3 + i for i, f in enumerate(fields)]
+    packed = _lib.PrefixAttentionArgs.from_buffer_copy(prefix._ARGS.pack(*values))
+    assert prefix._ARGS.size == want[0] and [getattr(packed, f) for f in fields] == values
 
 
 @pytest.fixture(scope="module")
