@@ -1,10 +1,12 @@
-// Attention over shared cached rows in 16-bit formats for few query rows at a time: the rows of an item's own, and shared
-// rows that up to 24 query rows see.
+// Attention over shared cached rows in 16-bit formats for up to eight query rows at a time: the rows of an item's own, and shared
+// rows that few queries see.
 //
-// A unit of work is a range of one sequence's cached rows and up to 24 query rows.  A warp takes units by itself: keys and values
-// travel by TMA into a ring of its own (boxes of 64 columns, 128-byte swizzle), and the ring runs on into the next unit (its
-// queries with its first tile) while this one is finished, so that a unit's start costs no wait and short ranges stream as
-// long ones do.  There is no barrier between warps: every unit writes a part of the result.
+// A unit of work is a range of one sequence's cached rows and up to eight query rows.  A warp takes units by itself: keys and values
+// come by cp.async into a ring of its own (rows of 128 bytes, 16-byte pieces exclusive-or swizzled), and the ring runs on into the
+// next unit (its queries with its first tile) while this one is finished, so that a unit's start costs no wait and short ranges
+// stream as long ones do.  There is no barrier between warps: every unit writes a part of the result, which a second kernel joins.
+// Where the rows of a whole group are few, the eight warps of one CTA take all units of a (group, key head) and join them in
+// shared memory: one launch in place of two and no parts in memory.
 // Descriptions of units are worked out for 32 units of a warp at once, one a lane.
 //
 // The products are transposed, so that the eight columns of m16n8k16 are queries: S^T = K Q^T (16 keys a product) and O^T += V^T P^T
@@ -14,9 +16,8 @@
 //
 // Rounding: a weight enters the product as two 16-bit pieces (p = hi + lo), since one piece alone would be as far off as the
 // output's own rounding; half queries over a bfloat16 cache are two bfloat16 pieces, which is exact.  With up to four query rows the
-// weights' pieces are columns of their own and cost nothing; with more than 16 in equal formats weights are one piece (sqrt 2 of the
-// output's own rounding error in all), where a second one would bind the kernel to its products.  Maxima, sums and all partial
-// results are fp32; a range's reference maximum is raised only when it grows by 2^8.
+// weights' pieces are columns of their own and cost nothing.  Maxima, sums and all partial results are fp32; a range's reference
+// maximum is raised only when it grows by 2^8.
 #include "attn_prefix_frag.cuh"
 #include "flash_common.cuh"
 #include "gemm.cuh"
@@ -27,7 +28,7 @@ using namespace sm100;
 namespace {
 
 constexpr float AR_RESCALE = 8.f;      // log2 units
-constexpr int AR_WARPS = 4;
+constexpr int AR_WARPS = 4;      // of a CTA; AP_GROUP_WARPS of one that takes a group
 
 template <int D>
 struct ArCfg {
@@ -44,8 +45,8 @@ struct ArCfg {
   static_assert(CTAS * (SMEM + 1024) <= 228 * 1024, "CTAs of an SM");
 };
 
-// What a warp keeps from unit to unit.
-template <int D>
+// What a warp keeps from unit to unit.  GROUP: the units are those of group g and key head kvh, the shared ranges and then the items'.
+template <int D, bool GROUP>
 struct ArWarp {
   using C = ArCfg<D>;
   static constexpr int CH = D / 8;         // 16-byte pieces of a row
@@ -59,12 +60,26 @@ struct ArWarp {
   int ahead_i, ahead_left, rows_left;      // the rows from the next one on, and where they are
   const char* from[2];
   int flight, put, get;                    // tiles asked for and not used up
+  int g, kvh, item0, items;                // GROUP: and its items
+  float* records;                          // GROUP: [query row][part][D + AP_PAD]
+
+  __device__ __forceinline__ ApWork work(long long u) const {
+    if constexpr (GROUP) {
+      const int splits = a.plan.shared.splits, own = (int)u - splits;
+      if (own < 0) return ap_work(a, ((long long)g * a.n_kv + kvh) * splits + u, true);
+      const int item = own / a.plan.own.splits;
+      if (item >= items) return ApWork{};
+      return ap_work(a, a.plan.shared.units + ((long long)(item0 + item) * a.n_kv + kvh) * a.plan.own.splits + own % a.plan.own.splits, true);
+    } else {
+      return ap_work(a, a.first_block + u, true);
+    }
+  }
 
   __device__ __forceinline__ ApWork unit(int i) {
     if (i >> 5 != batch_of) {
       batch_of = i >> 5;
       const long long u = first + (long long)((batch_of << 5) + lane) * stride;
-      if (u < n_units) batch = ap_work(a, a.first_block + u, true);
+      if (u < n_units) batch = work(u);
     }
     ApWork w;
     const int from = i & 31;
@@ -142,8 +157,8 @@ struct ArWarp {
 };
 
 // One unit.  PAIR: up to four query rows; columns 4 to 7 of the products are second pieces of weights.
-template <int D, bool HALF, bool QS, bool PAIR>
-__device__ __forceinline__ void ar_unit(ArWarp<D>& s, const ApWork& w, int i) {
+template <int D, bool HALF, bool QS, bool PAIR, bool GROUP>
+__device__ __forceinline__ void ar_unit(ArWarp<D, GROUP>& s, const ApWork& w, int i) {
   using C = ArCfg<D>;
   constexpr int DK = D / 16, MT = C::KEYS / 16;
   const AttnPrefixArgs& a = s.a;
@@ -287,7 +302,9 @@ __device__ __forceinline__ void ar_unit(ArWarp<D>& s, const ApWork& w, int i) {
     const int R = w.r0 + (in ? r : 0), item = w.item0 + R / a.rep;
     const long long ih = (long long)item * a.n_heads + w.kvh * a.rep + R % a.rep;
     const float inv = l[x] == 0.f || (whole && in && a.item_skip && a.item_skip[item]) ? 0.f : 1.f / l[x];
-    float* to = whole ? nullptr : ap_record(a, ih, w.part) + (lane >> 2);
+    float* to = whole ? nullptr
+                : GROUP ? s.records + (((item - s.item0) * a.rep + R % a.rep) * a.plan.parts + w.part) * (D + AP_PAD) + (lane >> 2)
+                        : ap_record(a, ih, w.part) + (lane >> 2);
 #pragma unroll
     for (int e = 0; e < DK; ++e)
 #pragma unroll
@@ -302,49 +319,99 @@ __device__ __forceinline__ void ar_unit(ArWarp<D>& s, const ApWork& w, int i) {
   }
 }
 
-template <int D, bool HALF, bool QS>
-__global__ void __launch_bounds__(AR_WARPS * 32, ArCfg<D>::CTAS)
+// A query row's parts, by one warp.
+template <int D>
+__device__ __forceinline__ void ar_join(const AttnPrefixArgs& a, const float* rec, int item, int head, int lane) {
+  if (lane * 4 >= D) return;
+  const int n = a.plan.parts;
+  float m = -INFINITY, l = 0.f;
+  for (int s = 0; s < n; ++s) m = fmaxf(m, rec[s * (D + AP_PAD) + D]);
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s = 0; s < n; ++s) {
+    const float* part = rec + s * (D + AP_PAD);
+    const float2 ml = *reinterpret_cast<const float2*>(part + D);
+    if (ml.x == -INFINITY) continue;       // an empty part's sums count for nothing, whatever they are
+    const float f = exp2f(ml.x - m);
+    const float4 v = *reinterpret_cast<const float4*>(part + lane * 4);
+    l += ml.y * f;
+    sum.x += v.x * f; sum.y += v.y * f; sum.z += v.z * f; sum.w += v.w * f;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const bool none = l == 0.f || (a.item_skip && a.item_skip[item]);
+  sum = none ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+  ap_store4(a.out, ((size_t)item * a.n_heads + head) * D + lane * 4, sum, a.act_fmt);
+}
+
+template <int D, bool HALF, bool QS, bool GROUP>
+__global__ void __launch_bounds__((GROUP ? AP_GROUP_WARPS : AR_WARPS) * 32, GROUP ? 1 : ArCfg<D>::CTAS)
 attn_prefix_rows_kernel(AttnPrefixArgs a, long long n_units) {
   using C = ArCfg<D>;
+  constexpr int W = GROUP ? AP_GROUP_WARPS : AR_WARPS;
   pdl_launch_dependents();
   if (!a.beside) pdl_wait();
   extern __shared__ __align__(128) uint8_t ar_smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long stride = (long long)gridDim.x * AR_WARPS, first = (long long)warp * gridDim.x + blockIdx.x;
-  if (first >= n_units) {
+  const long long stride = GROUP ? W : (long long)gridDim.x * W, first = GROUP ? warp : (long long)warp * gridDim.x + blockIdx.x;
+  if (!GROUP && first >= n_units) {
     if (a.beside) pdl_wait();
     return;
   }
   const uint32_t base = smem_u32(ar_smem), ring = base + warp * C::WARP;
   constexpr int CH = D / 8;
   const int row = lane / CH, col = lane % CH;
-  ArWarp<D> s{a, first, stride, n_units, (int)((n_units - first + stride - 1) / stride), lane, ring, ring + C::STAGES * C::STAGE,
-              (uint32_t)((col >> 3) * C::BOX + row * 128 + (((col & 7) ^ (row & 7)) << 4))};
+  ArWarp<D, GROUP> s{a, first, stride, n_units, (int)((n_units - first + stride - 1) / stride), lane, ring, ring + C::STAGES * C::STAGE,
+                     (uint32_t)((col >> 3) * C::BOX + row * 128 + (((col & 7) ^ (row & 7)) << 4))};
   s.batch_of = -1;
   s.flight = s.put = s.get = s.ahead_i = 0;
-  ApWork w = s.unit(0);
-  s.look_at(w);
-  for (int i = 0; i < s.n; ++i) {
-    if (w.rows <= 4) ar_unit<D, HALF, QS, true>(s, w, i);
-    else ar_unit<D, HALF, QS, false>(s, w, i);
-    if (i + 1 < s.n) {
-      if (s.ahead_i == i) s.look_at(s.unit(++s.ahead_i));
-      w = s.ahead;
+  if constexpr (GROUP) {
+    s.g = (int)blockIdx.x / a.n_kv;
+    s.kvh = (int)blockIdx.x % a.n_kv;
+    const ApWork all = ap_work(a, (long long)blockIdx.x * a.plan.shared.splits, false);
+    s.item0 = all.item0;
+    s.items = max(all.rows, 0) / a.rep;
+    s.records = reinterpret_cast<float*>(ar_smem + W * C::WARP);
+  }
+  if (s.n > 0) {
+    ApWork w = s.unit(0);
+    s.look_at(w);
+    for (int i = 0; i < s.n; ++i) {
+      if (w.rows <= 4) ar_unit<D, HALF, QS, true>(s, w, i);
+      else ar_unit<D, HALF, QS, false>(s, w, i);
+      if (i + 1 < s.n) {
+        if (s.ahead_i == i) s.look_at(s.unit(++s.ahead_i));
+        w = s.ahead;
+      }
     }
   }
+  if constexpr (GROUP) {
+    __syncthreads();
+    for (int r = warp; r < s.items * a.rep; r += W)
+      ar_join<D>(a, s.records + r * a.plan.parts * (D + AP_PAD), s.item0 + r / a.rep, s.kvh * a.rep + r % a.rep, lane);
+  }
   if (a.beside) pdl_wait();      // this launch's end is the other's too
+}
+
+template <int D, bool HALF, bool QS, bool GROUP>
+int ar_start(const AttnPrefixArgs& a, long long ctas, long long units, size_t smem, cudaStream_t stream) {
+  static std::atomic<unsigned long long> done{0};
+  const auto kernel = attn_prefix_rows_kernel<D, HALF, QS, GROUP>;
+  const size_t most = GROUP ? AP_GROUP_WARPS * ArCfg<D>::WARP + 8 * AP_GROUP_WARPS * (D + AP_PAD) * 4 : smem;
+  const cudaError_t e = arcb_opt_in_smem(kernel, (int)most, done);
+  if (e != cudaSuccess) return (int)e;
+  const dim3 grid((unsigned)ctas), block((GROUP ? AP_GROUP_WARPS : AR_WARPS) * 32);
+  return (int)(a.beside ? ap_launch_beside(kernel, grid, block, smem, stream, a, units) : arcb_launch(kernel, grid, block, smem, stream, a, units));
 }
 
 template <int D, bool HALF, bool QS>
 int ar_launch(const AttnPrefixArgs& a, long long units, cudaStream_t stream) {
   using C = ArCfg<D>;
-  static std::atomic<unsigned long long> done{0};
-  const cudaError_t e = arcb_opt_in_smem(attn_prefix_rows_kernel<D, HALF, QS>, C::SMEM, done);
-  if (e != cudaSuccess) return (int)e;
+  if (a.plan.grouped) {
+    const long long tasks = a.plan.shared.splits + (long long)a.max_group * a.plan.own.splits;
+    const size_t records = (size_t)a.max_group * a.rep * a.plan.parts * (D + AP_PAD) * 4;
+    return ar_start<D, HALF, QS, true>(a, (long long)a.n_groups * a.n_kv, tasks, AP_GROUP_WARPS * C::WARP + records, stream);
+  }
   const long long most = (long long)C::CTAS * arcb_num_sms();
-  const dim3 grid((unsigned)(units < most ? units : most));
-  return (int)(a.beside ? ap_launch_beside(attn_prefix_rows_kernel<D, HALF, QS>, grid, dim3(AR_WARPS * 32), C::SMEM, stream, a, units)
-                        : arcb_launch(attn_prefix_rows_kernel<D, HALF, QS>, grid, dim3(AR_WARPS * 32), C::SMEM, stream, a, units));
+  return ar_start<D, HALF, QS, false>(a, units < most ? units : most, units, C::SMEM, stream);
 }
 }  // namespace
 

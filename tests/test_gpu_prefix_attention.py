@@ -157,6 +157,21 @@ def test_many_queries_over_a_long_prefix(form):
 
 
 @pytest.mark.parametrize("form", FORMS, ids=FORM_IDS)
+@pytest.mark.parametrize("sizes,prefix,own", [([2], [190], 17), ([1, 2, 1], [0, 31, 33], 64), ([7, 6], [64, 1], 3), ([4, 1, 3, 2], [256, 200, 0, 97], 40), ([2, 2], [0, 0], 5)])
+def test_few_items_over_a_short_prefix(form, sizes, prefix, own):
+    """As few samples of a short prompt are: groups of one CTA."""
+    for heads, kv, dim in ((4, 4, 64), (8, 8, 128), (2, 1, 128)):
+        c = Case(sizes, prefix, [(own - 3 * i) % (own + 1) for i in range(sum(sizes))], heads, kv, dim, form, own)
+        hints = dict(max_group=max(sizes), max_prefix=max(1, max(prefix)), max_own=own)
+        c.check(c(**hints))
+        assert torch.equal(c(**hints), c(**hints))
+        c.check(c(**dict(hints, max_prefix=1, max_own=1)))          # bounds that are too small: longer ranges
+        skip = torch.zeros(sum(sizes), dtype=torch.uint8, device="cuda")
+        skip[-1] = 1
+        c.check(c(skip=skip, **hints), skip=(sum(sizes) - 1,))
+
+
+@pytest.mark.parametrize("form", FORMS, ids=FORM_IDS)
 def test_draft_tokens_of_a_sequence(form):
     """Item j of a group sees the shared rows and j + 1 rows behind them, of the same sequence."""
     sizes, prefix = [5, 1, 4], [130, 64, 1]
