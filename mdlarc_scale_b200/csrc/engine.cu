@@ -639,6 +639,8 @@ extern "C" int arcb_session_fork(arcb_session* s, int32_t src, int32_t rows, con
   if (!s || (n_dst > 0 && !h_dst)) return arcb_fail(ARCB_E_ARG, "null argument");
   const int B = s->desc.n_seqs, T = s->desc.t_max;
   if (src < 0 || src >= B || n_dst < 0 || rows < 0 || rows > T) return arcb_fail(ARCB_E_ARG, "a fork names a sequence or rows outside the session");
+  // a row of a group holds its own rows alone, and the first one everybody's
+  if (!s->ls && s->desc.prefix_group > 1) return arcb_fail(ARCB_E_UNSUPPORTED, "no forks between rows that share a prompt");
   cudaStream_t stream = (cudaStream_t)stream_v;
   try {
     std::vector<int32_t> copies;

@@ -17,6 +17,7 @@ _I32, _U8 = torch.int32, torch.uint8
 _ARGS = struct.Struct("@13P2q10if3i")
 _SCRATCH, _SCRATCH_AT = struct.Struct("@Pq"), _lib.PrefixAttentionArgs.d_scratch.offset
 _raw_stream = torch._C._cuda_getCurrentRawStream      # the current stream's handle; torch.cuda.current_stream() takes 2 us
+_current_device = torch._C._cuda_getDevice             # of a process that has CUDA tensors: nothing is left to initialise
 
 
 def _refuse_index(name: str, n: int):
@@ -57,6 +58,8 @@ def prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, group_fi
         if q.stride(2) != 1 or (heads > 1 and q.stride(1) != dim):
             raise ValueError("an item's heads must be consecutive")
         pitch = q.stride(0) if n > 1 else 0
+        if pitch == 0 and n > 1:
+            raise ValueError("every item has queries of its own (broadcast ones: contiguous())")
     if out is None:
         out = q.new_empty((n, heads, dim)) if pitch else torch.empty_like(q)
     elif out.shape != q.shape or out.dtype != q.dtype or out.get_device() != dev or not out.is_contiguous():
@@ -88,7 +91,7 @@ def prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, group_fi
         a = _ARGS.pack(*fields)
     except (struct.error, OverflowError):
         raise ValueError("scale, max_group, max_prefix and max_own must be numbers of 32 bits") from None
-    if dev != torch.cuda.current_device():
+    if dev != _current_device():
         with torch.cuda.device(dev):
             _attend(a, out, dev)
     else:
@@ -132,7 +135,7 @@ def copy_cache_rows(cache: torch.Tensor, copies) -> None:
         raise ValueError("the cache is empty")
     args = (cache.data_ptr(), total // (seqs * heads * rows * dim), seqs, heads, rows, dim * cache.element_size(), m.ctypes.data, len(m), _raw_stream(dev))
     lib = _lib.load()
-    if dev != torch.cuda.current_device():
+    if dev != _current_device():
         with torch.cuda.device(dev):
             code = lib.arcb_op_cache_copy(*args)
     else:

@@ -349,6 +349,9 @@ def test_refusals():
     bad = [
         lambda: prefix_attention(c.q, c.k, c.v),                                             # nothing to attend
         lambda: prefix_attention(c.q[0], c.k, c.v, *g, *it),
+        lambda: prefix_attention(c.q[:1].expand(n, -1, -1), c.k, c.v, *g, *it),              # one item's queries for all
+        lambda: prefix_attention(c.q, c.k, c.v, *g, *it, max_own=2 ** 31),
+        lambda: prefix_attention(c.q, c.k, c.v, *g, *it, scale=1e39),
         lambda: prefix_attention(c.q, c.k, c.v[:, :, :-1], *g, *it),
         lambda: prefix_attention(c.q, c.k.transpose(0, 1), c.v.transpose(0, 1), *g, *it),
         lambda: prefix_attention(c.q, c.k.cpu(), c.v, *g, *it),

@@ -100,6 +100,10 @@ def test_refusals_of_shared_prompts():
         with pytest.raises(_lib.ArcbError):
             session.copy_rows(*args)
     session.close()
+    session = eng.new_session(4, 32, 4, 64, prefix_group=2)
+    with pytest.raises(_lib.ArcbError):
+        session.copy_rows(1, 3, [0])          # row 0 holds the prompt of both
+    session.close()
     eng.close()
 
 
