@@ -488,11 +488,12 @@ int arcb_op_decode_attention_static(const void* d_q16, const void* d_k, const vo
  * An item that sees no row, or is skipped, gets zeros.  No counterpart in the reference, whose samples of a prompt each keep
  * and read a copy of it (src/inference.py:794-827).
  *   formats: queries and outputs in act_format, cache in kv_format; the two are equal, or half over a bfloat16 cache.
- *   Scores, maxima and sums are 32 bits; heads of 64 or 128.
+ *   Scores, maxima and sums are 32 bits; heads of 64 or 128.  With half queries over a bfloat16 cache, keys that an item sees are
+ *   finite (a query is a sum of two pieces there); what no item sees may hold anything.
  *   Arrays start on 16 bytes.  max_* are upper bounds the work is laid out for (0: n_items, t_max, t_max); more items in a
  *   group than max_group is an error, longer rows only cost time.
  *   d_status (optional): set to ARCB_DEV_BAD_INDEX's value, 4, where a group or an item names rows outside the cache, or the
- *   groups do not cover the items one after the other; such rows count as not there. */
+ *   groups do not cover the items one after the other; such rows count as not there.  1 to 3: a wait inside a kernel ran out. */
 typedef struct arcb_prefix_attention_args {
   const void* d_q;               /* item i, head h: dim values at d_q + i * q_pitch + h * dim         */
   const void* d_k;               /* [n_seqs][n_kv][t_max][dim]                                        */

@@ -8,10 +8,14 @@
 //   warp 1        products of A and of B in turn: O += P V with P read from TMEM, then the next S = Q K^T (128 TMEM columns)
 //   warps 4-11    a thread a query row: maxima, exponentials, row sums, P over the row's own score columns.  (Two threads a row
 //                 had to exchange maxima in every tile and took twice the instructions.)
-// Maxima, sums and results are fp32.  The reference maximum of a row is raised only when it grows by 2^8.  Half queries over a
-// bfloat16 cache are two bfloat16 pieces (exact), and their weights too (2^-16 of a weight off).  In equal formats a weight is one
-// 16-bit value: its error, half a step, adds to an output that is rounded by as much itself (sqrt 2 of that error alone), and a
-// second piece costs half as many products again where products are what bounds the kernel.
+// Maxima, sums and results are fp32.  A row's reference maximum is raised only when the sum of a tile's weights against it passes
+// 2^12.  Half queries over a bfloat16 cache are two bfloat16 pieces (exact), and their weights too (2^-16 of a weight off).  In equal
+// formats a weight is one 16-bit value: its error, half a step, adds to an output that is rounded by as much itself (sqrt 2 of that
+// error alone), and a second piece costs half as many products again where products are what bounds the kernel.
+//
+// What bounds it: the chain of a tile (scores, exponentials, weights to TMEM, values, the next scores), of which two overlap.  1024
+// query rows x 32768 cached rows x 8 key heads of 128 in half (138 GFLOP): 166 us in the kernel, 0.83 PFLOP/s, the tensor pipe 49 % busy,
+// softmax warps two thirds of the time at work at 4.8 cycles an instruction.
 #include <type_traits>
 
 #include "attn_prefix_impl.cuh"
@@ -24,8 +28,13 @@ using namespace sm100;
 namespace {
 
 constexpr int AT_ROWS = 128, AT_KEYS = 128, AT_THREADS = 384;
-constexpr float AT_RESCALE = 8.f;          // log2 units
+constexpr float AT_RAISE = 4096.f;         // sum of 128 weights from which a row's reference maximum is raised
 constexpr int AT_BOX = 128 * 64 * 2;
+
+__device__ __forceinline__ void add2_f32(uint64_t& sum, float a, float b) {
+  asm("add.rn.f32x2 %0, %0, %1;" : "+l"(sum) : "l"(pack_f32x2(a, b)));
+}
+__device__ __forceinline__ void unpack_f32x2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
 
 template <int D, bool QS>
 struct AtCfg {
@@ -272,14 +281,17 @@ attn_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
           if (c * 32 + e >= seen) sv[e] = 0xff800000u;
       }
     };
-    auto most = [&](const uint32_t (&sv)[32], float mx) {
-      float m0 = mx, m1 = -INFINITY;
+    auto largest = [&](int seen) {
+      float mx = -INFINITY;
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        uint32_t sv[32];
+        tmem_ld_32x32(t_s + c * 32, sv);
+        arrived(c, seen, sv);
 #pragma unroll
-      for (int e = 0; e < 32; e += 4) {
-        m0 = max3_f32(m0, __uint_as_float(sv[e]), __uint_as_float(sv[e + 1]));
-        m1 = max3_f32(m1, __uint_as_float(sv[e + 2]), __uint_as_float(sv[e + 3]));
+        for (int e = 0; e < 32; e += 2) mx = max3_f32(mx, __uint_as_float(sv[e]), __uint_as_float(sv[e + 1]));
       }
-      return fmaxf(m0, m1);
+      return mx * sc;
     };
     for (int i = 0; i < n_x; ++i) {
       if (!__all_sync(0xffffffffu, mbar_wait_bounded(b_s + 8 * x, i & 1))) {
@@ -296,39 +308,26 @@ attn_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
       const int j = wide ? i : 2 * i + x;
       const int seen = j == n_tiles - 1 ? left : AT_KEYS;
       uint32_t pr[2][32], second[WP > 1 ? 2 : 1][WP > 1 ? 32 : 1];      // pairs of 64 keys each
+      if (i == 0) m_ref = largest(seen);
       float total;
-      if (i == 0) {
-        float mx = -INFINITY;
-#pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          uint32_t sv[32];
-          tmem_ld_32x32(t_s + c * 32, sv);
-          arrived(c, seen, sv);
-          mx = most(sv, mx);
-        }
-        m_ref = mx * sc;
-      }
-      // Weights against the reference as it is, and the scores' maximum on the way.  Nearly always the reference stays; where it
-      // has to be raised, the scores are still there for a second time.
-      for (;;) {
+      // weights against the reference as it is
+      auto weights = [&]() {
         const float m_safe = m_ref == -INFINITY ? 0.f : m_ref;
         const uint64_t nm2 = pack_f32x2(-m_safe, -m_safe);
-        float sum[4] = {0.f, 0.f, 0.f, 0.f}, mx = -INFINITY;
+        uint64_t sum[2] = {0, 0};
         uint32_t sv[2][32];
         tmem_ld_32x32(t_s, sv[0]);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           arrived(c, seen, sv[c & 1]);
           if (c < 3) tmem_ld_32x32(t_s + (c + 1) * 32, sv[(c + 1) & 1]);      // while these are at work
-          mx = most(sv[c & 1], mx);
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             float t0, t1;
             shift2_f32(sv[c & 1][2 * e], sv[c & 1][2 * e + 1], sc2, nm2, t0, t1);
             t0 = ex2_fast(t0);
             t1 = ex2_fast(t1);
-            sum[2 * (e & 1)] += t0;
-            sum[2 * (e & 1) + 1] += t1;
+            add2_f32(sum[e & 1], t0, t1);
             const uint32_t h = pack2_prob(t0, t1, HALF ? 1 : 0);
             pr[c >> 1][(c & 1) * 16 + e] = h;
             if constexpr (WP > 1) {
@@ -337,10 +336,17 @@ attn_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
             }
           }
         }
-        total = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        mx *= sc;
-        const bool raise = mx > m_ref + AT_RESCALE;
-        if (!__any_sync(0xffffffffu, raise)) break;
+        float s0, s1, s2, s3;
+        unpack_f32x2(sum[0], s0, s1);
+        unpack_f32x2(sum[1], s2, s3);
+        total = (s0 + s1) + (s2 + s3);
+      };
+      weights();
+      // Nearly always the reference stays: maxima are looked for only where the weights' sum says that they have grown (they took a tenth
+      // of the instructions).  The scores are still there.
+      const bool raise = i > 0 && (total > AT_RAISE || m_ref == -INFINITY);
+      if (__any_sync(0xffffffffu, raise)) {
+        const float mx = largest(seen);
         float alpha = 1.f;
         if (raise) {
           alpha = m_ref == -INFINITY ? 0.f : ex2_fast(m_ref - mx);
@@ -348,16 +354,16 @@ attn_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
           l *= alpha;
         }
         // these scores were asked for behind the last product of values: its sums are complete
-        if (i > 0)
 #pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld_32x32(t_o + c * 32, o);
-            tmem_wait_ld_dep(o);
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld_32x32(t_o + c * 32, o);
+          tmem_wait_ld_dep(o);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-            tmem_st_32x32(t_o + c * 32, o);
-          }
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+          tmem_st_32x32(t_o + c * 32, o);
+        }
+        weights();
       }
       l += total;
       // over scores that have all been read

@@ -38,7 +38,9 @@ def prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, group_fi
     of its own.  Indices are int32 tensors on the device, read when the kernels run.  ``skip`` (uint8) marks items that get
     zeros, as those that see no row do.  The ``max_*`` are upper bounds of what the tensors hold and only plan the work, but
     ``max_group``: no group may have more items.  ``status`` (int32, one value) becomes non-zero when an index is outside the
-    cache.  The queries may be rows of a wider matrix; all else is contiguous.  Runs on the current stream."""
+    cache.  Keys that an item sees are finite where half queries meet a bfloat16 cache (a query is a sum of two pieces there,
+    which an infinity would turn into no number); what no item sees may hold anything.  The queries may be rows of a wider
+    matrix; all else is contiguous.  Runs on the current stream."""
     if q.dim() != 3 or k.dim() != 4 or k.shape != v.shape:
         raise ValueError("queries are [items, heads, dim], keys and values [sequences, kv_heads, rows, dim]")
     n, heads, dim = q.shape

@@ -172,6 +172,37 @@ def test_few_items_over_a_short_prefix(form, sizes, prefix, own):
 
 
 @pytest.mark.parametrize("form", FORMS, ids=FORM_IDS)
+@pytest.mark.parametrize("items", [2, 5, 33, 140])
+def test_scores_that_grow_along_the_rows(form, items):
+    """Maxima that have to be raised again and again, and ones that never are."""
+    for dim in (64, 128):
+        for ramp in ((0.05, 8.0), (8.0, 0.05)):
+            c = Case([items], [1600], [i % 3 for i in range(items)], 4, 2, dim, form, items, own_in_group=True, rows=4144)
+            c.k *= torch.linspace(*ramp, 4144, device="cuda").to(c.k.dtype)[None, None, :, None]
+            c.check(c())
+
+
+@pytest.mark.parametrize("form", FORMS[1:], ids=FORM_IDS[1:])
+@pytest.mark.parametrize("items", [2, 33, 140])
+def test_rows_whose_scores_are_infinite(form, items):
+    """Keys of minus infinity under queries that are not negative: scores of minus infinity, weights of 0, as if the rows were not there.
+    Half queries over bfloat16 keys are no case of it: a query is hi + lo there, lo is 0 or of either sign, and 0 times an infinity, like
+    the sum of two that differ in sign, is no number."""
+    gone = 260
+    for dim in (64, 128):
+        c = Case([items], [900], [0] * items, 4, 2, dim, form, items, own_in_group=True, rows=4144)
+        c.q = c.q.abs() + 0.01
+        seq = c.group_seq[0]
+        c.k[seq, :, :gone] = -math.inf
+        out = c()
+        assert bool(torch.isfinite(out).all())
+        c.k = c.k[:, :, gone:].contiguous()
+        c.v = c.v[:, :, gone:].contiguous()
+        c.prefix = [900 - gone]
+        c.check(out)
+
+
+@pytest.mark.parametrize("form", FORMS, ids=FORM_IDS)
 def test_draft_tokens_of_a_sequence(form):
     """Item j of a group sees the shared rows and j + 1 rows behind them, of the same sequence."""
     sizes, prefix = [5, 1, 4], [130, 64, 1]
