@@ -173,7 +173,8 @@ int arcb_launch_attn_prefix(AttnPrefixArgs a, cudaStream_t stream) {
     r = launch_part(a, p.own, p.own.units, stream);
   }
   if (r || p.parts == 1 || p.grouped) return r;
-  // Its CTAs come while the last ones of the parts are at work, and wait.  Four warps a result where a warp each would leave SMs without work
+  // Its CTAs come while the last ones of the parts are at work, and wait.  Four warps a result where a warp each would leave SMs without
+  // work (two samples in four parts: 9.3 us in all with a warp each, 7.7 with four).
   const bool few = joins < 4LL * arcb_num_sms();
   arcb_count_launch(1);
   return (int)(few ? ap_launch_beside(attn_prefix_join_cta_kernel, dim3((unsigned)((long long)a.n_items * a.n_heads)), dim3(128), 0, stream, a)

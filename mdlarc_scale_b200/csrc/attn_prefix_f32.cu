@@ -4,9 +4,9 @@
 // has RPT query rows x KPT keys of the scores, and of the results the same rows x D / TX columns.  Operands come from shared memory
 // 16 bytes at a time, 8 x 4 of a thread's scores for 12 such loads (16 of the memory's cycles beside 128 multiply-adds a warp), so
 // that the multiply-adds are what counts from 32 query rows on; below, with 4 x 2, the memory is (159 rows over 490 shared ones, 22
-// groups x 32 heads of 128: 557 us, 34 TFLOP/s of the about 74 that the units have).  Tiles come by cp.async: the
-// next keys while these values are at work, the next values while the next scores are.  Rows of 16-byte pieces are exclusive-or
-// swizzled.  Maxima, sums and results are fp32, and so is every operand: weights are not rounded.
+// groups x 32 heads of 128: 557 us, 34 TFLOP/s of the about 74 that the units have; 24 rows over 1501, 15 heads of 64: 11 us).  Tiles
+// come by cp.async: the next keys while these values are at work, the next values while the next scores are.  Rows of 16-byte
+// pieces are exclusive-or swizzled.  Maxima, sums and results are fp32, and so is every operand: weights are not rounded.
 #include "../../include/arcb200.h"
 #include "attn_prefix_impl.cuh"
 #include "launch.cuh"
@@ -196,8 +196,8 @@ attn_prefix_f32_kernel(AttnPrefixArgs a) {
 
 // Up to R query rows: a warp a unit, without shared memory.  Eight lanes have a cached row (16 or 8 of its values each), so that a
 // score takes three exchanges, and four rows are at work beside each other, each with a running maximum and sums of its own, which
-// are put together at the end.  Bound by the cache's rows; a CTA of 64 of them spent its time on rows that short parts do not have
-// (own rows of 3498 items x 32 heads, six at most, beside 490 shared ones: 2335 us).
+// are put together at the end.  Bound by the cache's rows: 16 x 20 items of 1000 rows of 64 with 3000 shared ones, 71 us, 5.7 TB/s.  (A
+// CTA of 64 keys spent its time on rows that short parts do not have: 3498 items x 32 heads of six rows at most 1.4 ms, now 0.18.)
 // U: cached rows under way, of every four.
 template <int D, int R, int U>
 __global__ void __launch_bounds__(128, U > 1 ? 2 : R == 4 ? 3 : 4)

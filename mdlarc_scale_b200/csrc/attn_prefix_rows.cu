@@ -12,7 +12,8 @@
 // The products are transposed, so that the eight columns of m16n8k16 are queries: S^T = K Q^T (16 keys a product) and O^T += V^T P^T
 // (16 value columns a product); weights change from the first one's result to the second one's operand by 8 x 8 transpositions
 // in the warp.  These products are slow here, 14 cycles each, and with 16 queries a product most of them would be padding.  What
-// bounds it is reading the cache.
+// bounds it is reading the cache: 64 x 20 groups of eight queries over 1193 shared rows and 300 of each one's own, heads of 64 (647 MB):
+// 121 us, 5.3 TB/s, the join of the parts 6 more.
 //
 // Rounding: a weight enters the product as two 16-bit pieces (p = hi + lo), since one piece alone would be as far off as the
 // output's own rounding; half queries over a bfloat16 cache are two bfloat16 pieces, which is exact.  With up to four query rows the

@@ -40,7 +40,8 @@ __device__ __forceinline__ CopyPlace cc_place(const CopyArgs<STEPS>& a, unsigned
 }
 
 // Programs of one source: four places a thread in a turn, the next turn's rows on their way while this one's are written.  (A CTA a
-// turn spent most of its time starting: 77 sequences moved in 475 us, 5.5 TB/s, or 775 us with the registers of the other kernel.)
+// turn spent most of its time starting: 77 sequences moved in 475 us,
+// now 436, 6.0 TB/s; 775 with the registers of the other kernel.)
 template <int STEPS, typename VEC>
 __global__ void __launch_bounds__(CC_THREADS)
 cache_spread_kernel(const __grid_constant__ CopyArgs<STEPS> a) {
