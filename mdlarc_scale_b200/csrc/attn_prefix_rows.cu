@@ -331,10 +331,10 @@ __device__ __forceinline__ void ar_join(const AttnPrefixArgs& a, const float* re
   for (int s = 0; s < n; ++s) {
     const float* part = rec + s * (D + AP_PAD);
     const float2 ml = *reinterpret_cast<const float2*>(part + D);
+    const float f = exp2f(ml.x - (m == -INFINITY ? 0.f : m));
+    l += ml.y * f;                         // scores that are no numbers leave no maximum, but no number as their sum
     if (ml.x == -INFINITY) continue;       // an empty part's sums count for nothing, whatever they are
-    const float f = exp2f(ml.x - m);
     const float4 v = *reinterpret_cast<const float4*>(part + lane * 4);
-    l += ml.y * f;
     sum.x += v.x * f; sum.y += v.y * f; sum.z += v.z * f; sum.w += v.w * f;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;

@@ -343,6 +343,58 @@ def test_offsets_beyond_32_bits():
     c.check(c(max_group=20))
 
 
+@pytest.mark.parametrize("form,items", [(F32, 20), (F32, 2), (BF16, 80), (F16, 3)])
+def test_offsets_beyond_32_bits_of_other_kernels(form, items):
+    rows, seqs = 40_016, 900
+    k, v = (torch.zeros((seqs, 1, rows, 64), device="cuda", dtype=form) for _ in range(2))
+    c = Case([items], [rows], [i % 7 for i in range(items)], 2, 1, 64, (form, form), 3, own_in_group=True, rows=rows + 8)
+    for big, small_one in ((k, c.k), (v, c.v)):
+        big[seqs - 1].copy_(small_one[0, :, :rows])
+    own = [min(o, rows) for o in c.own]
+    c.begin = [rows - o for o in own]
+    c.own, c.k, c.v, c.group_seq, c.item_seq = own, k, v, [seqs - 1], [seqs - 1] * items
+    ints = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")      # noqa: E731
+    c.groups, c.items = (ints([0, items]), ints(c.group_seq), ints([rows])), (ints(c.item_seq), ints(c.begin), ints([rows] * items))
+    c.check(c(max_own=7))
+
+
+@pytest.mark.parametrize("form", FORMS, ids=FORM_IDS)
+@pytest.mark.parametrize("items,heads,kv", [(2, 2, 2), (5, 4, 2), (33, 2, 1), (140, 2, 1)])
+def test_nan_in_a_query_of_any_size_of_group(form, items, heads, kv):
+    for dim in (64, 128):
+        c = Case([items], [700], [i % 9 for i in range(items)], heads, kv, dim, form, items, own_in_group=True, rows=4144)
+        for hints in ({}, dict(max_group=items, max_prefix=300, max_own=9)):
+            want = c(**hints)
+            q = c.q.clone()
+            q[items - 1, 1] = math.nan
+            out = prefix_attention(q, c.k, c.v, *c.groups, *c.items, **hints)
+            assert bool(torch.isnan(out[items - 1, 1]).all())
+            out[items - 1, 1] = want[items - 1, 1]
+            assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("form", FORMS, ids=FORM_IDS)
+@pytest.mark.parametrize("sizes,heads,kv", [([3, 2], 2, 2), ([5, 2], 16, 2), ([40, 3], 4, 2)])
+def test_bad_indices_in_any_size_of_group(form, sizes, heads, kv):
+    c = Case(sizes, [140, 130], [1 + i % 9 for i in range(sum(sizes))], heads, kv, 64, form, 29)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    hints = dict(max_group=max(sizes), max_prefix=140, max_own=9)
+    want, first = c(status=status, **hints), sizes[0]
+    assert status.item() == 0
+    for what, i, value in (("groups", 1, 99), ("groups", 1, -1), ("groups", 2, 10 ** 6), ("groups", 2, -3), ("groups", 0, 2), ("groups", 0, -2 ** 31), ("items", 0, 500),
+                           ("items", 0, -2 ** 31), ("items", 1, -2), ("items", 2, 2 ** 31 - 1)):
+        t = getattr(c, what)[i]
+        old = t[0].clone()
+        t[0] = value
+        status.zero_()
+        out = c(status=status, **hints)
+        assert status.item() == 4, (what, i, value)
+        t[0] = old
+        assert torch.equal(out[first:], want[first:])
+    status.zero_()
+    assert torch.equal(c(status=status, **hints), want) and status.item() == 0
+
+
 def test_nan_in_a_query_stays_in_its_item():
     c = small((F16, F16), 4, 2, 64, 22)
     c.q[2, 1] = math.nan
