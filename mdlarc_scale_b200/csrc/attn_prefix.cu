@@ -122,11 +122,11 @@ attn_prefix_join_cta_kernel(AttnPrefixArgs a) {
 
 void fill_plan(AttnPrefixArgs& a) {
   a.rep = a.n_heads / a.n_kv;
-  // tcgen05 from 512 shared rows on (64 queries of 4 heads: 59.1 us against 61.3 at 384 rows, 65.5 against 77.4 at 1024; 12 of 16 heads
-  // over one: 25 against 19 at 160); half queries over bfloat16, whose products are three, from 4096 on (128 rows: 66 us without and 71
-  // with it at 1500, 300 and 251 at 19327).
+  // tcgen05 from 512 shared rows on (64 queries of 4 heads, 8 groups: 60.2 us with it and 58.4 without at 384 rows, 63.8 and 70.7 at 1024;
+  // 24 queries 26.0 and 28.4 at 600); half queries over bfloat16, whose products are three, from 2048 on (128 query rows: 72 us and 66 at
+  // 1500, 77.5 and 86.6 at 3000).
   const bool split = a.act_fmt != a.kv_fmt;
-  const bool tc = a.kv_fmt != 2 && (!split || a.dim == 64) && a.scale != 0.f && a.max_prefix >= (split ? 4096 : 512);
+  const bool tc = a.kv_fmt != 2 && (!split || a.dim == 64) && a.scale != 0.f && a.max_prefix >= (split ? 2048 : 512);
   a.plan = prefix_plan(a.n_groups, a.max_group, a.max_prefix, a.n_items, a.item_end ? a.max_own : 0, a.n_kv, a.rep, a.dim, a.kv_fmt == 2, tc, arcb_num_sms());
 }
 
