@@ -4,16 +4,16 @@
 // swizzled by the row, so that the eight rows of a matrix load fall into different banks).  S = Q K^T and O += P V are
 // m16n8k16 products with fp32 sums; queries, sums and weights stay in registers (the sums of two neighbouring score tiles are
 // the weights' operand as they lie).  With 16, 32 or 64 query rows the warps divide the tile's keys among 4, 2 or 1 groups and
-// the rows among 1, 2 or 4; groups are merged once at the end.  What bounds it is reading the cache: 16 query rows cost
-// 16 keys x 128 dims x 2 products of 128 cycles beside 8 KB that an SM receives in 190; padding to 32 query rows takes as long as
-// the reading.  20 query rows over 4096 cached rows, 24 sequences x 8 key heads of 128 (267 MB): 69 us with the start, own rows and
-// join, 3.9 TB/s; 16 over 7500, 20 heads of 64: 19 us with the own rows running beside it.
+// the rows among 1, 2 or 4; groups are merged once at the end.  What bounds it is reading the cache with up to 16 query rows: they cost
+// 16 keys x 128 dims x 3 products of 128 cycles beside 8 KB that an SM receives in 190; 16 over 7500, 20 heads of 64: 19 us with the own
+// rows running beside it.  From 17 on products count, those of padding to 32 or 64 rows among them: 20 query rows over 4096 cached
+// rows, 24 sequences x 8 key heads of 128 (267 MB): 79 us with the start, own rows and join, 3.4 TB/s.
 //
-// Rounding: with up to 16 query rows, where reading the cache hides it, and with half queries over a bfloat16 cache weights enter
-// the product as two 16-bit pieces (p = hi + lo, 2^-16 of p off with bfloat16).  Elsewhere they are one, whose error, half a step, adds
-// to an output that is rounded by as much itself (sqrt 2 of that error alone): a second one took 76 us in place of 69 above, and
-// 195 in place of 171 with 64 query rows over 2000, 64 groups.  Half queries over a bfloat16 cache are two bfloat16 pieces, which is
-// exact.  Maxima, sums and all partial results are fp32; a range's reference maximum is raised only when it grows by 2^8.
+// Rounding: weights enter the product as two 16-bit pieces (p = hi + lo, half a step of the type squared of p off).  One piece is half
+// a step of a weight off, which adds up to half a step of sum p |v|: more than the output's own rounding without limit where
+// values cancel, and 1.4 times its error on random ones; it took 70 us in place of the 79 above.  Half queries over a bfloat16 cache
+// are two bfloat16 pieces, which is exact.  Maxima, sums and all partial results are fp32; a range's reference maximum is raised
+// only when it grows by 2^8.
 #include <type_traits>
 
 #include "attn_prefix_frag.cuh"
@@ -41,7 +41,6 @@ __device__ __forceinline__ void am_body(const AttnPrefixArgs& a, const ApWork& w
   constexpr int RG = 4 / KG;
   constexpr int KW = AM_KEYS / KG;         // keys of a tile that a warp has
   constexpr int NT = KW / 8, DK = D / 16, CH = D / 8;
-  constexpr int WP = QS || KG == 4 ? 2 : 1;      // 16-bit pieces of a weight
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rg = warp / KG, kg = warp % KG;
   const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
@@ -178,13 +177,9 @@ __device__ __forceinline__ void am_body(const AttnPrefixArgs& a, const ApWork& w
       }
 #pragma unroll
     for (int kk = 0; kk < KW / 16; ++kk) {
-      uint32_t hi[4], lo[WP > 1 ? 4 : 1];
+      uint32_t hi[4], lo[4];
 #pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        const float p0 = s[2 * kk + (y >> 1)][2 * (y & 1)], p1 = s[2 * kk + (y >> 1)][2 * (y & 1) + 1];
-        if constexpr (WP > 1) am_split<HALF>(p0, p1, hi[y], lo[y]);
-        else hi[y] = pack2_prob(p0, p1, HALF ? 1 : 0);
-      }
+      for (int y = 0; y < 4; ++y) am_split<HALF>(s[2 * kk + (y >> 1)][2 * (y & 1)], s[2 * kk + (y >> 1)][2 * (y & 1) + 1], hi[y], lo[y]);
       const int r = kg * KW + kk * 16 + (lane & 15);
 #pragma unroll
       for (int dt = 0; dt < DK; ++dt) {
@@ -192,10 +187,8 @@ __device__ __forceinline__ void am_body(const AttnPrefixArgs& a, const ApWork& w
         am_ld4t(vst + r * (CH * 16) + (((2 * dt + (lane >> 4)) ^ (r & 7)) << 4), b);
         am_mma<HALF>(acc[2 * dt], hi, b[0], b[1]);
         am_mma<HALF>(acc[2 * dt + 1], hi, b[2], b[3]);
-        if constexpr (WP > 1) {
-          am_mma<HALF>(acc[2 * dt], lo, b[0], b[1]);
-          am_mma<HALF>(acc[2 * dt + 1], lo, b[2], b[3]);
-        }
+        am_mma<HALF>(acc[2 * dt], lo, b[0], b[1]);
+        am_mma<HALF>(acc[2 * dt + 1], lo, b[2], b[3]);
       }
     }
   }

@@ -9,13 +9,12 @@
 //   warps 4-11    a thread a query row: maxima, exponentials, row sums, P over the row's own score columns.  (Two threads a row
 //                 had to exchange maxima in every tile and took twice the instructions.)
 // Maxima, sums and results are fp32.  A row's reference maximum is raised only when the sum of a tile's weights against it passes
-// 2^12.  Half queries over a bfloat16 cache are two bfloat16 pieces (exact), and their weights too (2^-16 of a weight off).  In equal
-// formats a weight is one 16-bit value: its error, half a step, adds to an output that is rounded by as much itself (sqrt 2 of that
-// error alone), and a second piece costs half as many products again where products are what bounds the kernel.
+// 2^12.  Half queries over a bfloat16 cache are two bfloat16 pieces (exact).  Weights are two 16-bit pieces in every format (half a
+// step of the type squared of a weight off): one is half a step off, which adds up to half a step of sum p |v|, more than the output's
+// own rounding without limit where values cancel, and 1.4 times its error on random ones (200 us in place of the 256 below).
 //
 // What bounds it: the chain of a tile (scores, exponentials, weights to TMEM, values, the next scores), of which two overlap.  1024
-// query rows x 32768 cached rows x 8 key heads of 128 in half (138 GFLOP): 166 us in the kernel, 0.83 PFLOP/s, the tensor pipe 49 % busy,
-// softmax warps two thirds of the time at work at 4.8 cycles an instruction.
+// query rows x 32768 cached rows x 8 key heads of 128 in half (138 GFLOP, 206 with the second pieces): 256 us with own rows and join.
 #include <type_traits>
 
 #include "attn_prefix_impl.cuh"
@@ -52,8 +51,7 @@ struct AtCfg {
 };
 
 // HALF: the cache's format.  QS: half queries over a bfloat16 cache.
-// WP: 16-bit pieces of a weight.
-template <int D, bool HALF, bool QS, int WP>
+template <int D, bool HALF, bool QS>
 __global__ void __launch_bounds__(AT_THREADS, 1)
 attn_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v, AttnPrefixArgs a, uint32_t idesc_qk,
                       uint32_t idesc_pv) {
@@ -235,7 +233,7 @@ attn_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
         if (i > 0) {
           const uint64_t dv = umma_desc_mn_sw128(v_smem + s1 * C::KV_BYTES, AT_BOX);
 #pragma unroll
-          for (int piece = 0; piece < WP; ++piece)
+          for (int piece = 0; piece < 2; ++piece)
 #pragma unroll
             for (int ks = 0; ks < AT_KEYS / 16; ++ks)
               umma_f16_ts_if(el, t_o, t_s + piece * 64 + ks * 8, dv + (uint64_t)(ks * (2048 >> 4)), idesc_pv, (i > 1 || piece || ks) ? 1u : 0u);
@@ -307,7 +305,7 @@ attn_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
       }
       const int j = wide ? i : 2 * i + x;
       const int seen = j == n_tiles - 1 ? left : AT_KEYS;
-      uint32_t pr[2][32], second[WP > 1 ? 2 : 1][WP > 1 ? 32 : 1];      // pairs of 64 keys each
+      uint32_t pr[2][32], second[2][32];      // pairs of 64 keys each
       if (i == 0) m_ref = largest(seen);
       float total;
       // weights against the reference as it is
@@ -330,10 +328,8 @@ attn_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
             add2_f32(sum[e & 1], t0, t1);
             const uint32_t h = pack2_prob(t0, t1, HALF ? 1 : 0);
             pr[c >> 1][(c & 1) * 16 + e] = h;
-            if constexpr (WP > 1) {
-              const float2 f = unpack2_act(h, HALF ? 1 : 0);
-              second[c >> 1][(c & 1) * 16 + e] = pack2_prob(t0 - f.x, t1 - f.y, HALF ? 1 : 0);
-            }
+            const float2 f = unpack2_act(h, HALF ? 1 : 0);
+            second[c >> 1][(c & 1) * 16 + e] = pack2_prob(t0 - f.x, t1 - f.y, HALF ? 1 : 0);
           }
         }
         float s0, s1, s2, s3;
@@ -370,7 +366,7 @@ attn_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         tmem_st_32x32(t_s + c * 32, pr[c]);
-        if constexpr (WP > 1) tmem_st_32x32(t_s + 64 + c * 32, second[c]);
+        tmem_st_32x32(t_s + 64 + c * 32, second[c]);
       }
       tmem_wait_st();
       tc_fence_before();
@@ -461,11 +457,11 @@ attn_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
   }
 }
 
-template <int D, bool HALF, bool QS, int WP>
+template <int D, bool HALF, bool QS>
 int at_launch(const AttnPrefixArgs& a, unsigned blocks, cudaStream_t stream) {
   using C = AtCfg<D, QS>;
   static std::atomic<unsigned long long> done{0};
-  cudaError_t e = arcb_opt_in_smem(attn_prefix_tc_kernel<D, HALF, QS, WP>, C::SMEM, done);
+  cudaError_t e = arcb_opt_in_smem(attn_prefix_tc_kernel<D, HALF, QS>, C::SMEM, done);
   if (e != cudaSuccess) return (int)e;
   CUtensorMap tk, tv;
   const uint64_t rows = (uint64_t)a.n_seqs * a.n_kv * a.t_max;
@@ -475,13 +471,13 @@ int at_launch(const AttnPrefixArgs& a, unsigned blocks, cudaStream_t stream) {
   const int fmt = HALF ? 0 : 1;
   const uint32_t idesc_qk = umma_idesc_f16(AT_ROWS, AT_KEYS, fmt, fmt, 0, 0);
   const uint32_t idesc_pv = umma_idesc_f16(AT_ROWS, D, fmt, fmt, 0, 1);      // values are MN-major
-  return (int)arcb_launch(attn_prefix_tc_kernel<D, HALF, QS, WP>, dim3(blocks), dim3(AT_THREADS), C::SMEM, stream, tk, tv, a, idesc_qk, idesc_pv);
+  return (int)arcb_launch(attn_prefix_tc_kernel<D, HALF, QS>, dim3(blocks), dim3(AT_THREADS), C::SMEM, stream, tk, tv, a, idesc_qk, idesc_pv);
 }
 
 }  // namespace
 
 int arcb_attn_prefix_tc(const AttnPrefixArgs& a, long long units, cudaStream_t stream) {
-  if (a.kv_fmt == 1) return a.dim == 64 ? at_launch<64, true, false, 1>(a, (unsigned)units, stream) : at_launch<128, true, false, 1>(a, (unsigned)units, stream);
-  if (a.act_fmt == 1) return a.dim == 64 ? at_launch<64, false, true, 2>(a, (unsigned)units, stream) : -1;
-  return a.dim == 64 ? at_launch<64, false, false, 1>(a, (unsigned)units, stream) : at_launch<128, false, false, 1>(a, (unsigned)units, stream);
+  if (a.kv_fmt == 1) return a.dim == 64 ? at_launch<64, true, false>(a, (unsigned)units, stream) : at_launch<128, true, false>(a, (unsigned)units, stream);
+  if (a.act_fmt == 1) return a.dim == 64 ? at_launch<64, false, true>(a, (unsigned)units, stream) : -1;
+  return a.dim == 64 ? at_launch<64, false, false>(a, (unsigned)units, stream) : at_launch<128, false, false>(a, (unsigned)units, stream);
 }
