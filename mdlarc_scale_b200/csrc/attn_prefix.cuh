@@ -33,7 +33,7 @@ struct AttnPrefixArgs {
   int beside;                 // the launch runs beside the one ahead of it, whose end it waits for at its own
 };
 
-constexpr int AP_PAD = 4;     // of a partial result: the sums of a row's values, its maximum (log2 units), its sum, two spare
+constexpr int AP_PAD = 4;     // of a partial result: the sums of a row's values, the reference of its weights (log2 units), their sum, two spare
 
 // 16-bit formats; `a` as the launcher has filled it, units from a.first_block on.  Warps for up to 8 query rows
 // (attn_prefix_rows.cu), CTAs for up to 64 (attn_prefix_mma.cu), or 256 with tcgen05 (attn_prefix_tc.cu).

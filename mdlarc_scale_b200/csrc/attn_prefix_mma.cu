@@ -12,8 +12,9 @@
 // Rounding: weights enter the product as two 16-bit pieces (p = hi + lo, half a step of the type squared of p off).  One piece is half
 // a step of a weight off, which adds up to half a step of sum p |v|: more than the output's own rounding without limit where
 // values cancel, and 1.4 times its error on random ones; it took 70 us in place of the 79 above.  Half queries over a bfloat16 cache
-// are two bfloat16 pieces, which is exact.  Maxima, sums and all partial results are fp32; a range's reference maximum is raised
-// only when it grows by 2^8.
+// are two bfloat16 pieces, which is exact.  Maxima, sums and all partial results are fp32.  A range's reference is raised only when
+// its maximum grows by 2^8; in half it is 2^7 below the maximum, so that weights are up to 2^15 and end at 2^-24 of it: weights down
+// to 2^-32 of a range's largest one count.
 #include <type_traits>
 
 #include "attn_prefix_frag.cuh"
@@ -23,7 +24,7 @@
 namespace {
 
 constexpr int AM_KEYS = 64;
-constexpr float AM_RESCALE = 8.f;      // log2 units
+constexpr float AM_RESCALE = 8.f, AM_BELOW = 7.f;      // log2 units
 
 template <int D>
 struct AmCfg {
@@ -39,6 +40,7 @@ template <int D, bool HALF, bool QS, int KG>
 __device__ __forceinline__ void am_body(const AttnPrefixArgs& a, const ApWork& w, uint8_t* smem) {
   using C = AmCfg<D>;
   constexpr int RG = 4 / KG;
+  constexpr float BELOW = HALF ? AM_BELOW : 0.f;
   constexpr int KW = AM_KEYS / KG;         // keys of a tile that a warp has
   constexpr int NT = KW / 8, DK = D / 16, CH = D / 8;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -145,7 +147,7 @@ __device__ __forceinline__ void am_body(const AttnPrefixArgs& a, const ApWork& w
       for (int n = 1; n < NT; ++n) mx = max3_f32(mx, s[n][2 * x], s[n][2 * x + 1]);
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      mx = mx == -INFINITY ? -INFINITY : mx * sc;
+      mx = mx == -INFINITY ? -INFINITY : fmaf(mx, sc, -BELOW);
       if (mx > m[x] + AM_RESCALE || (m[x] == -INFINITY && mx > -INFINITY)) {
         const float alpha = m[x] == -INFINITY ? 0.f : ex2_fast(m[x] - mx);
         raise = true;

@@ -17,8 +17,9 @@
 //
 // Rounding: a weight enters the product as two 16-bit pieces (p = hi + lo), since one piece alone would be as far off as the
 // output's own rounding; half queries over a bfloat16 cache are two bfloat16 pieces, which is exact.  With up to four query rows the
-// weights' pieces are columns of their own and cost nothing.  Maxima, sums and all partial results are fp32; a range's reference
-// maximum is raised only when it grows by 2^8.
+// weights' pieces are columns of their own and cost nothing.  Maxima, sums and all partial results are fp32.  A range's reference
+// is raised only when its maximum grows by 2^8; in half it is 2^7 below the maximum, so that weights are up to 2^15 and end at 2^-24
+// of it: weights down to 2^-32 of a range's largest one count.
 #include "attn_prefix_frag.cuh"
 #include "flash_common.cuh"
 #include "gemm.cuh"
@@ -28,7 +29,7 @@ using namespace sm100;
 
 namespace {
 
-constexpr float AR_RESCALE = 8.f;      // log2 units
+constexpr float AR_RESCALE = 8.f, AR_BELOW = 7.f;      // log2 units
 constexpr int AR_WARPS = 4;      // of a CTA; AP_GROUP_WARPS of one that takes a group
 
 template <int D>
@@ -162,6 +163,7 @@ template <int D, bool HALF, bool QS, bool PAIR, bool GROUP>
 __device__ __forceinline__ void ar_unit(ArWarp<D, GROUP>& s, const ApWork& w, int i) {
   using C = ArCfg<D>;
   constexpr int DK = D / 16, MT = C::KEYS / 16;
+  constexpr float BELOW = HALF ? AR_BELOW : 0.f;
   const AttnPrefixArgs& a = s.a;
   const int lane = s.lane;
   // A negative scale turns the queries, so that maxima are maxima; one of 0 makes them 0, since 0 times -inf is no score.
@@ -244,7 +246,7 @@ __device__ __forceinline__ void ar_unit(ArWarp<D, GROUP>& s, const ApWork& w, in
 #pragma unroll
       for (int mt = 1; mt < MT; ++mt) mx = max3_f32(mx, p[mt][x], p[mt][2 + x]);
       top[x] = mx;
-      raise |= mx * sc > m[x] + AR_RESCALE;
+      raise |= mx * sc > m[x] + (AR_RESCALE + BELOW);
     }
     if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
@@ -253,7 +255,7 @@ __device__ __forceinline__ void ar_unit(ArWarp<D, GROUP>& s, const ApWork& w, in
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-        mx = fmaxf(mx * sc, m[x]);
+        mx = fmaxf(fmaf(mx, sc, -BELOW), m[x]);
         if (mx == -INFINITY) continue;
         const float alpha = m[x] == -INFINITY ? 0.f : ex2_fast(m[x] - mx);
         m[x] = mx;

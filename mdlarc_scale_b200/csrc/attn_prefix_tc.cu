@@ -8,8 +8,9 @@
 //   warp 1        products of A and of B in turn: O += P V with P read from TMEM, then the next S = Q K^T (128 TMEM columns)
 //   warps 4-11    a thread a query row: maxima, exponentials, row sums, P over the row's own score columns.  (Two threads a row
 //                 had to exchange maxima in every tile and took twice the instructions.)
-// Maxima, sums and results are fp32.  A row's reference maximum is raised only when the sum of a tile's weights against it passes
-// 2^12.  Half queries over a bfloat16 cache are two bfloat16 pieces (exact).  Weights are two 16-bit pieces in every format (half a
+// Maxima, sums and results are fp32.  A row's reference is raised only when the sum of a tile's weights against its maximum passes
+// 2^12; in half it is 2^3 below the maximum, so that weights are up to 2^15 and end at 2^-24 of it: weights down to 2^-28 of a
+// range's largest one count.  Half queries over a bfloat16 cache are two bfloat16 pieces (exact).  Weights are two 16-bit pieces in every format (half a
 // step of the type squared of a weight off): one is half a step off, which adds up to half a step of sum p |v|, more than the output's
 // own rounding without limit where values cancel, and 1.4 times its error on random ones (200 us in place of the 256 below).
 //
@@ -27,7 +28,7 @@ using namespace sm100;
 namespace {
 
 constexpr int AT_ROWS = 128, AT_KEYS = 128, AT_THREADS = 384;
-constexpr float AT_RAISE = 4096.f;         // sum of 128 weights from which a row's reference maximum is raised
+constexpr float AT_RAISE = 4096.f, AT_BELOW = 3.f;         // sum of 128 weights from which a row's reference is raised; log2 units
 constexpr int AT_BOX = 128 * 64 * 2;
 
 __device__ __forceinline__ void add2_f32(uint64_t& sum, float a, float b) {
@@ -264,6 +265,7 @@ attn_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
     const int x = (warp - 4) >> 2, quarter = warp & 3, n_x = tiles_of(x);
     const uint32_t t_lane = tmem_base + ((uint32_t)(quarter * 32) << 16);
     const uint32_t t_s = t_lane + x * 128, t_o = t_lane + 256 + x * D;
+    constexpr float BELOW = HALF ? AT_BELOW : 0.f, RAISE = HALF ? AT_RAISE * 8.f : AT_RAISE;
     const float sc = fabsf(a.scale) * AP_LOG2E;
     const uint64_t sc2 = pack_f32x2(sc, sc);
     const int first_row = (wide ? x * AT_ROWS : 0) + quarter * 32;         // of the warp, among the CTA's
@@ -289,7 +291,7 @@ attn_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
 #pragma unroll
         for (int e = 0; e < 32; e += 2) mx = max3_f32(mx, __uint_as_float(sv[e]), __uint_as_float(sv[e + 1]));
       }
-      return mx * sc;
+      return fmaf(mx, sc, -BELOW);
     };
     for (int i = 0; i < n_x; ++i) {
       if (!__all_sync(0xffffffffu, mbar_wait_bounded(b_s + 8 * x, i & 1))) {
@@ -340,7 +342,7 @@ attn_prefix_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
       weights();
       // Nearly always the reference stays: maxima are looked for only where the weights' sum says that they have grown (they took a tenth
       // of the instructions).  The scores are still there.
-      const bool raise = i > 0 && (total > AT_RAISE || m_ref == -INFINITY);
+      const bool raise = i > 0 && (total > RAISE || m_ref == -INFINITY);
       if (__any_sync(0xffffffffu, raise)) {
         const float mx = largest(seen);
         float alpha = 1.f;

@@ -77,3 +77,26 @@ def test_no_weight_loses_its_second_piece(form, items, heads, kv, plan, dim):
     assert bool((want.abs() > 2 * tol).all())          # one piece alone is told from two
     err = (got.double() - want).abs()
     assert bool((err <= tol).all()), f"{float((err / tol).max()):.2f} of the tolerance"
+
+
+@pytest.mark.parametrize("form", FORMS, ids=FORM_IDS)
+@pytest.mark.parametrize("items,heads,kv,plan", SHAPES)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_many_small_weights_beside_large_ones(form, items, heads, kv, plan, dim):
+    """Every 50th row has the largest score and a value of 0, all others 2^-25.5 of its weight: the result is theirs alone.  A half cache's
+    weights are kept down to 2^-28 of a range's largest one."""
+    shared, own, pitch = 3011, 9, 4112
+    scale = dim ** -0.5
+    large = np.arange(pitch) % 50 == 7
+    k = keys(np.where(large, 0.0, -25.5 * math.log(2) / scale), dim, form[1])[None, None].expand(1, kv, -1, -1).contiguous()
+    v = torch.from_numpy(np.where(large, 0.0, 256.0))[:, None] * torch.tensor([2.0 ** (j % 3) for j in range(dim)])
+    v = v.to(form[1]).cuda()[None, None].expand(1, kv, -1, -1).contiguous()
+    q = torch.ones((items, heads, dim), device="cuda", dtype=form[0])
+    hints = dict(max_group=items, max_prefix=plan, max_own=own)
+    got = prefix_attention(q, k, v, ints([0, items]), ints([0]), ints([shared]), ints([0] * items), ints([0] * items), ints([own] * items), **hints)
+    rows = torch.cat([torch.arange(shared), torch.arange(own)]).cuda()
+    want, spread, size, floor = reference(q[0], k[0, 0, rows], v[0, 0, rows], scale)
+    tol = tolerance(form, shared + own, dim, want, spread, size, floor, least=3)
+    assert bool((want > 3 * tol).all())
+    err = (got.double() - want).abs()
+    assert bool((err <= tol).all()), f"{float((err / tol).max()):.2f} of the tolerance"
