@@ -150,15 +150,14 @@ bool arcb_attn_prefix_supported(int n_heads, int n_kv, int dim, int act_fmt, int
 long long arcb_attn_prefix_scratch(const AttnPrefixArgs& args) {
   AttnPrefixArgs a = args;
   fill_plan(a);
-  const int n = a.plan.parts;
-  return n > 1 && !a.plan.grouped ? (long long)a.n_items * a.n_heads * n * (a.dim + AP_PAD) * 4 : 0;
+  return a.plan.joined ? (long long)a.n_items * a.n_heads * a.plan.parts * (a.dim + AP_PAD) * 4 : 0;
 }
 
 int arcb_launch_attn_prefix(AttnPrefixArgs a, cudaStream_t stream) {
   if (a.n_items <= 0) return 0;
   fill_plan(a);
   const PrefixPlan& p = a.plan;
-  if (p.parts < 1 || (p.parts > 1 && !p.grouped && !a.scratch)) return -1;
+  if (p.parts < 1 || (p.joined && !a.scratch)) return -1;
   const long long joins = ((long long)a.n_items * a.n_heads + 3) / 4;
   if (p.shared.units + p.own.units > 0x7fffffffLL || joins > 0x1fffffffLL) return -1;
   a.first_block = 0;
@@ -172,7 +171,7 @@ int arcb_launch_attn_prefix(AttnPrefixArgs a, cudaStream_t stream) {
     a.beside = p.shared.units > 0 && !arcb_pdl_enabled();
     r = launch_part(a, p.own, p.own.units, stream);
   }
-  if (r || p.parts == 1 || p.grouped) return r;
+  if (r || !p.joined) return r;
   // Its CTAs come while the last ones of the parts are at work, and wait.  Four warps a result where a warp each would leave SMs without
   // work (two samples in four parts: 9.3 us in all with a warp each, 7.7 with four).
   const bool few = joins < 4LL * arcb_num_sms();

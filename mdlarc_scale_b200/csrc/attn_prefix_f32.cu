@@ -161,7 +161,7 @@ __device__ __forceinline__ void af_body(const AttnPrefixArgs& a, const ApWork& w
     if (row >= w.rows) continue;
     const int R = w.r0 + row, item = w.item0 + R / a.rep;
     const long long ih = (long long)item * a.n_heads + w.kvh * a.rep + R % a.rep;
-    const bool whole = a.plan.parts == 1;
+    const bool whole = !a.plan.joined;
     float* to = whole ? reinterpret_cast<float*>(a.out) + (size_t)ih * D : ap_record(a, ih, w.part);
     if (whole) {
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -287,7 +287,7 @@ attn_prefix_f32_few_kernel(AttnPrefixArgs a, unsigned units) {
       if (r >= w.rows) continue;        // of the whole warp
       const int Rr = w.r0 + r, item = w.item0 + Rr / a.rep;
       const long long ih = (long long)item * a.n_heads + w.kvh * a.rep + Rr % a.rep;
-      const bool whole = a.plan.parts == 1, none = whole && (l[r] == 0.f || (a.item_skip && a.item_skip[item]));
+      const bool whole = !a.plan.joined, none = whole && (l[r] == 0.f || (a.item_skip && a.item_skip[item]));
       const float by = whole && !none ? 1.f / l[r] : 1.f;
       float* to = whole ? reinterpret_cast<float*>(a.out) + (size_t)ih * D : ap_record(a, ih, w.part);
 #pragma unroll

@@ -211,7 +211,7 @@ __device__ __forceinline__ void am_body(const AttnPrefixArgs& a, const ApWork& w
     if ((lane & 3) == 0) *reinterpret_cast<float2*>(rec + D) = make_float2(m[x], l[x]);
   }
   __syncthreads();
-  const bool whole = a.plan.parts == 1;
+  const bool whole = !a.plan.joined;
   for (int i = threadIdx.x; i < RG * 16 * (D / 4); i += 128) {
     const int r = i / (D / 4), c = i % (D / 4) * 4;
     if (r >= w.rows) break;

@@ -294,7 +294,7 @@ __device__ __forceinline__ void ar_unit(ArWarp<D, GROUP>& s, const ApWork& w, in
     }
   }
   // The unit's part of the result: eight lanes have eight neighbouring value columns of a query.
-  const bool whole = a.plan.parts == 1;
+  const bool whole = !GROUP && !a.plan.joined;
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
     if (x >= w.rows) break;

@@ -21,6 +21,7 @@ struct PrefixPlan {
   int together;             // both parts in one launch
   int grouped;              // a CTA has all units of a (group, key head) and joins them itself
   int parts;                // of a result
+  int joined;               // a last kernel makes results of them; else there is one, or a group's CTA has joined them
 };
 
 // `rows` query rows at each of `heads` (groups or items) x n_kv; `tc`: tcgen05 may be used.
@@ -91,5 +92,6 @@ inline PrefixPlan prefix_plan(long long n_groups, long long max_group, long long
   p.shared.units *= p.shared.splits;
   p.own.units *= p.own.splits;
   p.parts = p.shared.splits + p.own.splits;
+  p.joined = !p.grouped && (p.parts > 1 || p.shared.kernel == AP_TC);      // the tcgen05 kernel writes parts alone
   return p;
 }

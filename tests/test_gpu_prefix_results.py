@@ -1,0 +1,40 @@
+"""Every item of every call has a result: one range without a part to join it with, items that bad groups leave out, indices at the ends of
+32 bits.  Tolerances are those of test_gpu_prefix_attention.py."""
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from gpu_util import have_b200
+from mdlarc_scale_b200 import _lib, prefix_attention
+from test_gpu_prefix_attention import BF16, F16, F32, FORM_IDS, FORMS, Case
+
+pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not have_b200(), reason="needs a B200")]
+CODES = {F16: _lib.ACT_F16, BF16: _lib.ACT_BF16, F32: _lib.ACT_F32}
+
+
+def scratch_of(c, **hints):
+    n, heads, dim = c.q.shape
+    a = _lib.PrefixAttentionArgs(n_groups=len(c.sizes), n_items=n, n_heads=heads, n_kv=c.k.shape[1], dim=dim, n_seqs=c.k.shape[0], t_max=c.k.shape[2],
+                                 scale=0.125, act_format=CODES[c.q.dtype], kv_format=CODES[c.k.dtype], **hints)
+    return _lib.load().arcb_prefix_attention_scratch_bytes(C.byref(a))
+
+
+@pytest.mark.parametrize("form", [(BF16, BF16), (F16, F16)], ids=["bf16", "f16"])
+@pytest.mark.parametrize("dim,heads,kv,most,prefix,groups", [(64, 8, 8, 100, 1024, 16), (128, 16, 4, 40, 700, 35), (64, 4, 2, 70, 513, 74)])
+def test_shared_rows_alone_in_one_range(form, dim, heads, kv, most, prefix, groups):
+    """Enough groups for one range each, more than 64 query rows, no rows of the items' own: parts of tensor memory's results, joined alone."""
+    sizes = [most, 0, 1] + [(g * 37) % (most + 1) for g in range(groups - 3)]
+    lens = [prefix, prefix, 0] + [prefix - (g * 131) % prefix for g in range(groups - 3)]
+    c = Case(sizes, lens, [0] * sum(sizes), heads, kv, dim, form, seed=groups, own_in_group=True, rows=prefix + 9)
+    hints = dict(max_group=most, max_prefix=prefix)
+    assert scratch_of(c, **hints) == c.q.numel() // dim * (dim + 4) * 4          # one part of every result
+    out = torch.full_like(c.q, math.nan)
+    prefix_attention(c.q, c.k, c.v, *c.groups, out=out, **hints)
+    c.check(out, mine=False)
+    skip = torch.zeros(sum(sizes), dtype=torch.uint8, device="cuda")
+    skip[0] = skip[-1] = 1
+    c.check(prefix_attention(c.q, c.k, c.v, *c.groups, skip=skip, **hints), mine=False, skip=(0, sum(sizes) - 1))
+    c.check(prefix_attention(c.q, c.k, c.v, *c.groups, scale=-0.2, **hints), scale=-0.2, mine=False)
