@@ -81,12 +81,12 @@ __device__ __forceinline__ ApWork ap_work(const AttnPrefixArgs& a, long long blo
     k.rows = min(a.plan.own.tile, a.rep - k.r0);
     k.seq = a.item_seq ? a.item_seq[k.item0] : k.item0;
     at0 = a.item_begin ? a.item_begin[k.item0] : 0;
-    len = a.item_end[k.item0] - at0;
-    if (len > 0 && (at0 < 0 || at0 + len > a.t_max || k.seq < 0 || k.seq >= a.n_seqs)) {
+    len = ap_row_count(at0, a.item_end[k.item0], k.seq, a.n_seqs, a.t_max);
+    if (len < 0) {
       if (report) arcb_set_error(a.status, ARCB_DEV_BAD_INDEX);
       len = 0;
     }
-    if (len < 0 || (a.item_skip && a.item_skip[k.item0])) len = 0;
+    if (a.item_skip && a.item_skip[k.item0]) len = 0;
     grain = a.plan.own.kernel == AP_ROWS ? 15 : 63;
     k.part = a.plan.shared.splits + split;
   }

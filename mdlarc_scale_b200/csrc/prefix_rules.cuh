@@ -1,6 +1,19 @@
-// How attention over shared prefixes is cut into units of work (host code, no CUDA).
+// How attention over shared prefixes is cut into units of work (host code, no CUDA), and what indices from the device may be.
 #pragma once
 #include <algorithm>
+
+#ifdef __CUDACC__
+#define AP_RULE __host__ __device__ inline
+#else
+#define AP_RULE inline
+#endif
+
+// How many rows [begin, end) of sequence seq are, -1 where some are outside the cache.  The ends are looked at before they are
+// subtracted: they may be any 32 bits.
+AP_RULE int ap_row_count(int begin, int end, int seq, int n_seqs, int t_max) {
+  if (end <= begin) return 0;
+  return begin < 0 || end > t_max || seq < 0 || seq >= n_seqs ? -1 : end - begin;
+}
 
 // Kernels, by the query rows of a unit: a warp for up to 8, a CTA for up to 64, a CTA with tcgen05 products for up to 256; in 32-bit
 // formats a warp for up to 4, a CTA for up to 64.

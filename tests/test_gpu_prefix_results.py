@@ -38,3 +38,26 @@ def test_shared_rows_alone_in_one_range(form, dim, heads, kv, most, prefix, grou
     skip[0] = skip[-1] = 1
     c.check(prefix_attention(c.q, c.k, c.v, *c.groups, skip=skip, **hints), mine=False, skip=(0, sum(sizes) - 1))
     c.check(prefix_attention(c.q, c.k, c.v, *c.groups, scale=-0.2, **hints), scale=-0.2, mine=False)
+
+
+@pytest.mark.parametrize("form", FORMS, ids=FORM_IDS)
+@pytest.mark.parametrize("sizes,heads,kv", [([3, 2], 2, 2), ([5, 2], 16, 2), ([40, 3], 4, 2)])
+def test_ends_of_32_bits(form, sizes, heads, kv):
+    """Ends whose difference does not fit 32 bits: rows outside the cache count as not there and are reported, an end before the begin is no
+    row and no error."""
+    c = Case(sizes, [140, 130], [1 + i % 9 for i in range(sum(sizes))], heads, kv, 64, form, 31)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    item = 1
+    for hints in (dict(max_group=max(sizes), max_prefix=140, max_own=9), {}):
+        for begin, end, code in ((-2 ** 31, 0, 4), (-2 ** 31, 2 ** 31 - 1, 4), (-2, 2 ** 31 - 1, 4), (-1, 2 ** 31 - 1, 4), (-2 ** 31, -1, 4), (1, -2 ** 31, 0),
+                                 (2 ** 31 - 1, -2 ** 31, 0), (2 ** 31 - 1, 2 ** 31 - 1, 0), (-2 ** 31, -2 ** 31, 0), (0, 2 ** 31 - 1, 4), (5, -3, 0)):
+            keep, old = [t[item].clone() for t in c.items], c.own[item]
+            c.items[1][item], c.items[2][item], c.own[item] = begin, end, 0
+            status.zero_()
+            out = c(status=status, **hints)
+            assert status.item() == code, (begin, end)
+            was, c.begin[item] = c.begin[item], 0
+            c.check(out)
+            c.begin[item], c.own[item] = was, old
+            for t, v in zip(c.items, keep):
+                t[item] = v

@@ -16,7 +16,9 @@ extern "C" void plan(const long long* in, int* out) {
   const PrefixPlan p = prefix_plan(in[0], in[1], in[2], in[3], in[4], (int)in[5], (int)in[6], (int)in[7], in[8] != 0, in[9] != 0, (int)in[10]);
   out[0] = p.shared.kernel == AP_TC; out[1] = p.parts; out[2] = p.grouped; out[3] = p.joined;
 }
+extern "C" int rows(int begin, int end, int seq, int n_seqs, int t_max) { return ap_row_count(begin, end, seq, n_seqs, t_max); }
 """
+LEAST, MOST = -2 ** 31, 2 ** 31 - 1
 # groups, items of each, key heads, heads of a key head, dim, shared rows: units enough for one range each, no rows of the items' own
 ONE_RANGE = [(64, 32, 8, 4, 128, 2048), (8, 64, 8, 4, 128, 1024), (20, 66, 20, 1, 64, 512), (1, 256, 32, 4, 128, 700)]
 
@@ -32,7 +34,18 @@ def plan(tmp_path_factory):
         out = (C.c_int * 4)()
         lib.plan((C.c_longlong * 11)(groups, items, prefix, max(1, groups) * items, own, kv, rep, dim, wide, tc, sms), out)
         return tuple(out)
+    of.rows = lib.rows
     return of
+
+
+def test_rows_of_any_ends(plan):
+    """Ends of any 32 bits: a range is counted, empty, or outside the cache, and never a difference that has wrapped around."""
+    ends = [LEAST, LEAST + 1, -100, -2, -1, 0, 1, 2, 99, 100, 101, 10 ** 9, MOST - 1, MOST]
+    for begin in ends:
+        for end in ends:
+            for seq in (LEAST, -1, 0, 4, 5, MOST):
+                inside = begin >= 0 and end <= 100 and 0 <= seq < 5
+                assert plan.rows(begin, end, seq, 5, 100) == (0 if end <= begin else end - begin if inside else -1), (begin, end, seq)
 
 
 @pytest.mark.parametrize("groups,items,kv,rep,dim,prefix", ONE_RANGE)
