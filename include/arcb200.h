@@ -493,7 +493,9 @@ int arcb_op_decode_attention_static(const void* d_q16, const void* d_k, const vo
  *   Arrays start on 16 bytes.  max_* are upper bounds the work is laid out for (0: n_items, t_max, t_max); more items in a
  *   group than max_group is an error, longer rows only cost time.
  *   d_status (optional): set to ARCB_DEV_BAD_INDEX's value, 4, where a group or an item names rows outside the cache, or the
- *   groups do not cover the items one after the other; such rows count as not there.  1 to 3: a wait inside a kernel ran out. */
+ *   groups do not cover the items one after the other; such rows count as not there, and so do the shared rows of items that
+ *   are in no group, or in one of more than max_group items.  Every item has a result all the same; that of an item which several
+ *   groups claim (bounds that go back) is undefined.  1 to 3: a wait inside a kernel ran out. */
 typedef struct arcb_prefix_attention_args {
   const void* d_q;               /* item i, head h: dim values at d_q + i * q_pitch + h * dim         */
   const void* d_k;               /* [n_seqs][n_kv][t_max][dim]                                        */

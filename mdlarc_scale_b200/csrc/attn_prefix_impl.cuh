@@ -27,10 +27,41 @@ inline cudaError_t ap_launch_beside(void (*kernel)(KArgs...), dim3 grid, dim3 bl
 }
 
 // A CTA's part of the work: query rows (row r is item item0 + (r0 + r) / rep, head kvh * rep + (r0 + r) % rep), cached rows
-// [begin, end) of a sequence, and which part of the results it is.
+// [begin, end) of a sequence, and which part of the results it is.  behind: items of a bad group that the plan has no units for.
 struct ApWork {
-  int item0, r0, rows, kvh, seq, begin, end, part;
+  int item0, r0, rows, kvh, seq, begin, end, part, behind;
 };
+
+__device__ __forceinline__ float* ap_record(const AttnPrefixArgs& a, long long ih, int part) {
+  return a.scratch + ((size_t)ih * a.plan.parts + part) * (a.dim + AP_PAD);
+}
+
+// Outputs saturate in half, as all of the library's do; NaN stays NaN.
+__device__ __forceinline__ void ap_store4(void* out, size_t at, float4 v, int fmt) {
+  if (fmt != 1 || !(isnan(v.x) || isnan(v.y) || isnan(v.z) || isnan(v.w))) {
+    st_act4(out, at, v, fmt);
+    return;
+  }
+  const float f[4] = {v.x, v.y, v.z, v.w};
+  for (int i = 0; i < 4; ++i) reinterpret_cast<__half*>(out)[at + i] = isnan(f[i]) ? __float2half_rn(f[i]) : __float2half_rn(fminf(fmaxf(f[i], -65504.f), 65504.f));
+}
+
+__device__ __forceinline__ void ap_store1(void* out, size_t at, float v, int fmt) {
+  if (fmt == 1 && isnan(v)) reinterpret_cast<__half*>(out)[at] = __float2half_rn(v);
+  else st_act(out, at, v, fmt);
+}
+
+// Part `part` of some items and a key head's heads when they see no rows: an empty one, or zeros where parts are not joined.  (The CTA of
+// a group joins its own.)
+__device__ __forceinline__ void ap_empty(const AttnPrefixArgs& a, int item0, int items, int kvh, int part) {
+  for (int i = 0; i < items; ++i)
+    for (int h = 0; h < a.rep; ++h) {
+      const long long ih = (long long)(item0 + i) * a.n_heads + kvh * a.rep + h;
+      if (a.plan.joined) *reinterpret_cast<float2*>(ap_record(a, ih, part) + a.dim) = make_float2(-INFINITY, 0.f);
+      else if (!a.plan.grouped)
+        for (int c = 0; c < a.dim; c += 4) ap_store4(a.out, (size_t)ih * a.dim + c, make_float4(0.f, 0.f, 0.f, 0.f), a.act_fmt);
+    }
+}
 
 // Numbers: tiles of one (group, head, range) follow each other, so that they find its rows in L2.
 __device__ __forceinline__ ApWork ap_work(const AttnPrefixArgs& a, long long block, bool report) {
@@ -58,11 +89,25 @@ __device__ __forceinline__ ApWork ap_work(const AttnPrefixArgs& a, long long blo
     }
     const bool bad = first < 0 || last < first || last > a.n_items || last - first > a.max_group || len < 0 || len > a.t_max ||
                      (len > 0 && (k.seq < 0 || k.seq >= a.n_seqs)) || (g == 0 && first != 0) || (g == a.n_groups - 1 && last != a.n_items);
+    k.behind = 0;
     if (bad) {
+      // Its items see no shared rows.  They are those between its ends, of which one that is no item's counts as the one ahead of it, the
+      // first of all as 0 and the last as n_items: from one group to the next these ends leave no item out, whatever they are.
       if (report) arcb_set_error(a.status, ARCB_DEV_BAD_INDEX);
-      first = min(max(first, 0), a.n_items);
-      last = min(max(last, first), min(a.n_items, first + a.max_group));
+      if (a.uniform <= 0) {
+        for (int i = g; i >= 0; --i) {
+          first = i == 0 ? 0 : a.group_first[i];
+          if (first >= 0 && first <= a.n_items) break;
+        }
+        if (g == a.n_groups - 1) last = a.n_items;
+        else if (last < first || last > a.n_items) last = first;
+      }
       len = 0;
+      if (last - first > a.max_group) {
+        k.behind = last - first - a.max_group;
+        last = first + a.max_group;
+        if (report && t == 0) ap_empty(a, last, k.behind, k.kvh, split);
+      }
     }
     k.item0 = first;
     k.r0 = t * a.plan.shared.tile;
@@ -95,25 +140,6 @@ __device__ __forceinline__ ApWork ap_work(const AttnPrefixArgs& a, long long blo
   k.begin = at0 + min(split * chunk, len);
   k.end = at0 + min((split + 1) * chunk, len);
   return k;
-}
-
-__device__ __forceinline__ float* ap_record(const AttnPrefixArgs& a, long long ih, int part) {
-  return a.scratch + ((size_t)ih * a.plan.parts + part) * (a.dim + AP_PAD);
-}
-
-// Outputs saturate in half, as all of the library's do; NaN stays NaN.
-__device__ __forceinline__ void ap_store4(void* out, size_t at, float4 v, int fmt) {
-  if (fmt != 1 || !(isnan(v.x) || isnan(v.y) || isnan(v.z) || isnan(v.w))) {
-    st_act4(out, at, v, fmt);
-    return;
-  }
-  const float f[4] = {v.x, v.y, v.z, v.w};
-  for (int i = 0; i < 4; ++i) reinterpret_cast<__half*>(out)[at + i] = isnan(f[i]) ? __float2half_rn(f[i]) : __float2half_rn(fminf(fmaxf(f[i], -65504.f), 65504.f));
-}
-
-__device__ __forceinline__ void ap_store1(void* out, size_t at, float v, int fmt) {
-  if (fmt == 1 && isnan(v)) reinterpret_cast<__half*>(out)[at] = __float2half_rn(v);
-  else st_act(out, at, v, fmt);
 }
 
 }  // namespace

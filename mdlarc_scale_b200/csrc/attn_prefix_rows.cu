@@ -62,13 +62,18 @@ struct ArWarp {
   int ahead_i, ahead_left, rows_left;      // the rows from the next one on, and where they are
   const char* from[2];
   int flight, put, get;                    // tiles asked for and not used up
-  int g, kvh, item0, items;                // GROUP: and its items
+  int g, kvh, item0, items;                // GROUP: and its items, max_group of them at a time
   float* records;                          // GROUP: [query row][part][D + AP_PAD]
 
   __device__ __forceinline__ ApWork work(long long u) const {
     if constexpr (GROUP) {
       const int splits = a.plan.shared.splits, own = (int)u - splits;
-      if (own < 0) return ap_work(a, ((long long)g * a.n_kv + kvh) * splits + u, true);
+      if (own < 0) {
+        ApWork w = ap_work(a, ((long long)g * a.n_kv + kvh) * splits + u, true);
+        w.item0 = item0;
+        w.rows = items * a.rep;
+        return w;
+      }
       const int item = own / a.plan.own.splits;
       if (item >= items) return ApWork{};
       return ap_work(a, a.plan.shared.units + ((long long)(item0 + item) * a.n_kv + kvh) * a.plan.own.splits + own % a.plan.own.splits, true);
@@ -366,6 +371,7 @@ attn_prefix_rows_kernel(AttnPrefixArgs a, long long n_units) {
                      (uint32_t)((col >> 3) * C::BOX + row * 128 + (((col & 7) ^ (row & 7)) << 4))};
   s.batch_of = -1;
   s.flight = s.put = s.get = s.ahead_i = 0;
+  int behind = 0;
   if constexpr (GROUP) {
     s.g = (int)blockIdx.x / a.n_kv;
     s.kvh = (int)blockIdx.x % a.n_kv;
@@ -373,23 +379,32 @@ attn_prefix_rows_kernel(AttnPrefixArgs a, long long n_units) {
     s.item0 = all.item0;
     s.items = max(all.rows, 0) / a.rep;
     s.records = reinterpret_cast<float*>(ar_smem + W * C::WARP);
+    behind = all.behind;
   }
-  if (s.n > 0) {
-    ApWork w = s.unit(0);
-    s.look_at(w);
-    for (int i = 0; i < s.n; ++i) {
-      if (w.rows <= 4) ar_unit<D, HALF, QS, true>(s, w, i);
-      else ar_unit<D, HALF, QS, false>(s, w, i);
-      if (i + 1 < s.n) {
-        if (s.ahead_i == i) s.look_at(s.unit(++s.ahead_i));
-        w = s.ahead;
+  for (;;) {
+    if (s.n > 0) {
+      ApWork w = s.unit(0);
+      s.look_at(w);
+      for (int i = 0; i < s.n; ++i) {
+        if (w.rows <= 4) ar_unit<D, HALF, QS, true>(s, w, i);
+        else ar_unit<D, HALF, QS, false>(s, w, i);
+        if (i + 1 < s.n) {
+          if (s.ahead_i == i) s.look_at(s.unit(++s.ahead_i));
+          w = s.ahead;
+        }
       }
     }
-  }
-  if constexpr (GROUP) {
+    if constexpr (!GROUP) break;
     __syncthreads();
     for (int r = warp; r < s.items * a.rep; r += W)
       ar_join<D>(a, s.records + r * a.plan.parts * (D + AP_PAD), s.item0 + r / a.rep, s.kvh * a.rep + r % a.rep, lane);
+    if (behind <= 0) break;
+    __syncthreads();               // a group of more items than it may have, which see their own rows alone: the next ones
+    s.item0 += s.items;
+    s.items = min(behind, a.max_group);
+    behind -= s.items;
+    s.batch_of = -1;
+    s.ahead_i = 0;
   }
   if (a.beside) pdl_wait();      // this launch's end is the other's too
 }

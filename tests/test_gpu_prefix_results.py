@@ -61,3 +61,54 @@ def test_ends_of_32_bits(form, sizes, heads, kv):
             c.begin[item], c.own[item] = was, old
             for t, v in zip(c.items, keep):
                 t[item] = v
+
+
+def dirty(c, **hints):
+    """The next call's scratch has held other parts."""
+    need = max(scratch_of(c, d_item_end=4096, **hints), scratch_of(c, **hints))
+    torch.full((max(4, need) // 4,), 3.0, device="cuda")
+    return torch.full_like(c.q, math.nan)
+
+
+# items of three groups, heads, key heads, rows of the longest group, what the plan is told: one CTA a group, warps, CTAs of 16 to 64 query
+# rows, tensor memory; results of one part where no item has rows of its own
+@pytest.mark.parametrize("form", FORMS, ids=FORM_IDS)
+@pytest.mark.parametrize("sizes,heads,kv,prefix,plan", [([3, 2, 4], 4, 4, 60, 60), ([3, 2, 4], 2, 2, 200, 200), ([3, 2, 4], 2, 1, 190, 4000), ([3, 2, 4], 16, 4, 60, 60),
+                                                        ([9, 5, 16], 2, 1, 300, 300), ([30, 7, 50], 1, 1, 200, 200), ([80, 70, 100], 2, 2, 700, 4000)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_items_that_bad_groups_leave_out(form, sizes, heads, kv, prefix, plan, dim):
+    """Items of groups that are wrong, and items between or behind groups, see their own rows alone, and nothing that scratch or output have held."""
+    n, ends = sum(sizes), np.cumsum([0] + sizes).tolist()
+    c = Case(sizes, [prefix, prefix - 7, prefix // 2], [i % 9 for i in range(n)], heads, kv, dim, form, seed=n)
+    hints = dict(max_group=max(sizes), max_prefix=plan, max_own=9)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    bad = [("first", 0, 2, [0]), ("first", 0, -2 ** 31, [0]), ("first", 0, n + 1, [0]), ("first", 3, n - 2, [2]), ("first", 3, 2 ** 31 - 1, [2]), ("first", 3, 0, [2]),
+           ("first", 1, -5, [0, 1]), ("first", 1, 10 ** 6, [0, 1]), ("first", 2, n + 1, [1, 2]), ("seq", 1, 99999, [1]), ("len", 2, -1, [2]),
+           ("group", 0, max(sizes) - 1, [2])]
+    tensors, lengths, own = dict(zip(("first", "seq", "len"), c.groups)), list(c.prefix), list(c.own)
+    assert tensors["first"].tolist() == ends
+    for what, at, value, gone in bad:
+        kw = dict(hints)
+        if what == "group":
+            kw["max_group"] = value
+        else:
+            old = tensors[what][at].clone()
+            tensors[what][at] = value
+        c.prefix = [0 if g in gone else p for g, p in enumerate(lengths)]
+        for mine in (True, False):
+            status.zero_()
+            out = dirty(c, **kw)
+            prefix_attention(c.q, c.k, c.v, *c.groups, *(c.items if mine else ()), out=out, status=status, **kw)
+            assert status.item() == 4, (what, at, value)
+            c.check(out, mine=mine)
+        if what != "group":
+            tensors[what][at] = old
+    # no group but the last one, which ends where it begins
+    tensors["first"].zero_()
+    c.prefix = [0, 0, 0]
+    for mine in (True, False):
+        status.zero_()
+        out = dirty(c, **hints)
+        prefix_attention(c.q, c.k, c.v, *c.groups, *(c.items if mine else ()), out=out, status=status, **hints)
+        assert status.item() == 4
+        c.check(out, mine=mine)
