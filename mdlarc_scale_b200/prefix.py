@@ -20,6 +20,10 @@ _raw_stream = torch._C._cuda_getCurrentRawStream      # the current stream's han
 _current_device = torch._C._cuda_getDevice             # of a process that has CUDA tensors: nothing is left to initialise
 
 
+def _refuse_gradient():
+    raise ValueError("there is no gradient of this operator: detach() what requires one, or call it under torch.no_grad()")
+
+
 def _refuse_index(name: str, n: int):
     raise ValueError(f"{name} must be a contiguous int32 tensor (skip: uint8) of {n} values on the queries' device")
 
@@ -40,7 +44,10 @@ def prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, group_fi
     ``max_group``: no group may have more items.  ``status`` (int32, one value) becomes non-zero when an index is outside the
     cache.  Keys that an item sees are finite where half queries meet a bfloat16 cache (a query is a sum of two pieces there,
     which an infinity would turn into no number); what no item sees may hold anything.  The queries may be rows of a wider
-    matrix; all else is contiguous.  Runs on the current stream."""
+    matrix; all else is contiguous.  Has no gradient, and refuses tensors that require one where it would be recorded.  Runs on the
+    current stream."""
+    if (q.requires_grad or k.requires_grad or v.requires_grad or (out is not None and out.requires_grad)) and torch.is_grad_enabled():
+        _refuse_gradient()
     if q.dim() != 3 or k.dim() != 4 or k.shape != v.shape:
         raise ValueError("queries are [items, heads, dim], keys and values [sequences, kv_heads, rows, dim]")
     n, heads, dim = q.shape
@@ -117,7 +124,10 @@ def copy_cache_rows(cache: torch.Tensor, copies) -> None:
     """Copies rows between the sequences of ``cache`` [..., n_seqs, heads, rows, dim], in place: (src, dst, begin, end) takes rows
     ``[begin, end)`` of every plane and head of sequence ``src`` to the same rows of ``dst``.  ``copies``: any number of them, as
     a list or an integer array [n, 4] on the host.  All rows are read before any is written, so sequences may change places; no
-    sequence may be written twice.  Runs on the current stream; ``copies`` may be changed after the call."""
+    sequence may be written twice.  Has no gradient, and refuses a cache that requires one where it would be recorded.  Runs on the
+    current stream; ``copies`` may be changed after the call."""
+    if cache.requires_grad and torch.is_grad_enabled():
+        _refuse_gradient()
     dev = cache.get_device()
     if cache.dim() < 4 or dev < 0 or not cache.is_contiguous():
         raise ValueError("the cache must be a contiguous CUDA tensor [..., n_seqs, heads, rows, dim]")

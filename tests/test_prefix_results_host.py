@@ -6,6 +6,7 @@ import subprocess
 from pathlib import Path
 
 import pytest
+import torch
 
 from mdlarc_scale_b200 import _lib
 
@@ -81,3 +82,22 @@ def test_results_are_written_once(plan):
         assert joined == (not grouped and (parts > 1 or tc))
         seen.add((tc, parts > 1, grouped))
     assert len(seen) == 5
+
+
+def test_gradients_are_refused():
+    """Neither operator has one: an output without it would end a backward pass in silence."""
+    from mdlarc_scale_b200 import copy_cache_rows, prefix_attention
+    q, k = torch.zeros((2, 2, 64)), torch.zeros((1, 2, 5, 64))
+    first, seq, length = (torch.zeros(n, dtype=torch.int32) for n in (2, 1, 1))
+    for at in range(3):
+        args = [t.clone().requires_grad_(i == at) for i, t in enumerate((q, k, k))]
+        with pytest.raises(ValueError, match="no gradient"):
+            prefix_attention(*args, first, seq, length)
+        with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
+            prefix_attention(*args, first, seq, length)
+    with pytest.raises(ValueError, match="no gradient"):
+        prefix_attention(q, k, k, first, seq, length, out=torch.zeros_like(q, requires_grad=True))
+    with pytest.raises(ValueError, match="no gradient"):
+        copy_cache_rows(k.clone().requires_grad_(), [(0, 0, 0, 1)])
+    with pytest.raises(ValueError, match="CUDA"):
+        copy_cache_rows(k, [(0, 0, 0, 1)])
