@@ -291,7 +291,7 @@ typedef struct arcb_session_desc {
   int32_t prefix_group;           /* grid model: n > 1 = rows g n ... g n + n - 1 are samples of one prompt, whose keys and
                                      values only row g n holds: decode steps read them there once for all of them, and a
                                      row's own cache from the end of the prompt on.  Prefill the prompts of rows g n alone and
-                                     name the same d_first_row for the n rows.  n divides n_seqs; the workspace grows by
+                                     name the same d_first_row for the n rows.  n divides n_seqs, attn_splits is 0, and the workspace grows by
                                      arcb_session_prefix_bytes.  0 or 1: every row holds its prompt            */
 } arcb_session_desc;
 

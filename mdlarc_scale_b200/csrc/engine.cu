@@ -310,6 +310,8 @@ extern "C" int arcb_session_create(arcb_engine* e, const arcb_session_desc* dsc,
   const WsLayout w = ws_layout(e, dsc->n_seqs, dsc->max_prefill_tokens, scratch_splits(e, dsc->n_seqs, dsc->attn_splits));
   const int64_t prefix_bytes = arcb_session_prefix_bytes(e, dsc->n_seqs, dsc->t_max, dsc->max_new, dsc->prefix_group);
   if (prefix_bytes < 0 || dsc->prefix_group < 0) return arcb_fail(ARCB_E_ARG, "prefix_group must divide n_seqs, in a cache of fewer than 2^31 rows");
+  if (dsc->prefix_group > 1 && dsc->attn_splits > 0)
+    return arcb_fail(ARCB_E_UNSUPPORTED, "attn_splits is for rows that hold their prompts: with prefix_group the ranges follow from the sizes");
   if ((size_t)dsc->workspace_bytes < w.total + (size_t)prefix_bytes) return arcb_fail(ARCB_E_ARG, "workspace too small");
   arcb_session* s = new arcb_session();
   s->eng = e;
