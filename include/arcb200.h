@@ -300,6 +300,10 @@ int64_t arcb_session_workspace_bytes(const arcb_engine* eng, int32_t n_seqs,
 int64_t arcb_kv_cache_bytes(const arcb_engine* eng, int32_t n_seqs, int32_t t_max);
 /* what a session with prefix_group > 1 needs in its workspace on top of arcb_session_workspace_bytes; < 0: not supported */
 int64_t arcb_session_prefix_bytes(const arcb_engine* eng, int32_t n_seqs, int32_t t_max, int32_t max_new, int32_t prefix_group);
+/* CTAs of the cluster that the decode steps of rows which hold their prompts run in, all of a call in one launch; 0: separate
+ * launches.  Where it is not 0, samples of a prompt are quicker as such rows (arcb_session_fork copies the prompt) than with
+ * prefix_group, whose steps are separate launches. */
+int32_t arcb_session_step_ctas(const arcb_engine* eng, int32_t n_seqs, int32_t t_max);
 /* Creating a session launches nothing: the session's device state (inside d_workspace) is cleared
  * by the session's FIRST arcb_prefill, on that call's stream, so a workspace recycled from an
  * earlier session is ordered after whatever that stream still has queued on it.  Use one stream

@@ -42,7 +42,7 @@ EXPORTS = [
     "arcb_engine_load_tensor", "arcb_session_workspace_bytes", "arcb_kv_cache_bytes",
     "arcb_session_create", "arcb_session_destroy", "arcb_prefill", "arcb_decode",
     "arcb_engine_create_layered", "arcb_session_feed", "arcb_session_step_logits", "arcb_session_finished",
-    "arcb_session_expand_rows", "arcb_session_prefix_bytes", "arcb_session_fork",
+    "arcb_session_expand_rows", "arcb_session_prefix_bytes", "arcb_session_step_ctas", "arcb_session_fork",
     "arcb_session_poll", "arcb_engine_saturation_count", "arcb_session_attention_probe", "arcb_launch_count", "arcb_op_rmsnorm", "arcb_op_gemm",
     "arcb_op_gemm_residual", "arcb_gemm_splitk_scratch_bytes", "arcb_op_gemm_residual_splitk",
     "arcb_attn_scratch_bytes", "arcb_op_decode_attention", "arcb_op_decode_attention_static",
@@ -196,6 +196,7 @@ def load() -> C.CDLL:
     lib.arcb_kv_cache_bytes.argtypes = [vp, i32, i32]
     lib.arcb_session_prefix_bytes.restype = i64
     lib.arcb_session_prefix_bytes.argtypes = [vp, i32, i32, i32, i32]
+    lib.arcb_session_step_ctas.argtypes = [vp, i32, i32]
     lib.arcb_session_fork.argtypes = [vp, i32, i32, vp, i32, vp]
     lib.arcb_session_create.argtypes = [vp, C.POINTER(SessionDesc), C.POINTER(vp)]
     lib.arcb_session_destroy.argtypes = [vp]

@@ -280,6 +280,12 @@ extern "C" int64_t arcb_session_prefix_bytes(const arcb_engine* e, int32_t n_seq
   return (int64_t)align_up((size_t)arcb_attn_prefix_scratch(prefix_args(e, n_seqs, t_max, max_new, group)), 256);
 }
 
+extern "C" int32_t arcb_session_step_ctas(const arcb_engine* e, int32_t n_seqs, int32_t t_max) {
+  // a caller that chooses kernels gets the separate launches
+  if (!e || n_seqs <= 0 || t_max <= 0 || e->lm || e->cfg.gemm_path != ARCB_GEMM_AUTO || e->cfg.attn_path != ARCB_ATTN_AUTO) return 0;
+  return arcb_step_cluster(n_seqs, e->cfg.d_model, e->cfg.d_ff, e->cfg.n_layers, t_max);
+}
+
 extern "C" int arcb_session_create(arcb_engine* e, const arcb_session_desc* dsc, arcb_session** out) {
   if (!e || !dsc || !out) return arcb_fail(ARCB_E_ARG, "null argument");
   if (!engine_complete(e)) return arcb_fail(ARCB_E_STATE, "engine is missing tensors");
@@ -358,9 +364,8 @@ extern "C" int arcb_session_create(arcb_engine* e, const arcb_session_desc* dsc,
   s->state_ints = ints;
   s->n_state_ints = w.n_int;
   s->step_probe = reinterpret_cast<unsigned long long*>(ints + ((13 * (size_t)B + 9) & ~(size_t)1));
-  // a caller that chooses kernels or splits gets the separate launches
-  if (dsc->attn_splits <= 0 && dsc->prefix_group <= 1 && e->cfg.gemm_path == ARCB_GEMM_AUTO && e->cfg.attn_path == ARCB_ATTN_AUTO)
-    s->step_cluster = arcb_step_cluster(B, e->cfg.d_model, e->cfg.d_ff, e->cfg.n_layers, dsc->t_max);
+  // a caller that chooses splits gets the separate launches
+  if (dsc->attn_splits <= 0 && dsc->prefix_group <= 1) s->step_cluster = arcb_session_step_ctas(e, B, dsc->t_max);
   cudaError_t r = cudaStreamCreateWithFlags(&s->capture_stream, cudaStreamNonBlocking);
   if (r != cudaSuccess) { delete s; return arcb_fail_cuda(r, "cudaStreamCreate"); }
   if (cudaEventCreate(&s->probe_begin) != cudaSuccess || cudaEventCreate(&s->probe_end) != cudaSuccess) {

@@ -122,6 +122,11 @@ class EngineBase:
                                                              _stream_ptr(self.device)))
         return int(n.value)
 
+    def step_ctas(self, n_seqs: int, t_max: int) -> int:
+        """CTAs of the one cluster that decode steps of such a session run in, 0 where they are separate launches."""
+        with torch.cuda.device(self.device):
+            return int(self.lib.arcb_session_step_ctas(self._handle, int(n_seqs), cache_row_pitch(t_max)))
+
     def new_session(self, n_seqs: int, t_max: int, max_new: int, max_prefill_tokens: int,
                     stop_on_end: bool = True, attn_splits: int = 0, forced: torch.Tensor | None = None,
                     want_step_logits: bool = False, out_tokens: torch.Tensor | None = None,

@@ -108,8 +108,9 @@ def generate_tokens(engine: Engine, ids: np.ndarray, pos: np.ndarray, mask: np.n
     which is what the reference does.
 
     ``samples`` > 1: that many rows for every prompt, row ``i samples + j`` the j-th of prompt i (``example_ids`` go by prompt,
-    ``forced`` and ``constraints`` by row).  A prompt is prefilled once, and the decode steps read its keys and values once for all
-    of its rows.
+    ``forced`` and ``constraints`` by row; no ``attn_splits``).  A prompt is prefilled once, and the decode steps read its keys and
+    values once for all of its rows.  Up to four rows of the smallest models, whose steps run in one cluster, hold copies of them
+    instead, which is quicker (256 wide, 4 layers, prompt of 190 tokens, 232 new ones: two samples 13 ms in place of 21).
     """
     dev = engine.device
     P, S = ids.shape
@@ -124,13 +125,15 @@ def generate_tokens(engine: Engine, ids: np.ndarray, pos: np.ndarray, mask: np.n
     t_max = int(lens.max()) + int(max_new)
     cap = int(min(max_prefill_tokens, int(lens.sum()) + 2 * P))
     cap = max(cap, int(lens.max()) + 2, B)
+    copied = False
     if session is None:
+        copied = samples > 1 and attn_splits <= 0 and engine.step_ctas(B, t_max) > 0
         session = engine.new_session(
             B, t_max, max_new, cap, stop_on_end=(2 if stop_on_end and not freeze_finished else stop_on_end),
             attn_splits=attn_splits,
             forced=None if forced is None else torch.from_numpy(np.ascontiguousarray(forced, dtype=np.int32)),
             want_step_logits=want_logits, constraints=constraints, temperature=temperature,
-            top_k=top_k or 0, sample_seed=sample_seed, prefix_group=samples if samples > 1 else 0)
+            top_k=top_k or 0, sample_seed=sample_seed, prefix_group=samples if samples > 1 and not copied else 0)
     elif session.prefix_group != (samples if samples > 1 else 0):
         raise ValueError("the session was made for another number of samples")
     ex_dev = None
@@ -155,6 +158,9 @@ def generate_tokens(engine: Engine, ids: np.ndarray, pos: np.ndarray, mask: np.n
             plan = plan.for_samples(samples)
         fl = None if first_logits is None else first_logits[int(rows[0]) * samples:(int(rows[-1]) + 1) * samples]     # consecutive rows
         session.prefill(plan, ex_dev, first_logits=fl)
+    if copied:
+        for i, n in enumerate(lens):
+            session.copy_rows(i * samples, int(n), range(i * samples + 1, (i + 1) * samples))
     if batch is not None:
         h2d += batch.h2d_bytes
     batch = plan = None             # their device memory (up to 33 bytes a padded position, 32 a token) is not kept through the steps
