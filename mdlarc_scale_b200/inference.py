@@ -134,7 +134,7 @@ def generate_tokens(engine: Engine, ids: np.ndarray, pos: np.ndarray, mask: np.n
             forced=None if forced is None else torch.from_numpy(np.ascontiguousarray(forced, dtype=np.int32)),
             want_step_logits=want_logits, constraints=constraints, temperature=temperature,
             top_k=top_k or 0, sample_seed=sample_seed, prefix_group=samples if samples > 1 and not copied else 0)
-    elif session.prefix_group != (samples if samples > 1 else 0):
+    elif max(session.prefix_group, 1) != samples:          # 0 and 1: every row holds its prompt
         raise ValueError("the session was made for another number of samples")
     ex_dev = None
     h2d = 0

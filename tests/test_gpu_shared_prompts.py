@@ -25,6 +25,25 @@ def test_a_number_of_splits_is_refused_not_ignored():
     eng.close()
 
 
+def test_groups_of_one_are_no_groups():
+    """prefix_group 0 and 1 say the same: every row holds its prompt."""
+    eng = engine(128, 64, 1)
+    ids, pos, mask, ex = batch(2, [5, 9])
+    tokens = []
+    for group in (0, 1):
+        session = eng.new_session(2, 32, 4, 64, stop_on_end=False, prefix_group=group)
+        tokens.append(generate_tokens(eng, ids, pos, mask, ex, 4, stop_on_end=False, session=session).tokens.clone())
+        with pytest.raises(ValueError):
+            generate_tokens(eng, ids[:1], pos[:1], mask[:1], ex[:1], 4, samples=2, session=session)
+        session.close()
+    assert torch.equal(*tokens)
+    session = eng.new_session(2, 32, 4, 64, prefix_group=2)
+    with pytest.raises(ValueError):
+        generate_tokens(eng, ids, pos, mask, ex, 4, session=session)
+    session.close()
+    eng.close()
+
+
 # models whose steps run in one cluster with so few rows, and ones whose do not
 @pytest.mark.parametrize("act", ["f16", "bf16"])
 @pytest.mark.parametrize("prompts,samples", [(1, 2), (1, 3), (1, 4), (2, 2), (2, 3)])
