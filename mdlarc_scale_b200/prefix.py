@@ -40,8 +40,8 @@ def prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, group_fi
     also sees rows ``[item_begin[i], item_end[i])`` of sequence ``item_seq[i]`` (by default sequence i from row 0).  The groups
     cover the items one after the other; without ``group_first`` nothing is shared, without ``item_end`` no item has rows
     of its own.  Indices are int32 tensors on the device, read when the kernels run.  ``skip`` (uint8) marks items that get
-    zeros, as those that see no row do.  The ``max_*`` are upper bounds of what the tensors hold and only plan the work, but
-    ``max_group``: no group may have more items.  ``status`` (int32, one value) becomes non-zero when an index is outside the
+    zeros, as those that see no row do.  The ``max_*`` are upper bounds of what the tensors hold (None: as many as there can be) and
+    only plan the work, but ``max_group``: no group may have more items.  ``status`` (int32, one value) becomes non-zero when an index is outside the
     cache.  Keys that an item sees are finite where half queries meet a bfloat16 cache (a query is a sum of two pieces there,
     which an infinity would turn into no number); what no item sees may hold anything.  The queries may be rows of a wider
     matrix; all else is contiguous.  Has no gradient, and refuses tensors that require one where it would be recorded.  Runs on the
@@ -89,7 +89,8 @@ def prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, group_fi
         if groups < 1 or group_seq is None or group_len is None:
             raise ValueError("groups need group_first, group_seq and group_len")
         first, seq, length = index(group_first, groups + 1, "group_first"), index(group_seq, groups, "group_seq"), index(group_len, groups, "group_len")
-    max_group, max_prefix, max_own = max_group or 0, max_prefix or 0, max_own or 0
+    # to the library 0 is a bound that is not known; one of no rows plans for as few as there can be
+    max_group, max_prefix, max_own = max_group or 0, 0 if max_prefix is None else max_prefix or 1, 0 if max_own is None else max_own or 1
     if max_group < 0 or max_prefix < 0 or max_own < 0:
         raise ValueError("max_group, max_prefix and max_own must not be negative")
     fields = (

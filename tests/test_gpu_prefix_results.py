@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from gpu_util import have_b200
-from mdlarc_scale_b200 import _lib, prefix_attention
+from mdlarc_scale_b200 import _lib, prefix, prefix_attention
 from test_gpu_prefix_attention import BF16, F16, F32, FORM_IDS, FORMS, Case
 
 pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not have_b200(), reason="needs a B200")]
@@ -112,3 +112,24 @@ def test_items_that_bad_groups_leave_out(form, sizes, heads, kv, prefix, plan, d
         prefix_attention(c.q, c.k, c.v, *c.groups, *(c.items if mine else ()), out=out, status=status, **hints)
         assert status.item() == 4
         c.check(out, mine=mine)
+
+
+@pytest.mark.parametrize("form", FORMS, ids=FORM_IDS)
+def test_bounds_of_no_rows(form, monkeypatch):
+    """0 rows is a bound, not an unknown one: the work is planned for as few as there can be, and what the tensors hold counts all the same."""
+    planned, attend = [], prefix._attend
+
+    def look(a, out, dev):
+        packed = _lib.PrefixAttentionArgs.from_buffer_copy(a)
+        planned.append((packed.max_group, packed.max_prefix, packed.max_own))
+        attend(a, out, dev)
+
+    monkeypatch.setattr(prefix, "_attend", look)
+    c = Case([3, 20], [300, 101], [i * 13 % 90 for i in range(23)], 4, 2, 64, form, 15)
+    for kw, want in ((dict(max_prefix=0, max_own=0), (0, 1, 1)), (dict(max_group=20, max_prefix=0), (20, 1, 0)), (dict(max_own=0), (0, 0, 1)), ({}, (0, 0, 0)),
+                     (dict(max_prefix=300, max_own=90), (0, 300, 90))):
+        c.check(c(**kw))
+        assert planned.pop() == want
+    for kw in (dict(max_prefix=-1), dict(max_own=-1), dict(max_group=-1)):
+        with pytest.raises(ValueError):
+            c(**kw)
