@@ -122,11 +122,11 @@ attn_prefix_join_cta_kernel(AttnPrefixArgs a) {
 
 void fill_plan(AttnPrefixArgs& a) {
   a.rep = a.n_heads / a.n_kv;
-  // tcgen05 from 512 shared rows on (64 queries of 4 heads, 8 groups: 60.2 us with it and 58.4 without at 384 rows, 63.8 and 70.7 at 1024;
-  // 24 queries 26.0 and 28.4 at 600); half queries over bfloat16, whose products are three, from 2048 on (128 query rows: 72 us and 66 at
-  // 1500, 77.5 and 86.6 at 3000).
+  // tcgen05 from 640 shared rows on (64 items of 4 heads, 8 groups: 51.5 us with it and 48.2 without at 512 rows, 52.7 and 52.4 at 640, 56.1
+  // and 60.8 at 768, 61.4 and 67.0 at 1024; 24 items 29.9 and 29.7 at 600, 32.4 and 37.0 at 768); half queries over bfloat16, whose scores
+  // take two products, from 2048 on (128 items of 20 heads: 39.5 us and 36.8 at 1500, 41.1 and 40.9 at 2100, 44.3 and 45.1 at 3000).
   const bool split = a.act_fmt != a.kv_fmt;
-  const bool tc = a.kv_fmt != 2 && (!split || a.dim == 64) && a.scale != 0.f && a.max_prefix >= (split ? 2048 : 512);
+  const bool tc = a.kv_fmt != 2 && (!split || a.dim == 64) && a.scale != 0.f && a.max_prefix >= (split ? 2048 : 640);
   a.plan = prefix_plan(a.n_groups, a.max_group, a.max_prefix, a.n_items, a.item_end ? a.max_own : 0, a.n_kv, a.rep, a.dim, a.kv_fmt == 2, tc, arcb_num_sms());
 }
 

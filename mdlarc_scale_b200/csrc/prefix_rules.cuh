@@ -47,10 +47,10 @@ inline PrefixPart prefix_part(long long heads, long long rows, int n_kv, bool wi
   return p;
 }
 // Ranges for `rows` cached rows where every slot of the GPU has `each` rows to read.  Up to 1024, what runs at once gets one range each,
-// rounded so that no few are left for a second wave (64 items x 8 key heads of 500 rows in three ranges for 1776 warps: 51 us with
-// all that goes with it, 55 in four).  Above, up to four a slot, so that lengths that differ even out, none under 1024 rows: five
-// tokens of 24 sequences over 4096 rows in four ranges 76 us, in eight 84; 33 items of 777 rows at most in one 122, in four 142; but
-// eight samples over 1193 rows, 1280 units, in two 127 and in one 129.
+// rounded so that no few are left for a second wave (64 items x 8 key heads of 500 rows in three ranges for 1776 warps: 60 us with
+// all that goes with it, 66 in four).  Above, up to four a slot, so that lengths that differ even out, none under 1024 rows: five
+// tokens of 24 sequences over 4096 rows in four ranges 76 us, in eight 84; 33 items of 777 rows at most in one 133, in four 153; but
+// eight samples over 1193 rows, 1280 units, in two 124 and in one 125.
 inline int prefix_cut(long long rows, long long each, long long least, long long most) {
   const long long fewest = (rows + least - 1) / least;
   const long long s = each <= 1024 ? rows / std::max(1LL, each) : (rows + std::max(1024LL, each / 4) - 1) / std::max(1024LL, each / 4);

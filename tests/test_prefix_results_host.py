@@ -21,7 +21,7 @@ extern "C" int rows(int begin, int end, int seq, int n_seqs, int t_max) { return
 """
 LEAST, MOST = -2 ** 31, 2 ** 31 - 1
 # groups, items of each, key heads, heads of a key head, dim, shared rows: units enough for one range each, no rows of the items' own
-ONE_RANGE = [(64, 32, 8, 4, 128, 2048), (8, 64, 8, 4, 128, 1024), (20, 66, 20, 1, 64, 512), (1, 256, 32, 4, 128, 700)]
+ONE_RANGE = [(64, 32, 8, 4, 128, 2048), (8, 64, 8, 4, 128, 1024), (20, 66, 20, 1, 64, 640), (1, 256, 32, 4, 128, 700)]
 
 
 @pytest.fixture(scope="module")
