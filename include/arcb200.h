@@ -404,9 +404,11 @@ int arcb_session_step_logits(arcb_session* s, float** d_logits, int32_t* pitch);
 int arcb_session_finished(arcb_session* s, int32_t* h_finished, void* stream);
 
 /* Copies what sequence src holds to the sequences h_dst[n_dst] (host memory, free when the call returns): keys, values or latents of its
- * first `rows` positions and, on layered engines, recurrent states and the position it continues at, so that `rows` is its
- * length there.  The targets then continue from there; what they have produced and whether they are armed stays theirs.  Not in
- * sessions with prefix_group > 1, whose rows do not hold their prompts. */
+ * first `rows` positions.  On layered engines recurrent states and the position it continues at go with them, so that `rows` is its
+ * length there and the targets continue from there; what they have produced and whether they are armed stays theirs.  In grid
+ * sessions positions and current tokens stay the targets': these are what arcb_prefill made them, as for samples of a prompt that
+ * is prefilled into src with the targets among its d_first_seq.  Not in sessions with prefix_group > 1, whose rows do not hold their
+ * prompts. */
 int arcb_session_fork(arcb_session* s, int32_t src, int32_t rows, const int32_t* h_dst, int32_t n_dst, void* stream);
 
 /* Synchronises `stream`, then reports how many rows have emitted END and the

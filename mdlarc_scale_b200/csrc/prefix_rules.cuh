@@ -94,8 +94,8 @@ inline PrefixPlan prefix_plan(long long n_groups, long long max_group, long long
     }
   }
   // A CTA of eight warps for a whole group, a warp a range or an item, where no warp gets more than 64 rows and no SM a second CTA:
-  // as fast on the device (two samples of a prompt of 190 rows: 7.6 us, 7.9 in two launches) and a launch and its scratch less on
-  // the host (13 us a call in place of 19).  With a second unit for some of the warps it is slower (eight samples: 10.8 us, 7.9).
+  // two samples of a prompt of 190 rows 5.8 us, 8.2 in two launches, four 6.2 and 8.3, and a launch and its scratch less on
+  // the host (a call of two samples 13 us in place of 19).  With a second unit for some of the warps it was slower (eight samples: 10.8 us, 7.9).
   const long long ranges = AP_GROUP_WARPS - max_group;
   if (p.together && p.shared.kernel == AP_ROWS && p.shared.tiles == 1 && n_groups * n_kv <= sms && max_prefix <= 64 * ranges && max_own <= 64) {
     p.grouped = 1;

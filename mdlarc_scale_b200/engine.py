@@ -334,7 +334,8 @@ class Session:
             _lib.check(self.eng.lib.arcb_prefill(self._handle, C.byref(a), _stream_ptr(self.eng.device)))
 
     def copy_rows(self, src: int, rows: int, targets) -> None:
-        """What sequence ``src`` holds at its first ``rows`` positions, for the sequences ``targets`` as well."""
+        """What sequence ``src`` holds at its first ``rows`` positions, for the sequences ``targets`` as well.  In grid sessions the targets'
+        positions and current tokens stay theirs."""
         dst = np.ascontiguousarray(targets, dtype=np.int32).reshape(-1)
         with torch.cuda.device(self.eng.device):
             _lib.check(self.eng.lib.arcb_session_fork(self._handle, int(src), int(rows), dst.ctypes.data, len(dst), _stream_ptr(self.eng.device)))
