@@ -7,6 +7,7 @@
 namespace {
 
 constexpr float AP_LOG2E = 1.4426950408889634f;
+constexpr int AP_LOOK_BACK = 4096;      // groups whose ends a bad one looks at
 
 // Launch with the programmatic attribute: the kernel's CTAs may come when all of the kernel ahead have started.
 template <typename... KArgs, typename... Args>
@@ -91,16 +92,20 @@ __device__ __forceinline__ ApWork ap_work(const AttnPrefixArgs& a, long long blo
                      (len > 0 && (k.seq < 0 || k.seq >= a.n_seqs)) || (g == 0 && first != 0) || (g == a.n_groups - 1 && last != a.n_items);
     k.behind = 0;
     if (bad) {
-      // Its items see no shared rows.  They are those between its ends, of which one that is no item's counts as the one ahead of it, the
-      // first of all as 0 and the last as n_items: from one group to the next these ends leave no item out, whatever they are.
+      // Its items see no shared rows.  They begin at the largest end of the groups ahead of it and end at its own, n_items if it is the last
+      // group; ends outside the items count for nothing.  So no item is left out, whatever the ends are: going from group to group, the
+      // largest end so far rises from 0 to n_items.  One that is further back than the loop goes only makes an item a bad group's too.
       if (report) arcb_set_error(a.status, ARCB_DEV_BAD_INDEX);
       if (a.uniform <= 0) {
-        for (int i = g; i >= 0; --i) {
-          first = i == 0 ? 0 : a.group_first[i];
-          if (first >= 0 && first <= a.n_items) break;
-        }
         if (g == a.n_groups - 1) last = a.n_items;
-        else if (last < first || last > a.n_items) last = first;
+        first = 0;
+        if (last >= 0 && last <= a.n_items) {
+          for (int i = max(1, g - AP_LOOK_BACK); i <= g; ++i) {
+            const int end = a.group_first[i];
+            if (end <= a.n_items) first = max(first, end);
+          }
+        }
+        if (last < first || last > a.n_items) last = first;
       }
       len = 0;
       if (last - first > a.max_group) {

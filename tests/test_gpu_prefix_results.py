@@ -133,3 +133,23 @@ def test_bounds_of_no_rows(form, monkeypatch):
     for kw in (dict(max_prefix=-1), dict(max_own=-1), dict(max_group=-1)):
         with pytest.raises(ValueError):
             c(**kw)
+
+
+@pytest.mark.parametrize("form", [(F16, BF16), (F32, F32)], ids=["f16-bf16", "f32"])
+@pytest.mark.parametrize("value", [-7, 2 ** 31 - 1, -2 ** 31, 0, 201])
+@pytest.mark.parametrize("kept", [0, 100])
+def test_ends_that_are_all_wrong(form, value, kept):
+    """Two thousand groups whose ends, but the first ones, are no items': the groups ahead of them have theirs, all other items their own rows."""
+    groups, n = 2000, 200
+    sizes = [1] * n + [0] * (groups - n)
+    c = Case(sizes, [20] * n + [0] * (groups - n), [i % 5 for i in range(n)], 2, 1, 64, form, seed=kept)
+    c.groups[0][kept + 1:] = value
+    c.prefix = [20 if i < kept else 0 for i in range(groups)]
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    hints = dict(max_group=1, max_prefix=20, max_own=5)
+    for mine in (True, False):
+        status.zero_()
+        out = dirty(c, **hints)
+        prefix_attention(c.q, c.k, c.v, *c.groups, *(c.items if mine else ()), out=out, status=status, **hints)
+        assert status.item() == 4
+        c.check(out, mine=mine)
